@@ -570,6 +570,59 @@ int mcn_l2reg_cost(const float* ground, const float* data, float* output, int nu
 int mcn_l2reg_grad(const float* ground, const float* data, float* target, int numD, int numCases, int add,
                    float coeff, void* stream);
 
+/* ---- the head of a classifier over many classes (no counterpart in the reference, which has neither layer norm nor dropout --
+ * its DeepID definitions carry a dropout key that no parser reads -- and keeps the logits of every class) ------------------- */
+/* Layer norm over the features of each case: inputs, target (numFeatures, numCases); gains, biases (numFeatures, may be NULL: 1 / 0);
+ *   target[f,n] = gains[f] * (inputs[f,n] - mean[n]) * r[n] + biases[f],  r = 1 / sqrt(var + eps), var over numFeatures, eps > 0.
+ * caseStats (2, numCases): the means, then r, for mcn_layer_norm_undo (may be NULL).  target may be inputs itself.  Sizes up to
+ * 2^28 each.  Calls that run at the same time need a workspace each; so do graphs that are replayed at the same time. */
+size_t mcn_layer_norm_workspace_bytes(int numFeatures, int numCases);
+int mcn_layer_norm(const float* inputs, const float* gains, const float* biases, float* target, float* caseStats, int numFeatures,
+                   int numCases, float eps, void* workspace, size_t workspaceBytes, void* stream);
+/* Its gradients, from outGrads (numFeatures, numCases), the inputs of the forward call and the caseStats it left; every output may
+ * be NULL (not wanted), but not all of them:
+ *   target (numFeatures, numCases) = scaleTargets*target + scaleOutput * d/d inputs,
+ *   gainGrads, biasGrads (numFeatures) = scale{Gain,Bias}Targets * old + scale{Gain,Bias}Output * d/d gains, biases.
+ * The target is neither outGrads nor inputs. */
+size_t mcn_layer_norm_undo_workspace_bytes(int numFeatures, int numCases);
+int mcn_layer_norm_undo(const float* outGrads, const float* inputs, const float* gains, const float* caseStats, float* target,
+                        float* gainGrads, float* biasGrads, int numFeatures, int numCases, float scaleTargets, float scaleOutput,
+                        float scaleGainTargets, float scaleGainOutput, float scaleBiasTargets, float scaleBiasOutput,
+                        void* workspace, size_t workspaceBytes, void* stream);
+/* Dropout: target[e] = scaleTargets*target[e] + (kept(e) ? scaleOutput * inputs[e] / (1 - dropProb) : 0), 0 <= dropProb < 1.  The
+ * mask is never stored: kept(e) follows from (seed, step, e) by a counter-based generator (Philox-4x32, ten rounds: counter
+ * (e / 4, step), key seed, word e % 4, kept when that is at least floor(dropProb * 2^32)), so the gradient is the same call with
+ * the same seed and step on the output's gradient.  Every call of a run takes a step of its own; layers and ranks differ in their
+ * seed.  deviceStep (device memory, may be NULL) is added to step when the kernel runs, so that replays of a captured graph draw new
+ * masks: advance it with mcn_counter_add.  target may be inputs itself; otherwise the two do not overlap. */
+int mcn_dropout(const float* inputs, float* target, size_t numElements, float dropProb, uint64_t seed, uint64_t step,
+                const uint64_t* deviceStep, float scaleTargets, float scaleOutput, void* stream);
+/* *counter += by, on the stream (counter: 8 bytes of device memory) */
+int mcn_counter_add(uint64_t* counter, uint64_t by, void* stream);
+/* FCLayer::fpropActs + SoftmaxLayer::fpropActs + LogregCostLayer::fpropActs (layer.cu:355-360,585-595,969-981) for layers of many
+ * classes, without the (numOutputs, numCases) matrices of logits and probabilities that mcn_gemm_bias_neuron_softmax_part and
+ * mcn_softmax_logreg_cost keep: weights (numOutputs x numInputs, row-major = the layer's own image), inputs (numInputs, numCases),
+ * biases (numOutputs, may be NULL; -inf takes a class out), labels (numCases).  A case whose label is not in [0, numOutputs) does not
+ * count: zero log probability, zero correct, zero gradient.  With z = weights * inputs + biases, per case
+ *   caseStats (2, numCases) = max_v z, then sum_v exp(z - max);  labelLogProbs = log p[label];
+ *   correctProbs = (z[label] is the max) / (number of entries at the max);
+ *   costOut (device doubles, may be NULL): [0] += -sum(labelLogProbs), [1] += cases that count - sum(correctProbs).
+ * A case all of whose classes are -inf has statistics (-inf, 0), log probability -inf and no gradient.  numOutputs up to 2^24 (labels
+ * are fp32), numInputs and numCases up to 2^20.  Workspaces as for mcn_layer_norm; backward != 0: for both calls, 0: the cost alone. */
+size_t mcn_fc_logreg_workspace_bytes(int numInputs, int numOutputs, int numCases, int backward);
+int mcn_fc_logreg_cost(const float* weights, const float* inputs, const float* biases, const float* labels, float* caseStats,
+                       float* labelLogProbs, float* correctProbs, int numInputs, int numOutputs, int numCases, double* costOut,
+                       void* workspace, size_t workspaceBytes, void* stream);
+/* The gradients, given the caseStats that mcn_fc_logreg_cost left for the same operands.  With dz = coeff * ((v == label) - p)
+ * (the sign of computeLogregSoftmaxGrad, layer_kernels.cu:287-308), computed again in pieces of the classes, each output may be NULL:
+ *   inputGrads (numInputs, numCases) = scaleInputTargets*inputGrads + weights^T dz,
+ *   weightGrads (as weights) = scaleWeightTargets*weightGrads + scaleWeightOutput * dz inputs^T,
+ *   biasGrads (numOutputs) = scaleBiasTargets*biasGrads + scaleBiasOutput * (row sums of dz). */
+int mcn_fc_logreg_grad(const float* weights, const float* inputs, const float* biases, const float* labels, const float* caseStats,
+                       float* inputGrads, float* weightGrads, float* biasGrads, int numInputs, int numOutputs, int numCases,
+                       float coeff, float scaleInputTargets, float scaleWeightTargets, float scaleWeightOutput,
+                       float scaleBiasTargets, float scaleBiasOutput, void* workspace, size_t workspaceBytes, void* stream);
+
 /* ---- weights.cuh:150-163 --------------------------------------------------------------------- */
 /* Weights::update in one pass: useGrad: inc = mom*inc + grad; wc>0: inc -= wc*eps*W; W += inc. */
 int mcn_sgd_update(float* W, float* inc, const float* grad, size_t n, float mom, float wc, float eps,

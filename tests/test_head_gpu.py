@@ -1,0 +1,537 @@
+"""Layer norm, dropout and the classifier cost without a logits matrix, against plain float64 implementations.
+
+Tolerances: u = 2^-24 is the largest relative rounding error of one fp32 operation.  A sum of k products of relative errors at most
+u each, in any order, is off by at most k u sum|terms| and, with errors of either sign, by LAMBDA sqrt(k) u sum|terms| but for a
+negligible share of inputs (Higham and Mary, "A new approach to probabilistic rounding error analysis", 2019; LAMBDA = 8)."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from kutil import call, capi, dev, dev_double, ws_bytes
+
+U = 2.0 ** -24
+LAMBDA = 8
+EPS = 1e-5
+TAIL = 64  # floats behind every output that no kernel may touch
+MARK = np.float32(1234.5)
+
+
+class Out(capi.DeviceBuffer):
+    """An output of `shape` filled with NaN (write-only outputs must not read it), or with `start`, with marks behind it."""
+
+    def __init__(self, shape, start=None):
+        self.want, self.count = shape, int(np.prod(shape))
+        a = np.full(self.count + TAIL, MARK, np.float32)
+        a[:self.count] = np.nan if start is None else np.asarray(start, np.float32).ravel()
+        super().__init__(array=a)
+
+    def get(self):
+        a = self.numpy()
+        assert np.all(a[self.count:] == MARK), 'wrote behind the end'
+        return a[:self.count].reshape(self.want).copy()
+
+
+def within(got, want, bound, what):
+    got = got.astype(np.float64)
+    bound = np.broadcast_to(bound, want.shape)
+    assert np.array_equal(np.isfinite(got), np.isfinite(want)), what
+    f = np.isfinite(want)
+    err = np.abs(got[f] - want[f])
+    bad = err > bound[f]
+    assert not bad.any(), '%s: %d of %d off, worst %.3g over a bound of %.3g' % (
+        what, bad.sum(), bad.size, err[bad].max(), bound[f][bad][np.argmax(err[bad])])
+
+
+def sum_err(k):
+    return min(k, LAMBDA * np.sqrt(k)) * U
+
+
+def need(name, *a):
+    b = ws_bytes(name, *a)
+    return capi.DeviceBuffer(nbytes=max(b, 16)), b
+
+
+# ------------------------------------------------------------------------------------------------------------- layer norm
+def norm_ref(x, gain, bias):
+    mean = x.mean(0)
+    var = ((x - mean) ** 2).mean(0)
+    r = 1 / np.sqrt(var + EPS)
+    return gain[:, None] * ((x - mean) * r) + bias[:, None], mean, r
+
+
+def norm_bounds(x, gain, bias, mean, r):
+    """Error of the mean, relative error of r, error of y."""
+    f = x.shape[0]
+    amax = np.abs(x).max(0)
+    e_mean = sum_err(f) * np.abs(x).mean(0) + 4 * U * amax
+    # var: deviations off by e_mean and 2u each, squares summed; r has half of var's relative error
+    dev_rms = np.sqrt(((x - mean) ** 2).mean(0))
+    e_r = 0.5 * (sum_err(f) + 8 * U + (2 * e_mean * dev_rms + e_mean ** 2 + 2 * U * amax * dev_rms) * r ** 2) + 4 * U
+    xh = np.abs((x - mean) * r)
+    e_xh = (e_mean + 2 * U * amax) * r + xh * (e_r + 4 * U)
+    return e_mean, e_r, np.abs(gain)[:, None] * (e_xh + 2 * U * xh) + 2 * U * (np.abs(gain[:, None]) * xh + np.abs(bias)[:, None]), e_xh
+
+
+def norm_data(f, n, seed, offset=2.0):
+    rng = np.random.default_rng(seed)
+    x = (rng.standard_normal((f, n)) * (0.5 + 2 * rng.random(n)) + rng.standard_normal(n) * offset).astype(np.float32)
+    gain = (1 + 0.2 * rng.standard_normal(f)).astype(np.float32)
+    bias = (0.2 * rng.standard_normal(f)).astype(np.float32)
+    return x, gain, bias, rng.standard_normal((f, n)).astype(np.float32)
+
+
+NORM_SHAPES = [(1, 1), (1, 5), (2, 1), (3, 64), (5, 3), (16, 16), (63, 65), (64, 4), (160, 128), (160, 37), (257, 12), (512, 1),
+               (512, 128), (1000, 31), (1025, 8), (2048, 20), (2049, 64), (4096, 36), (4097, 16), (9075, 5), (9075, 128), (40000, 1),
+               (20000, 4), (33, 5000), (128, 3000), (7, 20001)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('f,n', NORM_SHAPES)
+def test_layer_norm(f, n):
+    x, gain, bias, _ = norm_data(f, n, f * 131 + n)
+    want, mean, r = norm_ref(x.astype(np.float64), gain.astype(np.float64), bias.astype(np.float64))
+    e_mean, e_r, e_y, _ = norm_bounds(x.astype(np.float64), gain, bias, mean, r)
+    y, st = Out((f, n)), Out((2, n))
+    ws, size = need('mcn_layer_norm_workspace_bytes', f, n)
+    dx, dg, db = dev(x), dev(gain), dev(bias)
+    call('mcn_layer_norm', dx, dg, db, y, st, f, n, EPS, ws, size, None)
+    got, stats = y.get(), st.get()
+    within(stats[0], mean, e_mean, 'mean')
+    within(stats[1], r, e_r * r, 'r')
+    within(got, want, e_y, 'y')
+    # without gains, biases and statistics, in place, and at an address that is not 16-byte aligned
+    z = Out((f * n + 1,), np.concatenate([[0], x.ravel()]))
+    call('mcn_layer_norm', z.ptr + 4, None, None, z.ptr + 4, None, f, n, EPS, ws, size, None)
+    one, zero = np.ones(f), np.zeros(f)
+    want1, _, _ = norm_ref(x.astype(np.float64), one, zero)
+    within(z.get()[1:].reshape(f, n), want1, norm_bounds(x.astype(np.float64), one, zero, mean, r)[2], 'y in place')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('offset', [1e3, 1e5])
+def test_layer_norm_far_from_zero(offset):
+    """Large means: a variance formed as a difference of two large sums would lose everything."""
+    x, gain, bias, _ = norm_data(700, 24, 5, offset)
+    x64 = x.astype(np.float64)
+    want, mean, r = norm_ref(x64, gain.astype(np.float64), bias.astype(np.float64))
+    y, st = Out((700, 24)), Out((2, 24))
+    ws, size = need('mcn_layer_norm_workspace_bytes', 700, 24)
+    keep = dev(x), dev(gain), dev(bias)
+    call('mcn_layer_norm', *keep, y, st, 700, 24, EPS, ws, size, None)
+    within(y.get(), want, norm_bounds(x64, gain, bias, mean, r)[2], 'y')
+
+
+@pytest.mark.gpu
+def test_layer_norm_one_bad_case_stays_alone():
+    """An infinity or NaN in one case changes that case only; a constant case gives the biases."""
+    x, gain, bias, _ = norm_data(300, 40, 9)
+    x[7, 3], x[8, 11], x[:, 20] = np.inf, np.nan, 3.25
+    y = Out((300, 40))
+    ws, size = need('mcn_layer_norm_workspace_bytes', 300, 40)
+    keep = dev(x), dev(gain), dev(bias)
+    call('mcn_layer_norm', *keep, y, None, 300, 40, EPS, ws, size, None)
+    got = y.get()
+    assert not np.isfinite(got[:, 11]).any() and not np.isfinite(got[7, 3])
+    fine = [c for c in range(40) if c not in (3, 11)]
+    want, mean, r = norm_ref(x[:, fine].astype(np.float64), gain.astype(np.float64), bias.astype(np.float64))
+    within(got[:, fine], want, norm_bounds(x[:, fine].astype(np.float64), gain, bias, mean, r)[2], 'the other cases')
+
+
+def undo_ref(g, x, gain, mean, r):
+    h, xh = gain[:, None] * g, (x - mean) * r
+    return r * (h - h.mean(0) - xh * (h * xh).mean(0)), (g * xh).sum(1), g.sum(1)
+
+
+def undo_bounds(g, x, gain, bias, mean, r):
+    f, n = x.shape
+    _, e_r, _, e_xh = norm_bounds(x, gain, bias, mean, r)
+    h, xh = gain[:, None] * g, (x - mean) * r
+    e_m1 = (sum_err(f) + 4 * U) * np.abs(h).mean(0)
+    e_m2 = (sum_err(f) + 6 * U) * np.abs(h * xh).mean(0) + (np.abs(h) * e_xh).mean(0)
+    m2 = np.abs((h * xh).mean(0))
+    mag = np.abs(h) + np.abs(h.mean(0)) + np.abs(xh) * m2
+    e_dx = r * (e_m1 + np.abs(xh) * e_m2 + e_xh * m2 + 6 * U * mag + e_r * mag)
+    e_dg = (sum_err(n) + 4 * U) * np.abs(g * xh).sum(1) + (np.abs(g) * e_xh).sum(1)
+    return e_dx, e_dg, (sum_err(n) + 2 * U) * np.abs(g).sum(1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('f,n', NORM_SHAPES)
+def test_layer_norm_undo(f, n):
+    x, gain, bias, g = norm_data(f, n, f * 17 + n)
+    X, G, g64 = x.astype(np.float64), gain.astype(np.float64), g.astype(np.float64)
+    _, mean, r = norm_ref(X, G, bias.astype(np.float64))
+    wx, wg, wb = undo_ref(g64, X, G, mean, r)
+    ex, eg, eb = undo_bounds(g64, X, G, bias, mean, r)
+    st = Out((2, n), np.stack([mean, r]))
+    dx, dg, db = Out((f, n)), Out((f,)), Out((f,))
+    ws, size = need('mcn_layer_norm_undo_workspace_bytes', f, n)
+    kg, kx, ka = dev(g), dev(x), dev(gain)
+    call('mcn_layer_norm_undo', kg, kx, ka, st, dx, dg, db, f, n, 0.0, 1.0, 0.0, 1.0, 0.0, 1.0, ws, size, None)
+    first = dx.get(), dg.get(), db.get()
+    within(first[0], wx, ex, 'dx')
+    within(first[1], wg, eg, 'dgain')
+    within(first[2], wb, eb, 'dbias')
+    # again: the same bits
+    call('mcn_layer_norm_undo', kg, kx, ka, st, dx, dg, db, f, n, 0.0, 1.0, 0.0, 1.0, 0.0, 1.0, ws, size, None)
+    for a, b in zip(first, (dx.get(), dg.get(), db.get())):
+        assert np.array_equal(a, b)
+    # added onto what is there, scaled; then each output alone
+    t, tg, tb = (np.random.default_rng(1).standard_normal(s).astype(np.float32) for s in ((f, n), (f,), (f,)))
+    dx, dg, db = Out((f, n), t), Out((f,), tg), Out((f,), tb)
+    call('mcn_layer_norm_undo', kg, kx, ka, st, dx, dg, db, f, n, 1.0, 0.5, 0.9, -0.25, 0.5, 2.0, ws, size, None)
+    within(dx.get(), t + 0.5 * wx, 0.5 * ex + 4 * U * (np.abs(t) + np.abs(wx)), 'dx added')
+    within(dg.get(), 0.9 * tg - 0.25 * wg, 0.25 * eg + 4 * U * (np.abs(tg) + np.abs(wg)), 'dgain added')
+    within(db.get(), 0.5 * tb + 2 * wb, 2 * eb + 4 * U * (np.abs(tb) + 2 * np.abs(wb)), 'dbias added')
+    for k in range(3):
+        outs = [Out((f, n)), Out((f,)), Out((f,))]
+        args = [o if i == k else None for i, o in enumerate(outs)]
+        call('mcn_layer_norm_undo', kg, kx, ka, st, *args, f, n, 0.0, 1.0, 0.0, 1.0, 0.0, 1.0, ws, size, None)
+        assert np.array_equal(outs[k].get(), first[k])
+    # no gains; operands that are not 16-byte aligned
+    ug, ux = dev(np.concatenate([[0], g.ravel()])), dev(np.concatenate([[0], x.ravel()]))
+    dx = Out((f * n + 1,))
+    call('mcn_layer_norm_undo', ug.ptr + 4, ux.ptr + 4, None, st, dx.ptr + 4, None, None, f, n, 0.0, 1.0, 0.0, 1.0, 0.0, 1.0, ws, size, None)
+    one = np.ones(f)
+    within(dx.get()[1:].reshape(f, n), undo_ref(g64, X, one, mean, r)[0], undo_bounds(g64, X, one, bias, mean, r)[0], 'dx, no gains')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('f,n', [(24, 7), (130, 16)])
+def test_layer_norm_undo_against_differences(f, n):
+    """d sum(g y) along random directions, central differences of the float64 formula.
+
+    Differences: step 1e-4, error O(step^2) times third derivatives of order one: 1e-6 of the sum of magnitudes is ample."""
+    x, gain, bias, g = norm_data(f, n, 3)
+    X, G, B = (a.astype(np.float64) for a in (x, gain, bias))
+    _, mean, r = norm_ref(X, G, B)
+    outs = Out((f, n)), Out((f,)), Out((f,))
+    st = Out((2, n), np.stack([mean, r]))
+    ws, size = need('mcn_layer_norm_undo_workspace_bytes', f, n)
+    keep = dev(g), dev(x), dev(gain)
+    call('mcn_layer_norm_undo', *keep, st, *outs, f, n, 0.0, 1.0, 0.0, 1.0, 0.0, 1.0, ws, size, None)
+    got = [o.get().astype(np.float64) for o in outs]
+    bounds = undo_bounds(g.astype(np.float64), X, G, B, mean, r)
+    rng = np.random.default_rng(4)
+    for k in range(3):
+        d = [np.zeros_like(X), np.zeros_like(G), np.zeros_like(B)]
+        d[k] = rng.standard_normal(d[k].shape)
+        h = 1e-4
+        value = lambda s: (g * norm_ref(X + s * d[0], G + s * d[1], B + s * d[2])[0]).sum()  # noqa: E731
+        want = (value(h) - value(-h)) / (2 * h)
+        assert abs((got[k] * d[k]).sum() - want) <= (bounds[k] * np.abs(d[k])).sum() + 1e-6 * (np.abs(got[k] * d[k])).sum()
+
+
+# ------------------------------------------------------------------------------------------------------------- dropout
+def philox_words(count, seed, step, first_quad=0):
+    """Philox-4x32, ten rounds, in Python integers' width by uint64 arithmetic."""
+    low, quads = np.uint64(0xFFFFFFFF), (count + 3) // 4
+    q = np.arange(quads, dtype=np.uint64) + np.uint64(first_quad)
+    c = [q & low, q >> np.uint64(32), np.full_like(q, step & 0xFFFFFFFF), np.full_like(q, step >> 32)]
+    k = [seed & 0xFFFFFFFF, seed >> 32]
+    for _ in range(10):
+        a, b = c[0] * np.uint64(0xD2511F53), c[2] * np.uint64(0xCD9E8D57)
+        c = [(b >> np.uint64(32)) ^ c[1] ^ np.uint64(k[0]), b & low, (a >> np.uint64(32)) ^ c[3] ^ np.uint64(k[1]), a & low]
+        k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+    return np.stack(c, 1).astype(np.uint32).ravel()[:count]
+
+
+def kept(count, p, seed, step):
+    return philox_words(count, seed, step).astype(np.uint64) >= np.uint64(int(float(np.float32(p)) * 2.0 ** 32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n', [1, 3, 4, 5, 1023, 20480, 4213 * 37, 1 << 20])
+@pytest.mark.parametrize('p', [0.0, 0.4, 0.999])
+def test_dropout(n, p):
+    rng = np.random.default_rng(n)
+    x = rng.standard_normal(n).astype(np.float32)
+    seed, step = (0xDEADBEEF << 32) + n, (5 << 32) + 17
+    keep = kept(n, p, seed, step)
+    scale = 1 / (1 - float(np.float32(p)))
+    want = np.where(keep, x * scale, 0.0)
+    y, dx = Out((n,)), dev(x)
+    call('mcn_dropout', dx, y, n, p, seed, step, None, 0.0, 1.0, None)
+    got = y.get()
+    assert np.array_equal(got != 0, keep & (x != 0))
+    within(got, want, 2 * U * np.abs(want), 'y')
+    # in place, and at an address that is not 16-byte aligned: the same bits
+    z = Out((n + 1,), np.concatenate([[0], x]))
+    call('mcn_dropout', z.ptr + 4, z.ptr + 4, n, p, seed, step, None, 0.0, 1.0, None)
+    assert np.array_equal(z.get()[1:], got)
+    # added onto what is there; step given in parts, one of them in device memory
+    t = rng.standard_normal(n).astype(np.float32)
+    y = Out((n,), t)
+    counter = capi.DeviceBuffer(array=np.array([step - 20], np.uint64))
+    call('mcn_counter_add', counter.ptr, 9, None)
+    call('mcn_dropout', dx, y, n, p, seed, 11, counter.ptr, 0.5, -2.0, None)
+    within(y.get(), 0.5 * t - 2 * want, 4 * U * (np.abs(t) + 2 * np.abs(want)), 'added')
+
+
+@pytest.mark.gpu
+def test_dropout_masked_places_do_not_come_through():
+    n, p = 4096, 0.5
+    keep = kept(n, p, 7, 9)
+    x = np.where(keep, 1.0, np.nan).astype(np.float32)
+    x[~keep & (np.arange(n) % 3 == 0)] = np.inf
+    y, dx = Out((n,)), dev(x)
+    call('mcn_dropout', dx, y, n, p, 7, 9, None, 0.0, 1.0, None)
+    assert np.array_equal(y.get(), np.where(keep, np.float32(2), np.float32(0)))
+
+
+@pytest.mark.gpu
+def test_dropout_statistics():
+    """Share kept: 2^20 draws of probability 0.6 have a standard deviation of 5e-4 of the share; five of them are allowed.  Masks of
+    neighbouring steps and seeds agree on a share of 0.6^2 + 0.4^2 = 0.52, likewise."""
+    n = 1 << 20
+    one = dev(np.ones(n, np.float32))
+    masks = []
+    for seed, step in ((1, 1), (1, 2), (2, 1)):
+        y = Out((n,))
+        call('mcn_dropout', one, y, n, 0.4, seed, step, None, 0.0, 1.0, None)
+        masks.append(y.get() != 0)
+        assert abs(masks[-1].mean() - 0.6) < 2.5e-3
+    for a, b in ((0, 1), (0, 2), (1, 2)):
+        assert abs((masks[a] == masks[b]).mean() - 0.52) < 2.5e-3
+
+
+# ------------------------------------------------------------------------------------------------------------- classifier cost
+def fcl_data(d, v, n, seed, masked=0.0, padded=0, lean=6.0):
+    rng = np.random.default_rng(seed)
+    w = (rng.standard_normal((v, d)) / np.sqrt(d)).astype(np.float32)
+    labels = rng.integers(v, size=n)
+    x = (rng.standard_normal((d, n)) + lean * rng.random(n) * w[labels].T).astype(np.float32)
+    b = (0.1 * rng.standard_normal(v)).astype(np.float32)
+    if masked:
+        hide = rng.random(v) < masked
+        hide[labels] = False
+        b[hide] = -np.inf
+    lab = labels.astype(np.float32)
+    if padded:
+        lab[n - padded:] = -1
+    return w, x, b, lab
+
+
+def fcl_ref(w, x, b, lab, coeff):
+    w, x, b = (a.astype(np.float64) for a in (w, x, b))
+    v, n = w.shape[0], x.shape[1]
+    z = w @ x + b[:, None]
+    top = z.max(0)
+    e = np.exp(z - top)
+    tot = e.sum(0)
+    ok = (lab >= 0) & (lab < v)
+    li = np.where(ok, lab, 0).astype(int)
+    at = z[li, np.arange(n)]
+    logp = np.where(ok, at - top - np.log(tot), 0.0)
+    correct = np.where(ok & (at == top), 1.0 / (z == top).sum(0), 0.0)
+    dz = -e / tot
+    dz[li, np.arange(n)] += 1
+    dz *= coeff * ok
+    # the error of one logit, per case; of e / tot, relative; of dz
+    a = np.abs(w) @ np.abs(x) + np.where(np.isfinite(b), np.abs(b), 0)[:, None]
+    ez = (sum_err(w.shape[1]) + 4 * U) * a.max(0)
+    er = 2 * ez + sum_err(v) + 16 * U
+    edz = (np.abs(coeff) * ok) * (e / tot) * er + 4 * U * np.abs(dz)
+    return dict(z=z, top=top, tot=tot, logp=logp, correct=correct, dz=dz, dx=w.T @ dz, dw=dz @ x.T, db=dz.sum(1), ez=ez, er=er, ok=ok,
+                edx=np.abs(w).T @ edz + (sum_err(v) + 2 * U) * (np.abs(w).T @ np.abs(dz)),
+                edw=edz @ np.abs(x).T + (sum_err(n) + 2 * U) * (np.abs(dz) @ np.abs(x).T),
+                edb=edz.sum(1) + (sum_err(n) + 2 * U) * np.abs(dz).sum(1))
+
+
+def check_forward(ref, stats, logp, correct, what=''):
+    within(stats[0], ref['top'], ref['ez'] + 2 * U * np.abs(ref['top']), what + 'max')
+    within(stats[1], ref['tot'], ref['tot'] * ref['er'], what + 'sum')
+    within(logp, ref['logp'], 2 * ref['er'] + 4 * U * np.abs(ref['logp']), what + 'logp')
+    # decisions: where the two largest logits are further apart than their errors
+    z = np.sort(ref['z'], 0)
+    clear = z[-1] - z[-2] > 4 * ref['ez'] if z.shape[0] > 1 else np.ones(z.shape[1], bool)
+    assert np.array_equal(correct[clear], ref['correct'][clear].astype(np.float32)), what + 'correct'
+
+
+# inputs, outputs, cases
+FCL_SHAPES = [(1, 1, 1), (1, 2, 3), (3, 1, 5), (16, 2, 1), (160, 4213, 1), (160, 4213, 2), (33, 65, 7), (64, 64, 64), (32, 128, 128),
+              (160, 1000, 128), (512, 1999, 128), (100, 333, 129), (17, 4097, 33), (513, 130, 260), (1000, 257, 31), (2049, 96, 40),
+              (128, 640, 512), (96, 10575, 100), (256, 300, 1025)]
+
+
+def fcl_run(w, x, b, lab, coeff=1.0, scales=(0.0, 0.0, 1.0, 0.0, 1.0), start=(None, None, None), stream=None):
+    (v, d), n = w.shape, x.shape[1]
+    st, lp, ok = Out((2, n)), Out((n,)), Out((n,))
+    dx, dw, db = Out((d, n), start[0]), Out((v, d), start[1]), Out((v,), start[2])
+    cost = dev_double(2)
+    ws, size = need('mcn_fc_logreg_workspace_bytes', d, v, n, 1)
+    keep = dev(w), dev(x), dev(b) if b is not None else None, dev(lab)
+    call('mcn_fc_logreg_cost', *keep, st, lp, ok, d, v, n, cost, ws, size, stream)
+    call('mcn_fc_logreg_grad', *keep, st, dx, dw, db, d, v, n, coeff, *scales, ws, size, stream)
+    return [o.get() for o in (st, lp, ok, dx, dw, db)] + [cost.numpy()]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('d,v,n', FCL_SHAPES)
+def test_fc_logreg(d, v, n):
+    w, x, b, lab = fcl_data(d, v, n, d * 7 + v + n, masked=0.1 if v > 50 else 0, padded=n // 4)
+    coeff = 0.37
+    ref = fcl_ref(w, x, b, lab, coeff)
+    st, lp, ok, dx, dw, db, cost = first = fcl_run(w, x, b, lab, coeff)
+    check_forward(ref, st, lp, ok)
+    within(dx, ref['dx'], ref['edx'], 'dx')
+    within(dw, ref['dw'], ref['edw'], 'dw')
+    within(db, ref['db'], ref['edb'], 'db')
+    assert abs(cost[0] + lp.astype(np.float64).sum()) <= 1e-12 * n + 1e-12 * np.abs(lp).sum()
+    assert cost[1] == pytest.approx(ref['ok'].sum() - ok.astype(np.float64).sum(), abs=1e-9)
+    for a, c in zip(first, fcl_run(w, x, b, lab, coeff)):
+        assert np.array_equal(a, c), 'not the same bits again'
+    # added onto what is there, with scales; no biases
+    rng = np.random.default_rng(2)
+    t = [rng.standard_normal(s).astype(np.float32) for s in ((d, n), (v, d), (v,))]
+    ref = fcl_ref(w, x, np.zeros(v), lab, coeff)
+    got = fcl_run(w, x, None, lab, coeff, (1.0, 0.9, 0.5, 0.25, -2.0), t)
+    within(got[3], t[0] + ref['dx'], ref['edx'] + 4 * U * (np.abs(t[0]) + np.abs(ref['dx'])), 'dx added')
+    within(got[4], 0.9 * t[1] + 0.5 * ref['dw'], 0.5 * ref['edw'] + 4 * U * (np.abs(t[1]) + np.abs(ref['dw'])), 'dw added')
+    within(got[5], 0.25 * t[2] - 2 * ref['db'], 2 * ref['edb'] + 4 * U * (np.abs(t[2]) + 2 * np.abs(ref['db'])), 'db added')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('d,v,n', [(33, 65, 7), (160, 1000, 128), (100, 700, 300)])
+def test_fc_logreg_each_gradient_alone_and_unaligned(d, v, n):
+    w, x, b, lab = fcl_data(d, v, n, 11)
+    st, lp, ok, *grads, _ = fcl_run(w, x, b, lab, 0.5)
+    ws, size = need('mcn_fc_logreg_workspace_bytes', d, v, n, 1)
+    shift = lambda a: dev(np.concatenate([[0], a.ravel()]))  # noqa: E731
+    keep = [shift(a) for a in (w, x, b, lab)]
+    ptrs = [k.ptr + 4 for k in keep]
+    st2, lp2, ok2 = Out((2 * n + 1,)), Out((n + 1,)), Out((n + 1,))
+    call('mcn_fc_logreg_cost', *ptrs, st2.ptr + 4, lp2.ptr + 4, ok2.ptr + 4, d, v, n, None, ws, size, None)
+    ref = fcl_ref(w, x, b, lab, 0.5)
+    check_forward(ref, st2.get()[1:].reshape(2, n), lp2.get()[1:], ok2.get()[1:], 'unaligned ')
+    shapes = ((d, n), (v, d), (v,))
+    for k in range(3):
+        outs = [Out((int(np.prod(s)) + 1,)) for s in shapes]
+        args = [o.ptr + 4 if i == k else None for i, o in enumerate(outs)]
+        call('mcn_fc_logreg_grad', *ptrs, st2.ptr + 4, *args, d, v, n, 0.5, 0.0, 0.0, 1.0, 0.0, 1.0, ws, size, None)
+        name = ('dx', 'dw', 'db')[k]
+        within(outs[k].get()[1:].reshape(shapes[k]), ref[name], ref['e' + name], 'unaligned ' + name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n', [1, 6, 140])
+def test_fc_logreg_ties_and_masks(n):
+    """Equal classes tie exactly wherever they stand; masked classes, cases without a label, cases with no class left."""
+    d, v = 20, 400
+    w, x, b, lab = fcl_data(d, v, n, 13, lean=0)
+    lab[:] = 7
+    dirs = x / np.linalg.norm(x, axis=0)
+    if n == 1:
+        w[[7, 70, 250, 399]] = dirs[:, 0]  # far ahead of the others, and the same
+        w[[7, 70, 250, 399]] *= 100
+        b[[7, 70, 250, 399]] = 0.5
+        st, lp, ok, dx, dw, db, cost = fcl_run(w, x, b, lab)
+        assert ok[0] == 0.25 and cost[1] == 0.75
+        assert np.array_equal(dw[70], dw[250]) and db[7] == pytest.approx(0.75, rel=1e-5)
+        return
+    # the lowest value of the type, and minus infinity, as masks
+    for low in (-np.inf, np.finfo(np.float32).min):
+        b2 = b.copy()
+        b2[50:390] = low
+        st, lp, ok, dx, dw, db, _ = fcl_run(w, x, b2, lab)
+        ref = fcl_ref(w, x, b2, lab, 1.0)
+        check_forward(ref, st, lp, ok, 'masked ') if low == -np.inf else within(lp, ref['logp'], 2 * ref['er'] + 4 * U * np.abs(ref['logp']) + 1e-5, 'logp')
+        assert not dw[50:390].any() and not db[50:390].any()
+    # no class left
+    st, lp, ok, dx, dw, db, _ = fcl_run(w, x, np.full(v, -np.inf, np.float32), lab)
+    assert np.all(st[0] == -np.inf) and not st[1].any() and np.all(lp == -np.inf) and not ok.any()
+    assert not dx.any() and not dw.any() and not db.any()
+    # no labels: out of range on either side, not a number
+    for bad in (-1, v, 1e9, np.nan, np.inf, -np.inf):
+        st, lp, ok, dx, dw, db, cost = fcl_run(w, x, b, np.full(n, bad, np.float32))
+        assert not lp.any() and not ok.any() and not cost.any() and not dx.any() and not dw.any() and not db.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('d,v,n', [(12, 30, 9), (40, 150, 66)])
+def test_fc_logreg_gradient_against_differences(d, v, n):
+    """d sum(log p) along random directions (central differences of the float64 formula, step 1e-4: 1e-6 of the magnitudes)."""
+    w, x, b, lab = fcl_data(d, v, n, 17, padded=2)
+    _, _, _, dx, dw, db, _ = fcl_run(w, x, b, lab)
+    ref = fcl_ref(w, x, b, lab, 1.0)
+    rng = np.random.default_rng(6)
+    base = [a.astype(np.float64) for a in (x, w, b)]
+    for k, (got, e) in enumerate(((dx, 'edx'), (dw, 'edw'), (db, 'edb'))):
+        dirn = rng.standard_normal(got.shape)
+        h = 1e-4
+
+        def value(s):
+            p = [a + s * dirn if i == k else a for i, a in enumerate(base)]
+            z = p[1] @ p[0] + p[2][:, None]
+            top = z.max(0)
+            lse = top + np.log(np.exp(z - top).sum(0))
+            return sum(z[int(lab[c]), c] - lse[c] for c in range(n) if lab[c] >= 0)
+        want = (value(h) - value(-h)) / (2 * h)
+        assert abs((got * dirn).sum() - want) <= (ref[e] * np.abs(dirn)).sum() + 1e-6 * np.abs(got * dirn).sum()
+
+
+# ------------------------------------------------------------------------------------------------------------- together
+def head_ref(x, gain, bias, w, b, lab, keep, p, coeff):
+    y, mean, r = norm_ref(x, gain, bias)
+    s = keep / (1 - float(np.float32(p)))
+    ref = fcl_ref(w, y * s, b, lab, coeff)
+    dy = ref['dx'] * s
+    dx, dgain, dbias = undo_ref(dy, x, gain, mean, r)
+    return ref, dx, dgain, dbias
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('captured', [False, True])
+def test_head_together(captured):
+    """norm -> dropout -> classifier cost and back, on a stream of its own: eager, and as a graph that is replayed with new masks
+    between the program's own eager work.  Six stages, each with sums of at most 900 terms (sum_err(900) = 1.5e-5 of the magnitudes):
+    1e-4 of the largest value."""
+    f, v, n, p, coeff = 160, 900, 96, 0.4, 1.0 / 96
+    x, gain, bias, _ = norm_data(f, n, 21)
+    w, _, b, lab = fcl_data(f, v, n, 22)
+    stream = C.c_void_p()
+    call('mcn_stream_create', C.byref(stream))
+    kx, kg, kb, kw, kbb, kl = (dev(a) for a in (x, gain, bias, w, b, lab))
+    y, st, drop = Out((f, n)), Out((2, n)), Out((f, n))
+    cst, lp, ok = Out((2, n)), Out((n,)), Out((n,))
+    dd, dw, db, dn, dg, dbi = Out((f, n)), Out((v, f)), Out((v,)), Out((f, n)), Out((f,)), Out((f,))
+    counter = capi.DeviceBuffer(array=np.array([100], np.uint64))
+    sizes = [need('mcn_layer_norm_workspace_bytes', f, n), need('mcn_layer_norm_undo_workspace_bytes', f, n),
+             need('mcn_fc_logreg_workspace_bytes', f, v, n, 1)]
+    (w1, s1), (w2, s2), (w3, s3) = sizes
+
+    def step():
+        call('mcn_counter_add', counter.ptr, 1, stream)
+        call('mcn_layer_norm', kx, kg, kb, y, st, f, n, EPS, w1, s1, stream)
+        call('mcn_dropout', y, drop, f * n, p, 99, 0, counter.ptr, 0.0, 1.0, stream)
+        call('mcn_fc_logreg_cost', kw, drop, kbb, kl, cst, lp, ok, f, v, n, None, w3, s3, stream)
+        call('mcn_fc_logreg_grad', kw, drop, kbb, kl, cst, dd, dw, db, f, v, n, coeff, 0.0, 0.0, 1.0, 0.0, 1.0, w3, s3, stream)
+        call('mcn_dropout', dd, dd, f * n, p, 99, 0, counter.ptr, 0.0, 1.0, stream)
+        call('mcn_layer_norm_undo', dd, kx, kg, st, dn, dg, dbi, f, n, 0.0, 1.0, 0.0, 1.0, 0.0, 1.0, w2, s2, stream)
+
+    exe = C.c_void_p()
+    if captured:
+        step()  # once eagerly, as a program would
+        call('mcn_stream_sync', stream)
+        call('mcn_graph_begin_capture', stream)
+        step()
+        call('mcn_graph_end_capture', stream, C.byref(exe), None)
+    for k in range(4):
+        if captured:
+            call('mcn_graph_launch', exe, stream)
+        else:
+            step()
+        call('mcn_stream_sync', stream)
+        number = 101 + k + (1 if captured else 0)
+        keep = kept(f * n, p, 99, number).reshape(f, n)
+        ref, wx, wg, wb = head_ref(x.astype(np.float64), gain.astype(np.float64), bias.astype(np.float64), w, b, lab, keep, p, coeff)
+        for got, want, what in ((lp, ref['logp'], 'logp'), (dw, ref['dw'], 'dw'), (db, ref['db'], 'db'), (dn, wx, 'dx'), (dg, wg, 'dgain'), (dbi, wb, 'dbias')):
+            within(got.get(), want, 1e-4 * np.abs(want).max(), '%s of step %d' % (what, k))
+        # eager work of the program between the replays
+        other = Out((f, n))
+        call('mcn_layer_norm', kx, None, None, other, None, f, n, EPS, w1, s1, None)
+        call('mcn_device_sync')
+    if captured:
+        call('mcn_graph_destroy', exe)
+    call('mcn_stream_destroy', stream)
