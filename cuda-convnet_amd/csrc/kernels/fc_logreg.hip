@@ -147,33 +147,50 @@ __global__ __launch_bounds__(256) void k_fcl_tile(FclArgs p) {
     }
 }
 
-// Joins the tiles of every case: 16 cases x 16 tile lanes per block, tiles in a fixed order.
-__global__ __launch_bounds__(256) void k_fcl_join(const float* __restrict__ part, const float* __restrict__ labelLogits,
-                                                  const float* __restrict__ labels, float* __restrict__ caseStats, float* __restrict__ logProbs,
-                                                  float* __restrict__ correct, int V, int N, int tiles) {
-    __shared__ float sh[3][16][17];
+// Joins the tiles of every case: 16 cases x 64 tile lanes per block; first the max, then the sums, so that no exponential waits for
+// another (running joins of 782 tiles took 32 us for 1024 cases).
+__global__ __launch_bounds__(1024) void k_fcl_join(const float* __restrict__ part, const float* __restrict__ labelLogits,
+                                                   const float* __restrict__ labels, float* __restrict__ caseStats, float* __restrict__ logProbs,
+                                                   float* __restrict__ correct, int V, int N, int tiles) {
+    __shared__ float sh[2][64][17];
     const int c = threadIdx.x & 15, l = threadIdx.x >> 4, n = blockIdx.x * 16 + c;
-    Stat a = {-INFINITY, 0.f, 0.f};
-    if (n < N)
-        for (int t = l; t < tiles; t += 16) {
+    float m = -INFINITY;
+    if (n < N) {
+#pragma unroll 8
+        for (int t = l; t < tiles; t += 64) m = fmaxf(m, part[(size_t)t * 3 * N + n]);
+    }
+    sh[0][l][c] = m;
+    __syncthreads();
+    for (int k = 0; k < 64; k++) m = fmaxf(m, sh[0][k][c]);
+    __syncthreads();
+    float rest = 0.f, cnt = 0.f;
+    if (n < N) {
+#pragma unroll 8
+        for (int t = l; t < tiles; t += 64) {
             const float* q = part + (size_t)t * 3 * N + n;
-            stat_join(a, q[0], q[N], q[2 * (size_t)N]);
+            const bool top = q[0] == m;
+            // (a tile without a finite logit holds 0, or a NaN, which stays)
+            rest += top ? q[N] : (q[N] + q[2 * (size_t)N]) * (q[0] == -INFINITY ? 1.f : expf(q[0] - m));
+            cnt += top ? q[2 * (size_t)N] : 0.f;
         }
-    sh[0][l][c] = a.m;
-    sh[1][l][c] = a.rest;
-    sh[2][l][c] = a.cnt;
+    }
+    sh[0][l][c] = rest;
+    sh[1][l][c] = cnt;
     __syncthreads();
     if (l != 0 || n >= N) return;
-    for (int k = 1; k < 16; k++) stat_join(a, sh[0][k][c], sh[1][k][c], sh[2][k][c]);
-    const float s = a.cnt + a.rest;
-    caseStats[n] = a.m;
+    for (int k = 1; k < 64; k++) {
+        rest += sh[0][k][c];
+        cnt += sh[1][k][c];
+    }
+    const float s = cnt + rest;
+    caseStats[n] = m;
     caseStats[N + n] = s;
     int label;
     float lp = 0.f, hit = 0.f;
     if (label_of(labels[n], V, label)) {
         const float z = labelLogits[n];
-        lp = s == 0.f ? -INFINITY : a.cnt > 0.f ? (z - a.m) - (logf(a.cnt) + log1pf(a.rest / a.cnt)) : z - a.m - logf(s);
-        hit = z == a.m && a.cnt > 0.f ? 1.f / a.cnt : 0.f;
+        lp = s == 0.f ? -INFINITY : cnt > 0.f ? (z - m) - (logf(cnt) + log1pf(rest / cnt)) : z - m - logf(s);
+        hit = z == m && cnt > 0.f ? 1.f / cnt : 0.f;
     }
     logProbs[n] = lp;
     correct[n] = hit;
@@ -331,117 +348,150 @@ __device__ __forceinline__ void product_tile(const char* A, size_t aRow, const c
 __device__ __forceinline__ float acc_value(const Acc<2>& a, int i, int j, int r) { return a.c[0][i][j][r] + a.c[1][i][j][r] * (1.f / LO); }
 
 // ---- packing
-// Largest magnitudes of x (D, N): blocks of the first colBlocks take 64 cases each (over the features), the others 4 features each
-// (over the cases that count: a case without a label never enters the weight gradient, whatever it holds).
-__global__ __launch_bounds__(256) void k_fcl_x_scales(const float* __restrict__ X, const float* __restrict__ labels, int* __restrict__ caseExp,
-                                                      int* __restrict__ featExp, int D, int V, int N, int Np, int Dp, int colBlocks) {
-    __shared__ float sh[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    float m = 0.f;
-    if ((int)blockIdx.x < colBlocks) {
-        const int n = blockIdx.x * 64 + lane;
-        if (n < N)
-            for (int d = wave; d < D; d += 4) {
-                const float v = fabsf(X[(size_t)d * N + n]);
-                m = v > m || v != v ? v : m;
-            }
-        sh[wave][lane] = m;
-        __syncthreads();
-        if (wave == 0 && n < Np) {
-            for (int w = 1; w < 4; w++) m = sh[w][lane] > m || sh[w][lane] != sh[w][lane] ? sh[w][lane] : m;
-            caseExp[n] = scale_exp(m);
-        }
-        return;
-    }
-    const int d = (blockIdx.x - colBlocks) * 4 + wave;
-    if (d >= Dp) return;
-    if (d < D)
-        for (int n = lane; n < N; n += 64) {
-            int label;
-            const float v = label_of(labels[n], V, label) ? fabsf(X[(size_t)d * N + n]) : 0.f;
-            m = v > m || v != v ? v : m;
-        }
-    for (int o = 1; o < 64; o <<= 1) {
-        const float v = __shfl_xor(m, o, 64);
-        m = v > m || v != v ? v : m;
-    }
-    if (lane == 0) featExp[d] = scale_exp(m);
-}
-
-// Fragments of x, one wave each: first (rows = cases, k = features) for the logits, then (rows = features, k = cases) for the weights.
-__global__ __launch_bounds__(256) void k_fcl_pack_x(const float* __restrict__ X, const float* __restrict__ labels, const int* __restrict__ caseExp,
-                                                    const int* __restrict__ featExp, char* __restrict__ byCase, char* __restrict__ byFeat,
-                                                    int D, int V, int N, int Kd, int Kn, int caseFrags, int allFrags) {
-    const int lane = threadIdx.x & 63, f = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (f >= allFrags) return;
-    float y[8];
-    char* out;
-    if (f < caseFrags) {
-        const int n = f / Kd * 16 + (lane & 15), d0 = f % Kd * 32 + (lane >> 4) * 8, e = caseExp[n];
-#pragma unroll
-        for (int j = 0; j < 8; j++) y[j] = n < N && d0 + j < D ? ldexpf(X[(size_t)(d0 + j) * N + n], e) : 0.f;
-        out = byCase + (size_t)f * 2 * FRAG;
-    } else {
-        const int g = f - caseFrags, d = g / Kn * 16 + (lane & 15), n0 = g % Kn * 32 + (lane >> 4) * 8, e = featExp[d];
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            int label;
-            y[j] = d < D && n0 + j < N && label_of(labels[n0 + j], V, label) ? ldexpf(X[(size_t)d * N + n0 + j], e) : 0.f;
-        }
-        out = byFeat + (size_t)g * 2 * FRAG;
-    }
+__device__ __forceinline__ float max_or_nan(float m, float v) { return v > m || v != v ? v : m; }
+__device__ __forceinline__ void store_split16(char* out, int lane, const float (&y)[8]) {
     const Split16 s = split16(y);
     *reinterpret_cast<f16x8*>(out + lane * 16) = s.hi;
     *reinterpret_cast<f16x8*>(out + FRAG + lane * 16) = s.lo;
 }
 
+// Fragments of x (D, N).  The first caseBlocks blocks take 16 cases each: (rows = cases, k = features) for the logits; the others 16
+// features each: (rows = features, k = cases) for the weight gradient, in which a case without a label is zero, whatever it holds.
+// Each block finds its rows' largest magnitudes first; what it reads then comes from its caches.
+__global__ __launch_bounds__(512) void k_fcl_pack_x(const float* __restrict__ X, const float* __restrict__ labels, int* __restrict__ caseExp,
+                                                    int* __restrict__ featExp, char* __restrict__ byCase, char* __restrict__ byFeat, int D,
+                                                    int V, int N, int Kd, int Kn, int caseBlocks) {
+    __shared__ float sh[8][16];
+    __shared__ int exps[16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    float m = 0.f;
+    if ((int)blockIdx.x < caseBlocks) {
+        const int n = blockIdx.x * 16 + c;
+        if (n < N) {
+#pragma unroll 8
+            for (int d = threadIdx.x >> 4; d < D; d += 32) m = max_or_nan(m, fabsf(X[(size_t)d * N + n]));
+        }
+        m = max_or_nan(m, __shfl_xor(m, 16, 64));
+        m = max_or_nan(m, __shfl_xor(m, 32, 64));
+        sh[wave][c] = m;
+        __syncthreads();
+        if (threadIdx.x < 16) {
+            for (int w = 1; w < 8; w++) m = max_or_nan(m, sh[w][c]);
+            caseExp[n] = exps[c] = scale_exp(m);
+        }
+        __syncthreads();
+        const int e = exps[c];
+        for (int kb = wave; kb < Kd; kb += 8) {
+            const int d0 = kb * 32 + g * 8;
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) y[j] = n < N && d0 + j < D ? ldexpf(X[(size_t)(d0 + j) * N + n], e) : 0.f;
+            store_split16(byCase + ((size_t)blockIdx.x * Kd + kb) * 2 * FRAG, lane, y);
+        }
+        return;
+    }
+    const int d0 = (blockIdx.x - caseBlocks) * 16, r = threadIdx.x >> 5;
+    if (d0 + r < D) {
+#pragma unroll 4
+        for (int n = threadIdx.x & 31; n < N; n += 32) {
+            int label;
+            const bool counts = label_of(labels[n], V, label);
+            const float v = fabsf(X[(size_t)(d0 + r) * N + n]);
+            m = counts ? max_or_nan(m, v) : m;
+        }
+    }
+    for (int o = 1; o < 32; o <<= 1) m = max_or_nan(m, __shfl_xor(m, o, 64));
+    if ((threadIdx.x & 31) == 0) featExp[d0 + r] = exps[r] = scale_exp(m);
+    __syncthreads();
+    const int d = d0 + c, e = exps[c];
+    for (int kb = wave; kb < Kn; kb += 8) {
+        const int n0 = kb * 32 + g * 8;
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            int label;
+            y[j] = d < D && n0 + j < N && label_of(labels[n0 + j], V, label) ? ldexpf(X[(size_t)d * N + n0 + j], e) : 0.f;
+        }
+        store_split16(byFeat + ((size_t)(d0 / 16) * Kn + kb) * 2 * FRAG, lane, y);
+    }
+}
+
 // Fragments of a piece of W, 32 classes per block: (rows = classes, k = features, fp16) for the logits and, TRANS, (rows = features,
 // k = classes, bf16) for the input gradient.  k order of the latter: entry 8 g + j of a block of 32 is class 4 g + j (j < 4) or
-// 16 + 4 g + j - 4, which is how the lanes of the logits' tile hold them.
+// 16 + 4 g + j - 4, which is how the lanes of the logits' tile hold them.  512 features at a time go through registers (all of a
+// thread's loads in flight at once) and LDS; rows of at most 512 features are read once, longer ones a second time for their max.
+constexpr int CW = 512, CW_LD = CW + 4;
 template <bool TRANS>
-__global__ __launch_bounds__(256) void k_fcl_pack_w(const float* __restrict__ W, int* __restrict__ rowExp, char* __restrict__ byClass,
+__global__ __launch_bounds__(512) void k_fcl_pack_w(const float* __restrict__ W, int* __restrict__ rowExp, char* __restrict__ byClass,
                                                     char* __restrict__ byFeat, int D, int rows, int Kd, int Kv, int Dp) {
-    constexpr int CW = 128;
-    __shared__ float tile[32][CW + 4];
-    __shared__ int exps[32];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, v0 = blockIdx.x * 32;
-    for (int r = wave; r < 32; r += 4) {
-        float m = 0.f;
-        if (v0 + r < rows)
-            for (int d = lane; d < D; d += 64) {
-                const float v = fabsf(W[(size_t)(v0 + r) * D + d]);
-                m = v > m || v != v ? v : m;
+    extern __shared__ __attribute__((aligned(16))) float tile[];  // [32][CW_LD], then 32 exponents
+    int* exps = reinterpret_cast<int*>(tile + 32 * CW_LD);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, v0 = blockIdx.x * 32, c = lane & 15, g = lane >> 4;
+    f32x4 t[4][2];
+    auto load = [&](int d0) {  // a wave: rows 4 wave .. + 3, a lane: features d0 + 4 lane .. and 256 further on
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int v = v0 + wave * 4 + r, d = d0 + h * 256 + lane * 4;
+                const float* src = W + (size_t)v * D + d;
+                f32x4 x = {0.f, 0.f, 0.f, 0.f};
+                if (v < rows) {
+                    if (d + 4 <= D) {
+                        const f32x4u u = *reinterpret_cast<const f32x4u*>(src);
+                        x = (f32x4){u[0], u[1], u[2], u[3]};
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 3; j++)
+                            if (d + j < D) x[j] = src[j];
+                    }
+                }
+                t[r][h] = x;
             }
-        for (int o = 1; o < 64; o <<= 1) {
-            const float v = __shfl_xor(m, o, 64);
-            m = v > m || v != v ? v : m;
-        }
-        if (lane == 0) rowExp[v0 + r] = exps[r] = scale_exp(m);
+    };
+    float m[4] = {};
+    for (int d0 = 0; d0 < D; d0 += CW) {
+        load(d0);
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) m[r] = max_or_nan(m[r], fabsf(t[r][h][j]));
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        for (int o = 1; o < 64; o <<= 1) m[r] = max_or_nan(m[r], __shfl_xor(m[r], o, 64));
+        if (lane == 0) rowExp[v0 + wave * 4 + r] = exps[wave * 4 + r] = scale_exp(m[r]);
     }
     const int Dt = TRANS ? Dp : Kd * 32;
     for (int d0 = 0; d0 < Dt; d0 += CW) {
+        if (D > CW) load(d0);
         __syncthreads();
-        for (int e = threadIdx.x; e < 32 * CW; e += 256) {
-            const int r = e / CW, d = e % CW;
-            tile[r][d] = v0 + r < rows && d0 + d < D ? W[(size_t)(v0 + r) * D + d0 + d] : 0.f;
-        }
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) *reinterpret_cast<f32x4*>(tile + (wave * 4 + r) * CW_LD + h * 256 + lane * 4) = t[r][h];
         __syncthreads();
-        for (int f = wave; f < 8; f += 4) {  // 2 row blocks x 4 k blocks
-            const int rb = f >> 2, kb = d0 / 32 + (f & 3), r = rb * 16 + (lane & 15);
-            if (kb >= Kd) continue;
+        for (int f = wave; f < 2 * CW / 32; f += 8) {
+            const int rb = f & 1, kb = d0 / 32 + (f >> 1), r = rb * 16 + c;
+            if (kb >= Kd) break;
+            const f32x4* src = reinterpret_cast<const f32x4*>(tile + r * CW_LD + (f >> 1) * 32 + g * 8);
+            const f32x4 lo = src[0], hi = src[1];
+            const int e = exps[r];
             float y[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) y[j] = ldexpf(tile[r][(f & 3) * 32 + (lane >> 4) * 8 + j], exps[r]);
-            const Split16 s = split16(y);
-            char* out = byClass + (((size_t)blockIdx.x * 2 + rb) * Kd + kb) * 2 * FRAG + lane * 16;
-            *reinterpret_cast<f16x8*>(out) = s.hi;
-            *reinterpret_cast<f16x8*>(out + FRAG) = s.lo;
+            for (int j = 0; j < 4; j++) {
+                y[j] = ldexpf(lo[j], e);
+                y[4 + j] = ldexpf(hi[j], e);
+            }
+            store_split16(byClass + (((size_t)blockIdx.x * 2 + rb) * Kd + kb) * 2 * FRAG, lane, y);
         }
         if (TRANS)
-            for (int f = wave; f < CW / 16; f += 4) {
+            for (int f = wave; f < CW / 16 && d0 + f * 16 < Dp; f += 8) {
                 float y[8];
 #pragma unroll
-                for (int j = 0; j < 8; j++) y[j] = tile[(j < 4 ? 0 : 12) + (lane >> 4) * 4 + j][f * 16 + (lane & 15)];
+                for (int j = 0; j < 8; j++) y[j] = tile[((j < 4 ? 0 : 12) + g * 4 + j) * CW_LD + f * 16 + c];
                 const Split24 s = split24(y);
                 char* out = byFeat + ((size_t)(d0 / 16 + f) * Kv + blockIdx.x) * 3 * FRAG + lane * 16;
 #pragma unroll
@@ -449,6 +499,7 @@ __global__ __launch_bounds__(256) void k_fcl_pack_w(const float* __restrict__ W,
             }
     }
 }
+constexpr int PACK_LDS = (32 * CW_LD + 32) * 4;
 
 // ---- logits of a piece
 struct WideArgs {
@@ -699,6 +750,7 @@ __global__ __launch_bounds__(256) void k_fcl_finish(const float* __restrict__ sl
         if (i >= (size_t)D * N) return;
         const size_t d = i / N, n = i % N;
         float v = 0.f;
+#pragma unroll 8
         for (int s = 0; s < splits; s++) v += slabs[((size_t)s * Dp + d) * Np + n];
         dX[i] = (scaleInputTargets != 0.f ? scaleInputTargets * dX[i] : 0.f) + coeff * v;
         return;
@@ -706,6 +758,7 @@ __global__ __launch_bounds__(256) void k_fcl_finish(const float* __restrict__ sl
     const int v = (blockIdx.x - dxBlocks) * 256 + threadIdx.x;
     if (v >= V) return;
     float s = 0.f;
+#pragma unroll 8
     for (int t = 0; t < nTiles; t++) s += dbPart[(size_t)t * V + v];
     dB[v] = (scaleBiasTargets != 0.f ? scaleBiasTargets * dB[v] : 0.f) + scaleBiasOutput * coeff * s;
 }
@@ -772,14 +825,12 @@ int wide_cost(const float* W, const float* X, const float* bias, const float* la
     a.caseExp = (const int*)(ws + q.caseExp);
     a.bias = bias; a.labels = labels; a.V = V; a.N = N; a.Kd = q.Kd; a.nTiles = q.nTiles;
     a.labelLogits = (float*)(ws + q.labelLogits);
-    const int colBlocks = divup(q.Np, 64), frags = q.Np / 16 * q.Kd;
-    MCN_LAUNCH(k_fcl_x_scales, dim3(colBlocks), dim3(256), 0, s, X, labels, (int*)(ws + q.caseExp), (int*)(ws + q.featExp), D, V, N, q.Np, q.Dp, colBlocks);
-    MCN_LAUNCH(k_fcl_pack_x, dim3(divup(frags, 4)), dim3(256), 0, s, X, labels, (const int*)(ws + q.caseExp), (const int*)(ws + q.featExp),
-               ws + q.xByCase, (char*)nullptr, D, V, N, q.Kd, q.Kn, frags, frags);
+    MCN_LAUNCH(k_fcl_pack_x, dim3(q.Np / 16), dim3(512), 0, s, X, labels, (int*)(ws + q.caseExp), (int*)nullptr, ws + q.xByCase, (char*)nullptr,
+               D, V, N, q.Kd, q.Kn, q.Np / 16);
     int tiles = 0;
     for (int v0 = 0; v0 < V; v0 += q.rows) {
         const int rows = std::min(q.rows, V - v0), vTiles = divup(rows, TILE);
-        MCN_LAUNCH(k_fcl_pack_w<false>, dim3(vTiles * (TILE / 32)), dim3(256), 0, s, W + (size_t)v0 * D, (int*)(ws + q.rowExp), ws + q.wByClass,
+        MCN_LAUNCH(k_fcl_pack_w<false>, dim3(vTiles * (TILE / 32)), dim3(512), PACK_LDS, s, W + (size_t)v0 * D, (int*)(ws + q.rowExp), ws + q.wByClass,
                    (char*)nullptr, D, rows, q.Kd, vTiles * (TILE / 32), q.Dp);
         a.v0 = v0;
         a.rows = rows;
@@ -789,7 +840,7 @@ int wide_cost(const float* W, const float* X, const float* bias, const float* la
         tiles += vTiles;
         if (int rc = MCN_LAUNCH_CHECK("fcLogregCost")) return rc;
     }
-    MCN_LAUNCH(k_fcl_join, dim3(divup(N, 16)), dim3(256), 0, s, (const float*)(ws + q.part), a.labelLogits, labels, stats, logp, correct, V, N, tiles);
+    MCN_LAUNCH(k_fcl_join, dim3(divup(N, 16)), dim3(1024), 0, s, (const float*)(ws + q.part), a.labelLogits, labels, stats, logp, correct, V, N, tiles);
     return MCN_LAUNCH_CHECK("fcLogregCost");
 }
 
@@ -806,18 +857,15 @@ int wide_grad(const float* W, const float* X, const float* bias, const float* la
     a.dzByCase = dX ? ws + q.dzByCase : nullptr;
     a.dzByClass = dW ? ws + q.dzByClass : nullptr;
     a.dbPart = dB ? (float*)(ws + q.dbPart) : nullptr;
-    const int colBlocks = divup(q.Np, 64), caseFrags = q.Np / 16 * q.Kd, featFrags = dW ? q.Dp / 16 * q.Kn : 0;
-    MCN_LAUNCH(k_fcl_x_scales, dim3(colBlocks + (dW ? divup(q.Dp, 4) : 0)), dim3(256), 0, s, X, labels, (int*)(ws + q.caseExp),
-               (int*)(ws + q.featExp), D, V, N, q.Np, q.Dp, colBlocks);
-    MCN_LAUNCH(k_fcl_pack_x, dim3(divup(caseFrags + featFrags, 4)), dim3(256), 0, s, X, labels, (const int*)(ws + q.caseExp),
-               (const int*)(ws + q.featExp), ws + q.xByCase, ws + q.xByFeat, D, V, N, q.Kd, q.Kn, caseFrags, caseFrags + featFrags);
+    MCN_LAUNCH(k_fcl_pack_x, dim3(q.Np / 16 + (dW ? q.Dp / 16 : 0)), dim3(512), 0, s, X, labels, (int*)(ws + q.caseExp), (int*)(ws + q.featExp),
+               ws + q.xByCase, ws + q.xByFeat, D, V, N, q.Kd, q.Kn, q.Np / 16);
     for (int v0 = 0; v0 < V; v0 += q.rows) {
         const int rows = std::min(q.rows, V - v0), vTiles = divup(rows, TILE), Kv = vTiles * (TILE / 32);
         if (dX)
-            MCN_LAUNCH(k_fcl_pack_w<true>, dim3(Kv), dim3(256), 0, s, W + (size_t)v0 * D, (int*)(ws + q.rowExp), ws + q.wByClass,
+            MCN_LAUNCH(k_fcl_pack_w<true>, dim3(Kv), dim3(512), PACK_LDS, s, W + (size_t)v0 * D, (int*)(ws + q.rowExp), ws + q.wByClass,
                        ws + q.wByFeat, D, rows, q.Kd, Kv, q.Dp);
         else
-            MCN_LAUNCH(k_fcl_pack_w<false>, dim3(Kv), dim3(256), 0, s, W + (size_t)v0 * D, (int*)(ws + q.rowExp), ws + q.wByClass,
+            MCN_LAUNCH(k_fcl_pack_w<false>, dim3(Kv), dim3(512), PACK_LDS, s, W + (size_t)v0 * D, (int*)(ws + q.rowExp), ws + q.wByClass,
                        ws + q.wByFeat, D, rows, q.Kd, Kv, q.Dp);
         a.v0 = v0;
         a.rows = rows;
@@ -894,7 +942,7 @@ MCN_API int mcn_fc_logreg_cost(const float* weights, const float* inputs, const 
         p.part = (float*)workspace;
         p.labelLogits = (float*)((char*)workspace + al16b((size_t)tiles * 3 * numCases * sizeof(float)));
         MCN_LAUNCH(k_fcl_tile<false>, dim3(tiles * p.nTiles), dim3(256), 0, s, p);
-        MCN_LAUNCH(k_fcl_join, dim3(divup(numCases, 16)), dim3(256), 0, s, p.part, p.labelLogits, labels, caseStats, labelLogProbs, correctProbs,
+        MCN_LAUNCH(k_fcl_join, dim3(divup(numCases, 16)), dim3(1024), 0, s, p.part, p.labelLogits, labels, caseStats, labelLogProbs, correctProbs,
                    numOutputs, numCases, tiles);
     }
     if (costOut) MCN_LAUNCH(k_fcl_cost, dim3(1), dim3(256), 0, s, labels, labelLogProbs, correctProbs, numOutputs, numCases, costOut);
