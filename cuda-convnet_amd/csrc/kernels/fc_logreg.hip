@@ -225,136 +225,201 @@ __global__ __launch_bounds__(256) void k_fcl_cost(const float* __restrict__ labe
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------
-// Many cases: the three products on 16-bit matrix instructions with fp32 accuracy.  fp32 matrix instructions reach 157 TFLOP/s, 16-bit
-// ones 2500: an fp32 operand is split into 16-bit pieces whose products are exact in fp32, and the products that matter are added up.
-//   fp16 x 2 (logits, weight gradient): after scaling by a power of two (max of a row in [2^14, 2^15)) y = hi + 2^-11 lo with 11 bits
-//     each; hi hi, hi lo and lo hi are kept (3 instructions), the cross terms in an accumulator of their own, so that lo keeps its
-//     bits: relative error 2^-22 of a product, for entries down to 2^-28 of their row's max; an entry further down is off by 2^-50 of
-//     that max.  Rows are scaled along the dimension that is NOT summed over, so one large row never costs another its bits.
-//   bf16 x 3 (input gradient): y = h + m + l with 8 bits each, hh + hm + mh + hl + lh + mm kept (6 instructions): relative error about
-//     2^-24, with fp32's own range.  Its sum runs over the classes, whose weights have no common scale.
-// Operands are split ONCE by a pack launch into fragments, the 64 lanes x 16 bytes that one 16 x 16 x 32 instruction reads:
-//   fragment (rowBlock, kBlock, piece): lane l holds row l & 15, entries k = 8 (l >> 4) .. + 7 of the block's 32,
-// stored one after the other (1 KB each, the pieces of one block together), zero-padded to whole tiles.  A product kernel copies
-// fragments to LDS (global_load_lds, 16 bytes a lane, no registers, no swizzle: lanes read them back in order, conflict-free).
+// Many cases: the three products on fp16 matrix instructions with fp32 accuracy.  fp32 matrix instructions reach 157 TFLOP/s, fp16 ones
+// 2500: an fp32 operand, scaled by a power of two, is split into y = hi + 2^-11 lo with 11 bits each; the products of pieces are exact in
+// fp32, and hi hi, hi lo and lo hi are summed (3 instructions), the cross terms in an accumulator of their own, so that lo keeps its
+// bits.  With the largest magnitude of a scaled group below 2^15 the relative error of a product is about 2^-22 for entries down to
+// 2^-21 of the group's largest, and an entry further down is off by at most 2^-43 of it.  The groups: a case's features for the
+// logits, a feature's cases for the weight gradient, 32 classes' weights, and +-1 for dz / coeff.  Along the summed dimension a group
+// is either whole or, for the classes of the input gradient, its scale is carried along (k_fcl_igrad), so a row of large weights
+// takes no bits from the other groups.
+//
+// Operands are split ONCE by a pack launch into fragments of 16 rows x 32 k entries and two pieces, 1 KB each:
+//   entry (row c, k = 16 h + 4 g + j) of a piece lies at byte 512 h + 128 g + 8 c + 2 j, zero-padded to whole tiles.
+// A product copies fragments to LDS as they are (global_load_lds, 16 bytes a lane: no registers, no swizzle).  As the first operand,
+// and with k along its own k, a lane (c, g) of a 16 x 16 x 32 instruction reads two 8-byte entries, h = 0 and 1; as the operand whose k
+// is the fragments' ROW, a transposing LDS read (ds_read_b64_tr_b16) gives lane (k = 16 h + c, g) rows 4 g .. 4 g + 3 of two fragments.
+// Both read 512 contiguous bytes a wave, without conflicts, and in both a lane's eight entries are 4 g + j and 16 + 4 g + j of the step's
+// 32, so that every pairing sums the same terms.  So W and dz are each stored once, and serve two products.
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef __fp16 fp16x4 __attribute__((__vector_size__(4 * sizeof(__fp16))));  // (the type the transposing read is declared with)
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
-constexpr int FRAG = 1024;      // bytes of a fragment
-constexpr int TILE = 128;       // rows and columns of a product's tile
-constexpr float LO = 2048.f;    // scale of the low fp16 piece
+constexpr int FRAG = 1024, PAIR = 2 * FRAG;  // bytes of a fragment, of its two pieces
+constexpr int TILE = 128;                    // columns of a product's tile
+constexpr float LO = 2048.f;                 // scale of the low piece
+constexpr int DZ_EXP = 14;                   // |dz / coeff| <= 1
+constexpr int EXP_ZERO = 1 << 20;            // a group of zeros: any scale will do
 
-struct Split16 { f16x8 hi, lo; };
-__device__ __forceinline__ Split16 split16(const float (&y)[8]) {
-    Split16 s;
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-        s.hi[j] = (_Float16)y[j];
-        s.lo[j] = (_Float16)((y[j] - (float)s.hi[j]) * LO);
-    }
-    return s;
-}
-struct Split24 { bf16x8 p[3]; };
-__device__ __forceinline__ Split24 split24(const float (&y)[8]) {
-    Split24 s;
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-        float r = y[j];
-#pragma unroll
-        for (int q = 0; q < 3; q++) {
-            s.p[q][j] = (__bf16)r;
-            r -= (float)s.p[q][j];
-        }
-    }
-    return s;
-}
-// the power of two that brings a row of largest magnitude m to [2^14, 2^15); a row of zeros, infinities or NaNs stays as it is
+// the power of two that brings a group of largest magnitude m to [2^14, 2^15); infinities and NaNs stay as they are
 __device__ __forceinline__ int scale_exp(float m) { return m > 0.f && m < INFINITY ? 14 - ilogbf(m) : 0; }
+__device__ __forceinline__ float max_or_nan(float m, float v) { return v > m || v != v ? v : m; }
 
-// C tile of 128 x 128 by four waves, 64 x 64 each: acc[hi/cross][mb][nb].  P = 2: fp16 pieces, P = 3: bf16 pieces.  A, B: first fragment
-// of the tile's first row block; aRow, bRow: bytes between row blocks; k blocks [k0, k1).  LDS: two stages.  One barrier a step: it
-// says that a stage has landed (the copies are waited for in front of it) and that everyone has read the other one.
-template <int P>
+// entries k = 16 h + 4 g + j (y[4 h + j]) of row c into a fragment pair, lane = 16 g + c
+__device__ __forceinline__ void store_pair(char* out, int lane, const float (&y)[8]) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        f16x4 hi, lo;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            hi[j] = (_Float16)y[4 * h + j];
+            lo[j] = (_Float16)((y[4 * h + j] - (float)hi[j]) * LO);
+        }
+        *reinterpret_cast<f16x4*>(out + h * 512 + lane * 8) = hi;
+        *reinterpret_cast<f16x4*>(out + FRAG + h * 512 + lane * 8) = lo;
+    }
+}
+
+// ---- one product tile: (32 MB) x 128 by four waves, 2 x 2, each (16 MB) x 64.
+template <int MB>
 struct Acc {
-    f32x4 c[P == 2 ? 2 : 1][4][4];
+    f32x4 c[2][MB][4];  // hi hi; cross terms, still times LO
+    __device__ __forceinline__ float value(int i, int j, int r) const { return c[0][i][j][r] + c[1][i][j][r] * (1.f / LO); }
 };
-template <int P>
-__device__ __forceinline__ void product_tile(const char* A, size_t aRow, const char* B, size_t bRow, int k0, int k1, char* lds, Acc<P>& acc) {
-    constexpr int FRAGS = 16 * P, STAGE = FRAGS * FRAG;
+template <int MB>
+struct Frags {
+    f16x8 a[MB][2], b[4][2];
+};
+// LDS stages: as many as 144 KB hold, one block per CU.  A tile of 256 rows spends 1536 matrix cycles on a step of 48 KB, which two
+// stages in flight cover; a small one 384 on 24 KB, and needs five.
+constexpr int tile_stages(int mb) { return mb == 8 ? 3 : mb == 4 ? 4 : 6; }
+constexpr int tile_units(int mb) { return 2 * mb + 8; }
+constexpr int tile_lds(int mb) { return tile_stages(mb) * tile_units(mb) * PAIR; }
+
+// All but the N youngest copies of this wave have landed, its LDS reads are done, and everyone is here.
+template <int N>
+__device__ __forceinline__ void wait_copies_and_meet() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0), by the builtin: the compiler then knows that the reads are done
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+// The two pieces of a pair (2 KB) from global memory to LDS; the instruction's offset counts on both sides.  The compiler would drain
+// every such copy in front of the next LDS read if it knew of it; here the waits are wait_copies_and_meet's.  No register is written.
+__device__ __forceinline__ void copy_pair_half(const char* src, unsigned lds, unsigned laneOff, int piece) {
+    if (piece == 0) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(laneOff), "s"(src) : "memory");
+    else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024" ::"s"(lds), "v"(laneOff), "s"(src) : "memory");
+}
+__device__ __forceinline__ f16x8 read_frag(const char* p) {
+    const f16x4 a = *reinterpret_cast<const f16x4*>(p), b = *reinterpret_cast<const f16x4*>(p + 512);
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+__device__ __forceinline__ f16x8 read_frag_turned(const char* p, const char* q) {
+    const f16x4 a = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4*)p));
+    const f16x4 b = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4*)q));
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+struct NoScale {
+    template <int MB>
+    __device__ __forceinline__ void operator()(int, Acc<MB>&) const {}
+};
+
+// A: pair (row block 0 of the tile, k block 0); aRow: bytes between its row blocks.  B: the same, or, TURNED, pair (row block 0, k block 0
+// of the tile's columns) of fragments whose rows are this product's k.  scale(step, acc) runs in front of a step's products.
+//
+// Step t multiplies what step t - 1 read, reads stage t + 1 and asks for stage t + STAGES, whose buffer everyone has read by then.  One
+// wave a SIMD: whatever is not a matrix instruction has to be issued while one runs (16 cycles), so the reads and copies stand between
+// them, a few after every third, and the steps have no branches: behind the end, the last stage is copied again.
+template <int MB, bool TURNED, class Scale>
+__device__ __forceinline__ void product_tile(const char* A, size_t aRow, const char* B, size_t bRow, int k0, int k1, char* lds, Acc<MB>& acc,
+                                             const Scale& scale) {
+    constexpr int UNITS = tile_units(MB), STAGES = tile_stages(MB), STAGE = UNITS * PAIR, MINE = UNITS / 4, COPIES = MINE * 2;
+    constexpr int READS = 8 + 2 * MB, OPS = READS + COPIES, SLOTS = 4 * MB;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave >> 1, wn = wave & 1;
 #pragma unroll
-    for (int h = 0; h < (P == 2 ? 2 : 1); h++)
+    for (int h = 0; h < 2; h++)
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < MB; i++)
 #pragma unroll
             for (int j = 0; j < 4; j++) acc.c[h][i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    if (k0 >= k1) return;
-    auto copy = [&](int kb, char* stage) {
+    int n = k1 - k0;
+    if (n <= 0) return;
+    // this wave's units: where they are read from, and how far that moves in a step
+    const char* src[MINE];
+    size_t adv[MINE];
 #pragma unroll
-        for (int i = 0; i < FRAGS / 4; i++) {
-            const int f = wave * (FRAGS / 4) + i, blk = f / P, q = f % P;
-            const char* src = (blk < 8 ? A + (size_t)blk * aRow : B + (size_t)(blk - 8) * bRow) + ((size_t)kb * P + q) * FRAG + lane * 16;
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                             (__attribute__((address_space(3))) void*)(stage + f * FRAG), 16, 0, 0);
+    for (int i = 0; i < MINE; i++) {
+        const int u = wave * MINE + i, w = u - 2 * MB;
+        const bool isA = u < 2 * MB;
+        src[i] = isA      ? A + (size_t)u * aRow + (size_t)k0 * PAIR
+                 : TURNED ? B + (size_t)(2 * k0 + (w >> 2)) * bRow + (size_t)(w & 3) * PAIR
+                          : B + (size_t)w * bRow + (size_t)k0 * PAIR;
+        adv[i] = isA || !TURNED ? (size_t)PAIR : 2 * bRow;
+        asm volatile("" : "+s"(src[i]), "+s"(adv[i]));  // (kept in registers, not computed again from the arguments in every step)
+    }
+    asm volatile("" : "+s"(n));
+    const unsigned ldsBase = __builtin_amdgcn_readfirstlane((unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)lds) + wave * MINE * PAIR;
+    const unsigned laneOff = lane * 16;
+    const int offA = wm * MB * PAIR + lane * 8;
+    const int offB = (2 * MB + (TURNED ? wn * 2 : wn * 4)) * PAIR + (TURNED ? (lane & 3) * 128 + ((lane >> 4) * 4 + ((lane & 15) >> 2)) * 8 : lane * 8);
+    auto read = [&](Frags<MB>& f, const char* s, int r) {  // the r-th of READS
+        if (r < 8) {
+            const int j = r & 3, q = r >> 2;
+            if constexpr (TURNED) {
+                const char* p = s + offB + (j >> 1) * PAIR + q * FRAG + (j & 1) * 512;
+                f.b[j][q] = read_frag_turned(p, p + 4 * PAIR);
+            } else {
+                f.b[j][q] = read_frag(s + offB + j * PAIR + q * FRAG);
+            }
+        } else {
+            const int i = (r - 8) >> 1, q = (r - 8) & 1;
+            f.a[i][q] = read_frag(s + offA + i * PAIR + q * FRAG);
         }
     };
-    copy(k0, lds);
-    for (int kb = k0; kb < k1; kb++) {
-        const char* cur = lds + ((kb - k0) & 1) * STAGE;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if constexpr (P == 2) {
-            f16x8 a[4][2], b[4][2];
+    int left = n - 1;           // stages behind the one that src points at
+    unsigned fill = 0, take = 0;  // byte offsets of the buffers that are copied to, and read
+    auto next_stage = [&] {
+        const bool more = left > 0;
+        left -= more ? 1 : 0;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+        for (int i = 0; i < MINE; i++) src[i] += more ? adv[i] : 0;
+        fill = fill == (STAGES - 1) * STAGE ? 0 : fill + STAGE;
+    };
+    auto step = [&](int t, Frags<MB>& now, Frags<MB>& next) {
+        wait_copies_and_meet<(STAGES - 2) * COPIES>();  // stage t + 1 has landed
+        take = take == (STAGES - 1) * STAGE ? 0 : take + STAGE;
+        const char* from = lds + take;
+        scale(t, acc);
 #pragma unroll
-                for (int q = 0; q < 2; q++) {
-                    a[i][q] = *reinterpret_cast<const f16x8*>(cur + ((wm * 4 + i) * P + q) * FRAG + lane * 16);
-                    b[i][q] = *reinterpret_cast<const f16x8*>(cur + ((8 + wn * 4 + i) * P + q) * FRAG + lane * 16);
+        for (int m = 0; m < 12 * MB; m++) {
+            const int i = m / 12, k = m % 12 / 4, j = m % 4;
+            f32x4& to = acc.c[k ? 1 : 0][i][j];
+            to = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.a[i][k == 2], now.b[j][k == 1], to, 0, 0, 0);
+            if (m % 3 == 2) {
+                const int slot = m / 3;
+#pragma unroll
+                for (int o = slot * OPS / SLOTS; o < (slot + 1) * OPS / SLOTS; o++) {
+                    if (o < READS) read(next, from, o);
+                    else copy_pair_half(src[(o - READS) >> 1], ldsBase + fill + ((o - READS) >> 1) * PAIR, laneOff, (o - READS) & 1);
                 }
-            if (kb + 1 < k1) copy(kb + 1, lds + ((kb + 1 - k0) & 1) * STAGE);
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    acc.c[0][i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i][0], b[j][0], acc.c[0][i][j], 0, 0, 0);
-                    acc.c[1][i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i][0], b[j][1], acc.c[1][i][j], 0, 0, 0);
-                    acc.c[1][i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i][1], b[j][0], acc.c[1][i][j], 0, 0, 0);
-                }
-        } else {
-            bf16x8 a[4][3], b[4][3];
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int q = 0; q < 3; q++) {
-                    a[i][q] = *reinterpret_cast<const bf16x8*>(cur + ((wm * 4 + i) * P + q) * FRAG + lane * 16);
-                    b[i][q] = *reinterpret_cast<const bf16x8*>(cur + ((8 + wn * 4 + i) * P + q) * FRAG + lane * 16);
-                }
-            if (kb + 1 < k1) copy(kb + 1, lds + ((kb + 1 - k0) & 1) * STAGE);
-#pragma unroll
-            for (int s = 2; s >= 0; s--)  // small products first
-#pragma unroll
-                for (int q = 0; q <= s; q++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-#pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            acc.c[0][i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i][q], b[j][s - q], acc.c[0][i][j], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
+        next_stage();
+    };
+#pragma unroll
+    for (int t = 0; t < STAGES; t++) {
+#pragma unroll
+        for (int o = 0; o < COPIES; o++) copy_pair_half(src[o >> 1], ldsBase + fill + (o >> 1) * PAIR, laneOff, o & 1);
+        next_stage();
     }
+    wait_copies_and_meet<(STAGES - 1) * COPIES>();
+    Frags<MB> f0, f1;
+#pragma unroll
+    for (int r = 0; r < READS; r++) read(f0, lds, r);
+    int t = 0;
+    for (; t + 1 < n; t += 2) {
+        step(t, f0, f1);
+        step(t + 1, f1, f0);
+    }
+    if (t < n) step(t, f0, f1);
+    wait_copies_and_meet<0>();  // the buffers are free again
 }
-__device__ __forceinline__ float acc_value(const Acc<2>& a, int i, int j, int r) { return a.c[0][i][j][r] + a.c[1][i][j][r] * (1.f / LO); }
 
 // ---- packing
-__device__ __forceinline__ float max_or_nan(float m, float v) { return v > m || v != v ? v : m; }
-__device__ __forceinline__ void store_split16(char* out, int lane, const float (&y)[8]) {
-    const Split16 s = split16(y);
-    *reinterpret_cast<f16x8*>(out + lane * 16) = s.hi;
-    *reinterpret_cast<f16x8*>(out + FRAG + lane * 16) = s.lo;
-}
-
 // Fragments of x (D, N).  The first caseBlocks blocks take 16 cases each: (rows = cases, k = features) for the logits; the others 16
 // features each: (rows = features, k = cases) for the weight gradient, in which a case without a label is zero, whatever it holds.
 // Each block finds its rows' largest magnitudes first; what it reads then comes from its caches.
@@ -382,11 +447,13 @@ __global__ __launch_bounds__(512) void k_fcl_pack_x(const float* __restrict__ X,
         __syncthreads();
         const int e = exps[c];
         for (int kb = wave; kb < Kd; kb += 8) {
-            const int d0 = kb * 32 + g * 8;
             float y[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) y[j] = n < N && d0 + j < D ? ldexpf(X[(size_t)(d0 + j) * N + n], e) : 0.f;
-            store_split16(byCase + ((size_t)blockIdx.x * Kd + kb) * 2 * FRAG, lane, y);
+            for (int j = 0; j < 8; j++) {
+                const int d = kb * 32 + (j >> 2) * 16 + g * 4 + (j & 3);
+                y[j] = n < N && d < D ? ldexpf(X[(size_t)d * N + n], e) : 0.f;
+            }
+            store_pair(byCase + ((size_t)blockIdx.x * Kd + kb) * PAIR, lane, y);
         }
         return;
     }
@@ -405,38 +472,44 @@ __global__ __launch_bounds__(512) void k_fcl_pack_x(const float* __restrict__ X,
     __syncthreads();
     const int d = d0 + c, e = exps[c];
     for (int kb = wave; kb < Kn; kb += 8) {
-        const int n0 = kb * 32 + g * 8;
         float y[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
+            const int n = kb * 32 + (j >> 2) * 16 + g * 4 + (j & 3);
             int label;
-            y[j] = d < D && n0 + j < N && label_of(labels[n0 + j], V, label) ? ldexpf(X[(size_t)d * N + n0 + j], e) : 0.f;
+            y[j] = d < D && n < N && label_of(labels[n], V, label) ? ldexpf(X[(size_t)d * N + n], e) : 0.f;
         }
-        store_split16(byFeat + ((size_t)(d0 / 16) * Kn + kb) * 2 * FRAG, lane, y);
+        store_pair(byFeat + ((size_t)(d0 / 16) * Kn + kb) * PAIR, lane, y);
     }
 }
 
-// Fragments of a piece of W, 32 classes per block: (rows = classes, k = features, fp16) for the logits and, TRANS, (rows = features,
-// k = classes, bf16) for the input gradient.  k order of the latter: entry 8 g + j of a block of 32 is class 4 g + j (j < 4) or
-// 16 + 4 g + j - 4, which is how the lanes of the logits' tile hold them.  512 features at a time go through registers (all of a
-// thread's loads in flight at once) and LDS; rows of at most 512 features are read once, longer ones a second time for their max.
+// Fragments of a piece of W (rows = classes, k = features), 32 classes per block with one scale, a power of 2^8: its largest magnitude
+// comes to [2^7, 2^15), and neighbouring groups mostly share it (k_fcl_igrad).  A class that a bias of -inf takes out is zero, whatever
+// its weights hold.  512 features at a time go through registers (all of a thread's loads in flight at once) and LDS; rows of at most
+// 512 features are read once, longer ones a second time for their max.
 constexpr int CW = 512, CW_LD = CW + 4;
-template <bool TRANS>
-__global__ __launch_bounds__(512) void k_fcl_pack_w(const float* __restrict__ W, int* __restrict__ rowExp, char* __restrict__ byClass,
-                                                    char* __restrict__ byFeat, int D, int rows, int Kd, int Kv, int Dp) {
-    extern __shared__ __attribute__((aligned(16))) float tile[];  // [32][CW_LD], then 32 exponents
-    int* exps = reinterpret_cast<int*>(tile + 32 * CW_LD);
+constexpr int PACK_LDS = (32 * CW_LD + 8) * 4;
+__global__ __launch_bounds__(512) void k_fcl_pack_w(const float* __restrict__ W, const float* __restrict__ bias, int* __restrict__ classExp,
+                                                    char* __restrict__ byClass, int D, int rows, int Kd) {
+    extern __shared__ __attribute__((aligned(16))) float tile[];  // [32][CW_LD], then the waves' maxima
+    float* maxima = tile + 32 * CW_LD;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, v0 = blockIdx.x * 32, c = lane & 15, g = lane >> 4;
+    bool live[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const int v = v0 + wave * 4 + r;
+        live[r] = v < rows && (!bias || bias[v] != -INFINITY);
+    }
     f32x4 t[4][2];
     auto load = [&](int d0) {  // a wave: rows 4 wave .. + 3, a lane: features d0 + 4 lane .. and 256 further on
 #pragma unroll
         for (int r = 0; r < 4; r++)
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                const int v = v0 + wave * 4 + r, d = d0 + h * 256 + lane * 4;
-                const float* src = W + (size_t)v * D + d;
+                const int d = d0 + h * 256 + lane * 4;
+                const float* src = W + (size_t)(v0 + wave * 4 + r) * D + d;
                 f32x4 x = {0.f, 0.f, 0.f, 0.f};
-                if (v < rows) {
+                if (live[r]) {
                     if (d + 4 <= D) {
                         const f32x4u u = *reinterpret_cast<const f32x4u*>(src);
                         x = (f32x4){u[0], u[1], u[2], u[3]};
@@ -449,7 +522,7 @@ __global__ __launch_bounds__(512) void k_fcl_pack_w(const float* __restrict__ W,
                 t[r][h] = x;
             }
     };
-    float m[4] = {};
+    float m = 0.f;
     for (int d0 = 0; d0 < D; d0 += CW) {
         load(d0);
 #pragma unroll
@@ -457,96 +530,78 @@ __global__ __launch_bounds__(512) void k_fcl_pack_w(const float* __restrict__ W,
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) m[r] = max_or_nan(m[r], fabsf(t[r][h][j]));
+                for (int j = 0; j < 4; j++) m = max_or_nan(m, fabsf(t[r][h][j]));
     }
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-        for (int o = 1; o < 64; o <<= 1) m[r] = max_or_nan(m[r], __shfl_xor(m[r], o, 64));
-        if (lane == 0) rowExp[v0 + wave * 4 + r] = exps[wave * 4 + r] = scale_exp(m[r]);
-    }
-    const int Dt = TRANS ? Dp : Kd * 32;
-    for (int d0 = 0; d0 < Dt; d0 += CW) {
+    for (int o = 1; o < 64; o <<= 1) m = max_or_nan(m, __shfl_xor(m, o, 64));
+    if (lane == 0) maxima[wave] = m;
+    int e = 0;
+    for (int d0 = 0; d0 < Kd * 32; d0 += CW) {
         if (D > CW) load(d0);
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < 4; r++)
 #pragma unroll
             for (int h = 0; h < 2; h++) *reinterpret_cast<f32x4*>(tile + (wave * 4 + r) * CW_LD + h * 256 + lane * 4) = t[r][h];
+        if (d0 == 0) {
+            for (int w = 0; w < 8; w++) m = max_or_nan(m, maxima[w]);  // (every wave: the barrier above covers the maxima)
+            e = scale_exp(m) & ~7;
+            if (threadIdx.x == 0) classExp[blockIdx.x] = m == 0.f ? EXP_ZERO : e;
+        }
         __syncthreads();
         for (int f = wave; f < 2 * CW / 32; f += 8) {
             const int rb = f & 1, kb = d0 / 32 + (f >> 1), r = rb * 16 + c;
             if (kb >= Kd) break;
-            const f32x4* src = reinterpret_cast<const f32x4*>(tile + r * CW_LD + (f >> 1) * 32 + g * 8);
-            const f32x4 lo = src[0], hi = src[1];
-            const int e = exps[r];
             float y[8];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                y[j] = ldexpf(lo[j], e);
-                y[4 + j] = ldexpf(hi[j], e);
+            for (int h = 0; h < 2; h++) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(tile + r * CW_LD + (f >> 1) * 32 + h * 16 + g * 4);
+#pragma unroll
+                for (int j = 0; j < 4; j++) y[4 * h + j] = ldexpf(x[j], e);
             }
-            store_split16(byClass + (((size_t)blockIdx.x * 2 + rb) * Kd + kb) * 2 * FRAG, lane, y);
+            store_pair(byClass + (((size_t)blockIdx.x * 2 + rb) * Kd + kb) * PAIR, lane, y);
         }
-        if (TRANS)
-            for (int f = wave; f < CW / 16 && d0 + f * 16 < Dp; f += 8) {
-                float y[8];
-#pragma unroll
-                for (int j = 0; j < 8; j++) y[j] = tile[((j < 4 ? 0 : 12) + g * 4 + j) * CW_LD + f * 16 + c];
-                const Split24 s = split24(y);
-                char* out = byFeat + ((size_t)(d0 / 16 + f) * Kv + blockIdx.x) * 3 * FRAG + lane * 16;
-#pragma unroll
-                for (int q = 0; q < 3; q++) *reinterpret_cast<bf16x8*>(out + q * FRAG) = s.p[q];
-            }
     }
 }
-constexpr int PACK_LDS = (32 * CW_LD + 32) * 4;
 
 // ---- logits of a piece
 struct WideArgs {
     const char *wByClass, *xByCase;
-    const int *rowExp, *caseExp;
+    const int *classExp, *caseExp;
     const float *bias, *labels, *stats;
-    int V, N, v0, rows, Kd, vTiles, nTiles;
+    int V, N, v0, rows, Kd, kSteps, vTiles, nTiles;
     float *part, *labelLogits;  // forward: part + the piece's first tile
-    char *dzByCase, *dzByClass; // backward: (rows = cases, k = classes, bf16) and (rows = classes, k = cases, fp16), of dz / coeff
+    char* dz;                   // backward: dz / coeff, (rows = cases, k = classes)
     float* dbPart;              // backward: [nTiles][V], row sums of dz / coeff
-    int Kv, Kn;
+    int Kv;
 };
 
-constexpr int DZ_EXP = 14;                 // |dz / coeff| <= 1
-constexpr int DZ_LD = TILE + 4;
-constexpr int LOGIT_LDS = TILE * DZ_LD * 4;  // the dz tile; the product's two stages take 64 KB of it
-
-template <bool BWD>
-__global__ __launch_bounds__(256, 2) void k_fcl_logits(WideArgs p) {
+template <int MB, bool BWD>
+__global__ __launch_bounds__(256, 1) void k_fcl_logits(WideArgs p) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     // the tiles of one block of classes on one XCD: they read the same rows of W
     int tv, tn;
     mcn_xcd_group(blockIdx.x, p.nTiles, p.vTiles, tv, tn);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
     const int c = lane & 15, g = lane >> 4;
-    const size_t row = (size_t)p.Kd * 2 * FRAG;
-    Acc<2> acc;
-    product_tile<2>(p.wByClass + (size_t)tv * 8 * row, row, p.xByCase + (size_t)tn * 8 * row, row, 0, p.Kd, lds, acc);
-    const int vBase = tv * TILE + wm * 64, nBase = tn * TILE + wn * 64;
-    // z in place of the first accumulator; a class behind the last one gets -inf
+    const size_t row = (size_t)p.Kd * PAIR;
+    Acc<MB> acc;
+    product_tile<MB, false>(p.wByClass + (size_t)tv * 2 * MB * row, row, p.xByCase + (size_t)tn * 8 * row, row, 0, p.kSteps, lds, acc, NoScale());
+    const int vBase = tv * 32 * MB + wm * 16 * MB, nBase = tn * TILE + wn * 64;
+    int ex[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        int fw[4];
-        float bv[4];
+    for (int j = 0; j < 4; j++) ex[j] = p.caseExp[nBase + j * 16 + c];
+    // z in place of the first accumulator; a class behind the last one, or taken out by its bias, gets -inf
+#pragma unroll
+    for (int i = 0; i < MB; i++) {
+        const int ew = p.classExp[(vBase + i * 16) / 32];
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const int v = vBase + i * 16 + g * 4 + r;
-            fw[r] = p.rowExp[v];
-            bv[r] = v < p.rows ? (p.bias ? p.bias[p.v0 + v] : 0.f) : -INFINITY;
-        }
+            const float bv = v < p.rows ? (p.bias ? p.bias[p.v0 + v] : 0.f) : -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int e = p.caseExp[nBase + j * 16 + c];
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const float z = ldexpf(acc_value(acc, i, j, r), -(fw[r] + e));
-                acc.c[0][i][j][r] = bv[r] == -INFINITY && z == z ? -INFINITY : z + bv[r];
+            for (int j = 0; j < 4; j++) {
+                const float z = ew == EXP_ZERO ? acc.value(i, j, r) : ldexpf(acc.value(i, j, r), -(ew + ex[j]));
+                acc.c[0][i][j][r] = bv == -INFINITY && z == z ? -INFINITY : z + bv;
             }
         }
     }
@@ -560,7 +615,7 @@ __global__ __launch_bounds__(256, 2) void k_fcl_logits(WideArgs p) {
             if (n < p.N) label_of(p.labels[n], p.V, label);
             float m = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < MB; i++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const float z = acc.c[0][i][j][r];
@@ -571,7 +626,7 @@ __global__ __launch_bounds__(256, 2) void k_fcl_logits(WideArgs p) {
             for (int o = 16; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
             float rest = 0.f, cnt = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < MB; i++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const float z = acc.c[0][i][j][r];
@@ -606,6 +661,7 @@ __global__ __launch_bounds__(256, 2) void k_fcl_logits(WideArgs p) {
         }
         return;
     } else {
+        float sums[MB][4] = {};
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int n = nBase + j * 16 + c;
@@ -617,82 +673,57 @@ __global__ __launch_bounds__(256, 2) void k_fcl_logits(WideArgs p) {
             }
             const bool counts = S != 0.f;  // (no label, or no class left: nothing; a NaN goes on)
             const float inv = counts ? 1.f / S : 0.f;
+            char* out = p.dz + ((size_t)(nBase / 16 + j) * p.Kv + vBase / 32) * PAIR + lane * 8;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < MB; i++) {
+                f16x4 hi, lo;
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const float z = acc.c[0][i][j][r];
                     const float hot = label == p.v0 + vBase + i * 16 + g * 4 + r ? 1.f : 0.f;
-                    acc.c[0][i][j][r] = counts ? hot - (z == -INFINITY ? 0.f : expf(z - M) * inv) : 0.f;
+                    const float t = counts ? hot - (z == -INFINITY ? 0.f : expf(z - M) * inv) : 0.f;
+                    sums[i][r] += t;
+                    const float y = t * (float)(1 << DZ_EXP);
+                    hi[r] = (_Float16)y;
+                    lo[r] = (_Float16)((y - (float)hi[r]) * LO);
                 }
-            if (p.dzByCase) {
-#pragma unroll
-                for (int q = 0; q < 2; q++) {
-                    float y[8];
-#pragma unroll
-                    for (int k = 0; k < 8; k++) y[k] = acc.c[0][2 * q + (k >> 2)][j][k & 3];
-                    const Split24 s = split24(y);
-                    char* out = p.dzByCase + ((size_t)(nBase / 16 + j) * p.Kv + vBase / 32 + q) * 3 * FRAG + lane * 16;
-#pragma unroll
-                    for (int k = 0; k < 3; k++) *reinterpret_cast<bf16x8*>(out + k * FRAG) = s.p[k];
-                }
+                *reinterpret_cast<f16x4*>(out + (i >> 1) * PAIR + (i & 1) * 512) = hi;
+                *reinterpret_cast<f16x4*>(out + (i >> 1) * PAIR + FRAG + (i & 1) * 512) = lo;
             }
         }
-        // turned over in LDS for the weight gradient, whose sum runs over the cases; the row sums on the way
-        __syncthreads();
-        float* T = reinterpret_cast<float*>(lds);
+        if (p.dbPart) {  // row sums: over the lanes of a row, then the two waves of 64 cases
+            __syncthreads();
+            float(*rowSum)[32 * MB] = reinterpret_cast<float(*)[32 * MB]>(lds);
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+            for (int i = 0; i < MB; i++)
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) T[(wm * 64 + i * 16 + g * 4 + r) * DZ_LD + wn * 64 + j * 16 + c] = acc.c[0][i][j][r];
-        __syncthreads();
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int vb = wave * 2 + u;
-            float sum = 0.f;
-#pragma unroll
-            for (int kb = 0; kb < 4; kb++) {
-                const f32x4* src = reinterpret_cast<const f32x4*>(T + (vb * 16 + c) * DZ_LD + kb * 32 + g * 8);
-                const f32x4 lo = src[0], hi = src[1];
-                float y[8];
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    y[k] = lo[k] * (float)(1 << DZ_EXP);
-                    y[4 + k] = hi[k] * (float)(1 << DZ_EXP);
+                for (int r = 0; r < 4; r++) {
+                    float t = sums[i][r];
+                    for (int o = 1; o < 16; o <<= 1) t += __shfl_xor(t, o, 64);
+                    if (c == 0) rowSum[wn][wm * 16 * MB + i * 16 + g * 4 + r] = t;
                 }
-                sum += ((lo[0] + lo[1]) + (lo[2] + lo[3])) + ((hi[0] + hi[1]) + (hi[2] + hi[3]));
-                if (p.dzByClass) {
-                    const Split16 s = split16(y);
-                    char* out = p.dzByClass + ((size_t)(tv * 8 + vb) * p.Kn + tn * 4 + kb) * 2 * FRAG + lane * 16;
-                    *reinterpret_cast<f16x8*>(out) = s.hi;
-                    *reinterpret_cast<f16x8*>(out + FRAG) = s.lo;
-                }
-            }
-            sum += __shfl_xor(sum, 16, 64);
-            sum += __shfl_xor(sum, 32, 64);
-            const int v = tv * TILE + vb * 16 + c;
-            if (p.dbPart && g == 0 && v < p.rows) p.dbPart[(size_t)tn * p.V + p.v0 + v] = sum;
+            __syncthreads();
+            const int t = threadIdx.x, v = tv * 32 * MB + t;
+            if (t < 32 * MB && v < p.rows) p.dbPart[(size_t)tn * p.V + p.v0 + v] = rowSum[0][t] + rowSum[1][t];
         }
     }
 }
 
 // ---- weight gradient of a piece: (features x classes) tiles, so that a lane's four rows are four neighbours of one row of W
-__global__ __launch_bounds__(256, 2) void k_fcl_wgrad(const char* xByFeat, const char* dzByClass, const int* __restrict__ featExp,
-                                                      float* __restrict__ dW, int D, int rows, int Kn, int dTiles, int vTiles, float scaleTargets,
-                                                      float scaleOutput) {
+template <int MB>
+__global__ __launch_bounds__(256, 1) void k_fcl_wgrad(const char* xByFeat, const char* dz, const int* __restrict__ featExp, float* __restrict__ dW,
+                                                      int D, int rows, int Kn, int Kv, int dTiles, int vTiles, float scaleTargets, float scaleOutput) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     int tv, td;
     mcn_xcd_group(blockIdx.x, dTiles, vTiles, tv, td);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
     const int c = lane & 15, g = lane >> 4;
-    const size_t row = (size_t)Kn * 2 * FRAG;
-    Acc<2> acc;
-    product_tile<2>(xByFeat + (size_t)td * 8 * row, row, dzByClass + (size_t)tv * 8 * row, row, 0, Kn, lds, acc);
+    const size_t row = (size_t)Kn * PAIR;
+    Acc<MB> acc;
+    product_tile<MB, true>(xByFeat + (size_t)td * 2 * MB * row, row, dz + (size_t)tv * 4 * PAIR, (size_t)Kv * PAIR, 0, Kn, lds, acc, NoScale());
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int d = td * TILE + wm * 64 + i * 16 + g * 4;
+    for (int i = 0; i < MB; i++) {
+        const int d = td * 32 * MB + wm * 16 * MB + i * 16 + g * 4;
         int e[4];
 #pragma unroll
         for (int r = 0; r < 4; r++) e[r] = -(featExp[d + r] + DZ_EXP);
@@ -703,7 +734,7 @@ __global__ __launch_bounds__(256, 2) void k_fcl_wgrad(const char* xByFeat, const
             float* out = dW + (size_t)v * D + d;
             float y[4];
 #pragma unroll
-            for (int r = 0; r < 4; r++) y[r] = scaleOutput * ldexpf(acc_value(acc, i, j, r), e[r]);
+            for (int r = 0; r < 4; r++) y[r] = scaleOutput * ldexpf(acc.value(i, j, r), e[r]);
             if (d + 4 <= D) {
                 f32x4u t = {y[0], y[1], y[2], y[3]};
                 if (scaleTargets != 0.f) {
@@ -721,23 +752,60 @@ __global__ __launch_bounds__(256, 2) void k_fcl_wgrad(const char* xByFeat, const
     }
 }
 
+// The accumulators are in units of 2^-(exponent of the group they last added): when the next 32 classes have another scale, they are
+// brought to it, exactly, by a power of two.  A group of zeros has none.  Exponents come 64 at a time into a register of the lanes.
+struct CarryScale {
+    const int* exps;  // of the product's k blocks, from k0 on
+    int count;
+    mutable int held, cur;
+    __device__ __forceinline__ CarryScale(const int* e, int n) : exps(e), count(n), held(load(0)), cur(EXP_ZERO) {}
+    __device__ __forceinline__ int load(int t) const {
+        const int i = t + (int)(threadIdx.x & 63);
+        return i < count ? exps[i] : EXP_ZERO;
+    }
+    template <int MB>
+    __device__ __forceinline__ void operator()(int t, Acc<MB>& acc) const {
+        if (t > 0 && (t & 63) == 0) held = load(t);
+        const int e = __builtin_amdgcn_readlane(held, t & 63);
+        if (e == EXP_ZERO || e == cur) return;
+        if (cur != EXP_ZERO) {
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int i = 0; i < MB; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) acc.c[h][i][j][r] = ldexpf(acc.c[h][i][j][r], e - cur);
+        }
+        cur = e;
+    }
+};
+
 // ---- input gradient: the sum over the classes is split; slab s of (Dp, Np) adds up its share of every piece, in order
-__global__ __launch_bounds__(256, 1) void k_fcl_igrad(const char* dzByCase, const char* wByFeat, float* __restrict__ slabs, int Np, int Dp,
-                                                      int Kv, int kPerSplit, int nTiles, int dTiles, int first) {
+template <int MB>
+__global__ __launch_bounds__(256, 1) void k_fcl_igrad(const char* dz, const char* wByClass, const int* __restrict__ classExp, float* __restrict__ slabs,
+                                                      int Np, int Dp, int Kv, int Kd, int kPerSplit, int nTiles, int dTiles, int first) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int tiles = nTiles * dTiles, s = blockIdx.x / tiles, t = blockIdx.x % tiles, td = t / nTiles, tn = t % nTiles;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
     const int c = lane & 15, g = lane >> 4;
-    const size_t row = (size_t)Kv * 3 * FRAG;
-    Acc<3> acc;
-    product_tile<3>(dzByCase + (size_t)tn * 8 * row, row, wByFeat + (size_t)td * 8 * row, row, s * kPerSplit, min(Kv, (s + 1) * kPerSplit), lds, acc);
+    const size_t row = (size_t)Kv * PAIR;
+    const int k0 = s * kPerSplit, k1 = min(Kv, k0 + kPerSplit);
+    Acc<MB> acc;
+    const CarryScale carry(classExp + k0, k1 - k0);
+    product_tile<MB, true>(dz + (size_t)tn * 2 * MB * row, row, wByClass + (size_t)td * 4 * PAIR, (size_t)Kd * PAIR, k0, k1, lds, acc, carry);
+    const int e = carry.cur == EXP_ZERO ? 0 : -(carry.cur + DZ_EXP);
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+    for (int i = 0; i < MB; i++)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const int d = td * TILE + wn * 64 + j * 16 + c, n = tn * TILE + wm * 64 + i * 16 + g * 4;
+            const int d = td * TILE + wn * 64 + j * 16 + c, n = tn * 32 * MB + wm * 16 * MB + i * 16 + g * 4;
             f32x4* out = reinterpret_cast<f32x4*>(slabs + ((size_t)s * Dp + d) * Np + n);
-            *out = first ? acc.c[0][i][j] : *out + acc.c[0][i][j];
+            f32x4 y;
+#pragma unroll
+            for (int r = 0; r < 4; r++) y[r] = ldexpf(acc.value(i, j, r), e);
+            *out = first ? y : *out + y;
         }
 }
 
@@ -763,13 +831,31 @@ __global__ __launch_bounds__(256) void k_fcl_finish(const float* __restrict__ sl
     dB[v] = (scaleBiasTargets != 0.f ? scaleBiasTargets * dB[v] : 0.f) + scaleBiasOutput * coeff * s;
 }
 
+// Rows of a product's tile / 32: the whole launch runs in rounds of one tile per CU, and a tile costs its rows plus a fixed part (the
+// fill of its stages, its epilogue) of about 32 rows.  With 256 rows an LDS byte feeds 1.5 times the matrix work that it does with 128.
+int tile_choice(int rows32, int colTiles) {
+    int best = 2;
+    long cost = -1;
+    for (int mb : {8, 4, 2}) {
+        const long c = (long)divup(divup(rows32, mb) * colTiles, 256) * (mb + 1);
+        if (cost < 0 || c < cost) {
+            cost = c;
+            best = mb;
+        }
+    }
+    return best;
+}
+
 // Sizes and workspace of the wide path: a function of the shape alone.
 struct WidePlan {
-    int Np, Dp, Kd, Kn, nTiles, dTiles;
-    int rows, pieces;        // classes per piece (a multiple of TILE), pieces
-    int splits, kPerSplit;   // input gradient
-    size_t rowExp, caseExp, featExp, xByCase, xByFeat, wByClass, wByFeat, dzByCase, dzByClass, dbPart, slabs, part, labelLogits, total;
+    int Np, Dp, Kd, kSteps, Kn, nTiles, dTiles;  // Kd: k blocks of W's and x's fragments, padded; kSteps: those that hold anything
+    int rows, Kv;                                // classes per piece; k blocks of a whole piece, padded
+    int mbWgrad, mbIgrad;
+    int splits;                                  // input gradient
+    size_t classExp, caseExp, featExp, xByCase, xByFeat, wByClass, dz, dbPart, slabs, part, labelLogits, total;
 };
+// rows of a piece padded to whole tiles of either kind
+int padded_rows(int rows, int mb) { return divup(rows, std::max(TILE, 32 * mb)) * std::max(TILE, 32 * mb); }
 
 bool wide_usable(int D, int V, int N) { return N > 48; }
 
@@ -779,65 +865,93 @@ WidePlan wide_plan(int D, int V, int N, bool bwd) {
     WidePlan p = {};
     p.nTiles = divup(N, TILE);
     p.dTiles = divup(D, TILE);
-    p.Np = p.nTiles * TILE;
-    p.Dp = p.dTiles * TILE;
-    p.Kd = divup(D, 32);
+    p.kSteps = divup(D, 32);
+    p.Kd = p.dTiles * 4;
+    // a piece's fragments should stay in the 256 MB last-level cache between the launches that write and read them; whole rounds of
+    // 256-row tiles where the classes fill some
+    const size_t perRow = (size_t)p.Kd * 128 + (bwd ? (size_t)p.nTiles * TILE * 4 : 0);
+    const int most = (int)std::max<size_t>(TILE, std::min<size_t>(((size_t)128 << 20) / perRow / 256 * 256, (size_t)1 << 17));
+    const int round = std::max(1, 256 / p.nTiles) * 256;
+    p.rows = std::min(V, most > round ? most / round * round : most);
+    const int v32 = divup(p.rows, 32);
+    p.Kv = std::max({padded_rows(p.rows, 8), padded_rows(p.rows, 4)}) / 32;
+    p.mbIgrad = 4;
+    if (p.nTiles % 2 == 0) p.mbIgrad = 8;
+    p.mbWgrad = tile_choice(divup(D, 32), divup(v32, 4));
+    p.Np = divup(N, std::max(TILE, 32 * p.mbIgrad)) * std::max(TILE, 32 * p.mbIgrad);
+    p.Dp = divup(D, std::max(TILE, 32 * p.mbWgrad)) * std::max(TILE, 32 * p.mbWgrad);
     p.Kn = p.Np / 32;
-    // a piece's fragments should stay in the 256 MB last-level cache between the launches that write and read them
-    const size_t perRow = (size_t)p.Kd * 128 + (bwd ? (size_t)p.Dp * 6 + (size_t)p.Np * 10 : 0);
-    const int most = (int)std::max<size_t>(1, std::min<size_t>(((size_t)128 << 20) / perRow / TILE, (size_t)1 << 16));
-    p.pieces = divup(divup(V, TILE), most);
-    p.rows = divup(divup(V, TILE), p.pieces) * TILE;
-    p.pieces = divup(V, p.rows);
-    const int Kv = p.rows / 32;
-    p.splits = std::max(1, std::min(Kv / 8, 256 / (p.nTiles * p.dTiles)));
-    p.kPerSplit = divup(Kv, p.splits);
-    p.splits = divup(Kv, p.kPerSplit);
+    p.splits = std::max(1, std::min(p.Kv / 8, 256 / (p.Np / (32 * p.mbIgrad) * p.dTiles)));
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t o = at; at += al256(bytes); return o; };
-    p.rowExp = take((size_t)p.rows * 4);
+    p.classExp = take((size_t)p.Kv * 4);
     p.caseExp = take((size_t)p.Np * 4);
-    p.featExp = take((size_t)p.Dp * 4);
-    p.xByCase = take((size_t)p.Np / 16 * p.Kd * 2 * FRAG);
-    p.wByClass = take((size_t)p.rows / 16 * p.Kd * 2 * FRAG);
+    p.xByCase = take((size_t)p.Np / 16 * p.Kd * PAIR);
+    p.wByClass = take((size_t)p.Kv * 2 * p.Kd * PAIR);
     if (bwd) {
-        p.xByFeat = take((size_t)p.Dp / 16 * p.Kn * 2 * FRAG);
-        p.wByFeat = take((size_t)p.Dp / 16 * Kv * 3 * FRAG);
-        p.dzByCase = take((size_t)p.Np / 16 * Kv * 3 * FRAG);
-        p.dzByClass = take((size_t)p.rows / 16 * p.Kn * 2 * FRAG);
+        p.featExp = take((size_t)p.Dp * 4);
+        p.xByFeat = take((size_t)p.Dp / 16 * p.Kn * PAIR);
+        p.dz = take((size_t)p.Np / 16 * p.Kv * PAIR);
         p.dbPart = take((size_t)p.nTiles * V * 4);
-        p.slabs = take((size_t)p.splits * p.Dp * p.Np * 4);
+        p.slabs = take((size_t)p.splits * p.dTiles * TILE * p.Np * 4);
     } else {
-        p.part = take((size_t)p.pieces * (p.rows / TILE) * 3 * N * 4);
+        p.part = take((size_t)(divup(V, 64) + divup(V, p.rows) * 4) * 3 * N * 4);
         p.labelLogits = take((size_t)N * 4);
     }
     p.total = at;
     return p;
 }
 
-int wide_cost(const float* W, const float* X, const float* bias, const float* labels, float* stats, float* logp, float* correct, int D, int V,
-              int N, char* ws, hipStream_t s) {
-    const WidePlan q = wide_plan(D, V, N, false);
+template <bool BWD>
+void launch_logits(int mb, const WideArgs& a, hipStream_t s) {
+    const dim3 grid(a.vTiles * a.nTiles), block(256);
+    switch (mb) {
+        case 8: MCN_LAUNCH((k_fcl_logits<8, BWD>), grid, block, tile_lds(8), s, a); break;
+        case 4: MCN_LAUNCH((k_fcl_logits<4, BWD>), grid, block, tile_lds(4), s, a); break;
+        default: MCN_LAUNCH((k_fcl_logits<2, BWD>), grid, block, tile_lds(2), s, a); break;
+    }
+}
+
+WideArgs wide_args(const WidePlan& q, const float* bias, const float* labels, int V, int N, char* ws) {
     WideArgs a = {};
     a.wByClass = ws + q.wByClass;
     a.xByCase = ws + q.xByCase;
-    a.rowExp = (const int*)(ws + q.rowExp);
+    a.classExp = (const int*)(ws + q.classExp);
     a.caseExp = (const int*)(ws + q.caseExp);
-    a.bias = bias; a.labels = labels; a.V = V; a.N = N; a.Kd = q.Kd; a.nTiles = q.nTiles;
+    a.bias = bias;
+    a.labels = labels;
+    a.V = V;
+    a.N = N;
+    a.Kd = q.Kd;
+    a.kSteps = q.kSteps;
+    return a;
+}
+// one piece: its packed rows, tiles and k blocks
+int wide_piece(const WidePlan& q, WideArgs& a, const float* W, int D, int v0, char* ws, hipStream_t s) {
+    a.v0 = v0;
+    a.rows = std::min(q.rows, a.V - v0);
+    a.nTiles = q.nTiles;
+    const int mb = tile_choice(divup(a.rows, 32), q.nTiles), padded = padded_rows(a.rows, mb);
+    a.vTiles = padded / (32 * mb);
+    a.Kv = padded / 32;
+    MCN_LAUNCH(k_fcl_pack_w, dim3(a.Kv), dim3(512), PACK_LDS, s, W + (size_t)v0 * D, a.bias ? a.bias + v0 : nullptr, (int*)(ws + q.classExp),
+               ws + q.wByClass, D, a.rows, q.Kd);
+    return mb;
+}
+
+int wide_cost(const float* W, const float* X, const float* bias, const float* labels, float* stats, float* logp, float* correct, int D, int V,
+              int N, char* ws, hipStream_t s) {
+    const WidePlan q = wide_plan(D, V, N, false);
+    WideArgs a = wide_args(q, bias, labels, V, N, ws);
     a.labelLogits = (float*)(ws + q.labelLogits);
     MCN_LAUNCH(k_fcl_pack_x, dim3(q.Np / 16), dim3(512), 0, s, X, labels, (int*)(ws + q.caseExp), (int*)nullptr, ws + q.xByCase, (char*)nullptr,
                D, V, N, q.Kd, q.Kn, q.Np / 16);
     int tiles = 0;
     for (int v0 = 0; v0 < V; v0 += q.rows) {
-        const int rows = std::min(q.rows, V - v0), vTiles = divup(rows, TILE);
-        MCN_LAUNCH(k_fcl_pack_w<false>, dim3(vTiles * (TILE / 32)), dim3(512), PACK_LDS, s, W + (size_t)v0 * D, (int*)(ws + q.rowExp), ws + q.wByClass,
-                   (char*)nullptr, D, rows, q.Kd, vTiles * (TILE / 32), q.Dp);
-        a.v0 = v0;
-        a.rows = rows;
-        a.vTiles = vTiles;
+        const int mb = wide_piece(q, a, W, D, v0, ws, s);
         a.part = (float*)(ws + q.part) + (size_t)tiles * 3 * N;
-        MCN_LAUNCH(k_fcl_logits<false>, dim3(vTiles * q.nTiles), dim3(256), LOGIT_LDS, s, a);
-        tiles += vTiles;
+        launch_logits<false>(mb, a, s);
+        tiles += a.vTiles;
         if (int rc = MCN_LAUNCH_CHECK("fcLogregCost")) return rc;
     }
     MCN_LAUNCH(k_fcl_join, dim3(divup(N, 16)), dim3(1024), 0, s, (const float*)(ws + q.part), a.labelLogits, labels, stats, logp, correct, V, N, tiles);
@@ -848,42 +962,42 @@ int wide_grad(const float* W, const float* X, const float* bias, const float* la
               int V, int N, float coeff, float scaleInputTargets, float scaleWeightTargets, float scaleWeightOutput, float scaleBiasTargets,
               float scaleBiasOutput, char* ws, hipStream_t s) {
     const WidePlan q = wide_plan(D, V, N, true);
-    WideArgs a = {};
-    a.wByClass = ws + q.wByClass;
-    a.xByCase = ws + q.xByCase;
-    a.rowExp = (const int*)(ws + q.rowExp);
-    a.caseExp = (const int*)(ws + q.caseExp);
-    a.bias = bias; a.labels = labels; a.stats = stats; a.V = V; a.N = N; a.Kd = q.Kd; a.nTiles = q.nTiles; a.Kn = q.Kn;
-    a.dzByCase = dX ? ws + q.dzByCase : nullptr;
-    a.dzByClass = dW ? ws + q.dzByClass : nullptr;
+    WideArgs a = wide_args(q, bias, labels, V, N, ws);
+    a.stats = stats;
+    a.dz = ws + q.dz;
     a.dbPart = dB ? (float*)(ws + q.dbPart) : nullptr;
+    const int* featExp = (const int*)(ws + q.featExp);
+    float* slabs = (float*)(ws + q.slabs);
     MCN_LAUNCH(k_fcl_pack_x, dim3(q.Np / 16 + (dW ? q.Dp / 16 : 0)), dim3(512), 0, s, X, labels, (int*)(ws + q.caseExp), (int*)(ws + q.featExp),
                ws + q.xByCase, ws + q.xByFeat, D, V, N, q.Kd, q.Kn, q.Np / 16);
     for (int v0 = 0; v0 < V; v0 += q.rows) {
-        const int rows = std::min(q.rows, V - v0), vTiles = divup(rows, TILE), Kv = vTiles * (TILE / 32);
-        if (dX)
-            MCN_LAUNCH(k_fcl_pack_w<true>, dim3(Kv), dim3(512), PACK_LDS, s, W + (size_t)v0 * D, (int*)(ws + q.rowExp), ws + q.wByClass,
-                       ws + q.wByFeat, D, rows, q.Kd, Kv, q.Dp);
-        else
-            MCN_LAUNCH(k_fcl_pack_w<false>, dim3(Kv), dim3(512), PACK_LDS, s, W + (size_t)v0 * D, (int*)(ws + q.rowExp), ws + q.wByClass,
-                       ws + q.wByFeat, D, rows, q.Kd, Kv, q.Dp);
-        a.v0 = v0;
-        a.rows = rows;
-        a.vTiles = vTiles;
-        a.Kv = Kv;
-        MCN_LAUNCH(k_fcl_logits<true>, dim3(vTiles * q.nTiles), dim3(256), LOGIT_LDS, s, a);
-        if (dW)
-            MCN_LAUNCH(k_fcl_wgrad, dim3(vTiles * q.dTiles), dim3(256), 2 * 32 * FRAG, s, ws + q.xByFeat, a.dzByClass, (const int*)(ws + q.featExp),
-                       dW + (size_t)v0 * D, D, rows, q.Kn, q.dTiles, vTiles, scaleWeightTargets, scaleWeightOutput * coeff);
-        if (dX)
-            MCN_LAUNCH(k_fcl_igrad, dim3(q.splits * q.nTiles * q.dTiles), dim3(256), 2 * 48 * FRAG, s, a.dzByCase, ws + q.wByFeat,
-                       (float*)(ws + q.slabs), q.Np, q.Dp, Kv, q.kPerSplit, q.nTiles, q.dTiles, v0 == 0);
+        const int mb = wide_piece(q, a, W, D, v0, ws, s);
+        launch_logits<true>(mb, a, s);
+        if (dW) {
+            const int vTiles = a.Kv / 4, dTiles = q.Dp / (32 * q.mbWgrad);
+            const dim3 grid(vTiles * dTiles), block(256);
+            const float sO = scaleWeightOutput * coeff;
+            float* out = dW + (size_t)v0 * D;
+#define WGRAD(MB) MCN_LAUNCH((k_fcl_wgrad<MB>), grid, block, tile_lds(MB), s, ws + q.xByFeat, a.dz, featExp, out, D, a.rows, q.Kn, a.Kv, dTiles, vTiles, scaleWeightTargets, sO)
+            if (q.mbWgrad == 8) WGRAD(8);
+            else if (q.mbWgrad == 4) WGRAD(4);
+            else WGRAD(2);
+#undef WGRAD
+        }
+        if (dX) {
+            const int nTiles = q.Np / (32 * q.mbIgrad), kPer = divup(a.Kv, q.splits);
+            const dim3 grid(q.splits * nTiles * q.dTiles), block(256);
+#define IGRAD(MB) MCN_LAUNCH((k_fcl_igrad<MB>), grid, block, tile_lds(MB), s, a.dz, a.wByClass, a.classExp, slabs, q.Np, q.dTiles * TILE, a.Kv, q.Kd, kPer, nTiles, q.dTiles, v0 == 0)
+            if (q.mbIgrad == 8) IGRAD(8);
+            else IGRAD(4);
+#undef IGRAD
+        }
         if (int rc = MCN_LAUNCH_CHECK("fcLogregGrad")) return rc;
     }
     if (dX || dB) {
         const int dxBlocks = dX ? (int)divup_sz((size_t)D * N, 256) : 0;
-        MCN_LAUNCH(k_fcl_finish, dim3(dxBlocks + (dB ? divup(V, 256) : 0)), dim3(256), 0, s, (const float*)(ws + q.slabs), (const float*)(ws + q.dbPart),
-                   dX, dB, D, V, N, q.Np, q.Dp, q.splits, q.nTiles, dxBlocks, coeff, scaleInputTargets, scaleBiasTargets, scaleBiasOutput);
+        MCN_LAUNCH(k_fcl_finish, dim3(dxBlocks + (dB ? divup(V, 256) : 0)), dim3(256), 0, s, slabs, (const float*)(ws + q.dbPart), dX, dB, D, V, N, q.Np,
+                   q.dTiles * TILE, q.splits, q.nTiles, dxBlocks, coeff, scaleInputTargets, scaleBiasTargets, scaleBiasOutput);
     }
     return MCN_LAUNCH_CHECK("fcLogregGrad");
 }
