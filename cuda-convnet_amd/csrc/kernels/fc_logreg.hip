@@ -563,6 +563,16 @@ __global__ __launch_bounds__(512) void k_fcl_pack_w(const float* __restrict__ W,
     }
 }
 
+// exp(x) for x <= 0, to about one unit in the last place: 2^(x log2 e) with the product's rounding error carried along.  Below -104 the
+// result is no normal number, and 0 will do; a NaN comes through.
+__device__ __forceinline__ float exp_neg(float x) {
+    constexpr float L = 1.44269504f, L_LOW = 1.925963033500e-8f, LN2 = 0.693147181f;  // log2 e = L + L_LOW
+    x = x < -104.f ? -104.f : x;
+    const float h = x * L, l = fmaf(x, L_LOW, fmaf(x, L, -h));
+    const float e = __builtin_amdgcn_exp2f(h);
+    return fmaf(e * LN2, l, e);
+}
+
 // ---- logits of a piece
 struct WideArgs {
     const char *wByClass, *xByCase;
@@ -587,55 +597,68 @@ __global__ __launch_bounds__(256, 1) void k_fcl_logits(WideArgs p) {
     Acc<MB> acc;
     product_tile<MB, false>(p.wByClass + (size_t)tv * 2 * MB * row, row, p.xByCase + (size_t)tn * 8 * row, row, 0, p.kSteps, lds, acc, NoScale());
     const int vBase = tv * 32 * MB + wm * 16 * MB, nBase = tn * TILE + wn * 64;
-    int ex[4];
+    // z in place of the first accumulator.  A class behind the last one, or taken out by its bias, has fragments of zeros: -inf.
+    int ex[4], label[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) ex[j] = p.caseExp[nBase + j * 16 + c];
-    // z in place of the first accumulator; a class behind the last one, or taken out by its bias, gets -inf
+    for (int j = 0; j < 4; j++) {
+        const int n = nBase + j * 16 + c;
+        ex[j] = p.caseExp[n];
+        label[j] = -1;
+        if (n < p.N) label_of(p.labels[n], p.V, label[j]);
+    }
 #pragma unroll
     for (int i = 0; i < MB; i++) {
-        const int ew = p.classExp[(vBase + i * 16) / 32];
+        const int we = p.classExp[(vBase + i * 16) / 32], ew = we == EXP_ZERO ? 0 : we;
+        float bv[4];
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const int v = vBase + i * 16 + g * 4 + r;
-            const float bv = v < p.rows ? (p.bias ? p.bias[p.v0 + v] : 0.f) : -INFINITY;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float z = ew == EXP_ZERO ? acc.value(i, j, r) : ldexpf(acc.value(i, j, r), -(ew + ex[j]));
-                acc.c[0][i][j][r] = bv == -INFINITY && z == z ? -INFINITY : z + bv;
-            }
+            bv[r] = v < p.rows ? (p.bias ? p.bias[p.v0 + v] : 0.f) : -INFINITY;
         }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) acc.c[0][i][j][r] = ldexpf(acc.value(i, j, r), -(ew + ex[j])) + bv[r];
+    }
+    // where the label's entry lies among a lane's 4 MB rows, if it does: row 16 i + r from here
+    int at[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        at[j] = label[j] - (p.v0 + vBase + g * 4);
+        if (label[j] < 0 || at[j] < 0 || at[j] >= 16 * MB || (at[j] & 15) > 3) at[j] = -1;
     }
     if constexpr (!BWD) {
         __syncthreads();
         float(*red)[3][64] = reinterpret_cast<float(*)[3][64]>(lds);  // [wave][max, rest, count][64 cases]
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const int n = nBase + j * 16 + c;
-            int label = -1;
-            if (n < p.N) label_of(p.labels[n], p.V, label);
             float m = -INFINITY;
 #pragma unroll
             for (int i = 0; i < MB; i++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float z = acc.c[0][i][j][r];
-                    m = z > m ? z : m;
-                    const int v = vBase + i * 16 + g * 4 + r;
-                    if (label == p.v0 + v && v < p.rows) p.labelLogits[n] = z;
-                }
+                for (int r = 0; r < 4; r += 2) m = fmaxf(fmaxf(acc.c[0][i][j][r], acc.c[0][i][j][r + 1]), m);
+            if (__any(at[j] >= 0)) {
+#pragma unroll
+                for (int i = 0; i < MB; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (at[j] == i * 16 + r) p.labelLogits[nBase + j * 16 + c] = acc.c[0][i][j][r];
+            }
             for (int o = 16; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-            float rest = 0.f, cnt = 0.f;
+            const float from = m == -INFINITY ? 0.f : m;
+            float rest = 0.f;
+            int tops = 0;
 #pragma unroll
             for (int i = 0; i < MB; i++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const float z = acc.c[0][i][j][r];
-                    const bool top = z == m && m < INFINITY;
-                    if (z != -INFINITY) {
-                        rest += top ? 0.f : expf(z - m);
-                        cnt += top ? 1.f : 0.f;
-                    }
+                    const float x = acc.c[0][i][j][r] - from;
+                    const bool top = x == 0.f && m != -INFINITY;
+                    const float e = exp_neg(x);
+                    rest += top ? 0.f : e;
+                    tops += top ? 1 : 0;
                 }
+            float cnt = (float)tops;
             for (int o = 16; o < 64; o <<= 1) {
                 rest += __shfl_xor(rest, o, 64);
                 cnt += __shfl_xor(cnt, o, 64);
@@ -665,23 +688,33 @@ __global__ __launch_bounds__(256, 1) void k_fcl_logits(WideArgs p) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int n = nBase + j * 16 + c;
-            int label = -1;
             float M = 0.f, S = 0.f;
-            if (n < p.N && label_of(p.labels[n], p.V, label)) {
+            if (label[j] >= 0) {
                 M = p.stats[n];
                 S = p.stats[p.N + n];
             }
             const bool counts = S != 0.f;  // (no label, or no class left: nothing; a NaN goes on)
             const float inv = counts ? 1.f / S : 0.f;
+#pragma unroll
+            for (int i = 0; i < MB; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float t = -exp_neg(acc.c[0][i][j][r] - M) * inv;
+                    acc.c[0][i][j][r] = counts ? t : 0.f;
+                }
+            if (__any(at[j] >= 0 && counts)) {
+#pragma unroll
+                for (int i = 0; i < MB; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) acc.c[0][i][j][r] += counts && at[j] == i * 16 + r ? 1.f : 0.f;
+            }
             char* out = p.dz + ((size_t)(nBase / 16 + j) * p.Kv + vBase / 32) * PAIR + lane * 8;
 #pragma unroll
             for (int i = 0; i < MB; i++) {
                 f16x4 hi, lo;
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const float z = acc.c[0][i][j][r];
-                    const float hot = label == p.v0 + vBase + i * 16 + g * 4 + r ? 1.f : 0.f;
-                    const float t = counts ? hot - (z == -INFINITY ? 0.f : expf(z - M) * inv) : 0.f;
+                    const float t = acc.c[0][i][j][r];
                     sums[i][r] += t;
                     const float y = t * (float)(1 << DZ_EXP);
                     hi[r] = (_Float16)y;
