@@ -419,6 +419,66 @@ __device__ __forceinline__ void product_tile(const char* A, size_t aRow, const c
     wait_copies_and_meet<0>();  // the buffers are free again
 }
 
+// The same product on 128 x 128 tiles with two blocks per CU: half the registers, so a stage's fragments are read in the step that
+// multiplies them, and two stages of LDS.  For the logits, whose epilogue (an exponential per entry) takes as long as their products:
+// one block's epilogue runs next to the other's products.
+constexpr int SHARED_LDS = 2 * tile_units(4) * PAIR;
+__device__ __forceinline__ void product_tile_shared(const char* A, size_t aRow, const char* B, size_t bRow, int k0, int k1, char* lds, Acc<4>& acc) {
+    constexpr int UNITS = tile_units(4), STAGE = UNITS * PAIR, MINE = UNITS / 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave >> 1, wn = wave & 1;
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc.c[h][i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    int n = k1 - k0;
+    if (n <= 0) return;
+    const char* src[MINE];
+#pragma unroll
+    for (int i = 0; i < MINE; i++) {
+        const int u = wave * MINE + i, w = u - 8;
+        src[i] = (u < 8 ? A + (size_t)u * aRow : B + (size_t)w * bRow) + (size_t)k0 * PAIR;
+        asm volatile("" : "+s"(src[i]));
+    }
+    asm volatile("" : "+s"(n));
+    const unsigned ldsBase = __builtin_amdgcn_readfirstlane((unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)lds) + wave * MINE * PAIR;
+    const unsigned laneOff = lane * 16;
+    const char* mine = lds + lane * 8;
+    unsigned fill = 0, take = 0;
+    auto copy = [&] {
+#pragma unroll
+        for (int o = 0; o < 2 * MINE; o++) copy_pair_half(src[o >> 1], ldsBase + fill + (o >> 1) * PAIR, laneOff, o & 1);
+#pragma unroll
+        for (int i = 0; i < MINE; i++) src[i] += PAIR;
+        fill ^= STAGE;
+    };
+    copy();
+    for (int t = 0; t < n; t++) {
+        wait_copies_and_meet<0>();  // stage t has landed, and everyone has read the other buffer
+        Frags<4> f;
+        const char* s = mine + take;
+        take ^= STAGE;
+#pragma unroll
+        for (int q = 0; q < 2; q++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) f.b[j][q] = read_frag(s + (8 + wn * 4 + j) * PAIR + q * FRAG);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int q = 0; q < 2; q++) f.a[i][q] = read_frag(s + (wm * 4 + i) * PAIR + q * FRAG);
+        if (t + 1 < n) copy();
+#pragma unroll
+        for (int m = 0; m < 48; m++) {
+            const int i = m / 12, k = m % 12 / 4, j = m % 4;
+            f32x4& to = acc.c[k ? 1 : 0][i][j];
+            to = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.a[i][k == 2], f.b[j][k == 1], to, 0, 0, 0);
+        }
+    }
+    wait_copies_and_meet<0>();
+}
+
 // ---- packing
 // Fragments of x (D, N).  The first caseBlocks blocks take 16 cases each: (rows = cases, k = features) for the logits; the others 16
 // features each: (rows = features, k = cases) for the weight gradient, in which a case without a label is zero, whatever it holds.
@@ -585,8 +645,9 @@ struct WideArgs {
     int Kv;
 };
 
-template <int MB, bool BWD>
-__global__ __launch_bounds__(256, 1) void k_fcl_logits(WideArgs p) {
+// SHARED: two blocks per CU (MB = 4)
+template <int MB, bool BWD, bool SHARED>
+__global__ __launch_bounds__(256, SHARED ? 2 : 1) void k_fcl_logits(WideArgs p) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     // the tiles of one block of classes on one XCD: they read the same rows of W
     int tv, tn;
@@ -595,7 +656,10 @@ __global__ __launch_bounds__(256, 1) void k_fcl_logits(WideArgs p) {
     const int c = lane & 15, g = lane >> 4;
     const size_t row = (size_t)p.Kd * PAIR;
     Acc<MB> acc;
-    product_tile<MB, false>(p.wByClass + (size_t)tv * 2 * MB * row, row, p.xByCase + (size_t)tn * 8 * row, row, 0, p.kSteps, lds, acc, NoScale());
+    if constexpr (SHARED)
+        product_tile_shared(p.wByClass + (size_t)tv * 2 * MB * row, row, p.xByCase + (size_t)tn * 8 * row, row, 0, p.kSteps, lds, acc);
+    else
+        product_tile<MB, false>(p.wByClass + (size_t)tv * 2 * MB * row, row, p.xByCase + (size_t)tn * 8 * row, row, 0, p.kSteps, lds, acc, NoScale());
     const int vBase = tv * 32 * MB + wm * 16 * MB, nBase = tn * TILE + wn * 64;
     // z in place of the first accumulator.  A class behind the last one, or taken out by its bias, has fragments of zeros: -inf.
     int ex[4], label[4];
@@ -820,7 +884,10 @@ template <int MB>
 __global__ __launch_bounds__(256, 1) void k_fcl_igrad(const char* dz, const char* wByClass, const int* __restrict__ classExp, float* __restrict__ slabs,
                                                       int Np, int Dp, int Kv, int Kd, int kPerSplit, int nTiles, int dTiles, int first) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const int tiles = nTiles * dTiles, s = blockIdx.x / tiles, t = blockIdx.x % tiles, td = t / nTiles, tn = t % nTiles;
+    // the tiles of one split on one XCD: they read the same classes of dz and W
+    int s, t;
+    mcn_xcd_group(blockIdx.x, nTiles * dTiles, gridDim.x / (nTiles * dTiles), s, t);
+    const int td = t / nTiles, tn = t % nTiles;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
     const int c = lane & 15, g = lane >> 4;
     const size_t row = (size_t)Kv * PAIR;
@@ -928,7 +995,7 @@ WidePlan wide_plan(int D, int V, int N, bool bwd) {
         p.dbPart = take((size_t)p.nTiles * V * 4);
         p.slabs = take((size_t)p.splits * p.dTiles * TILE * p.Np * 4);
     } else {
-        p.part = take((size_t)(divup(V, 64) + divup(V, p.rows) * 4) * 3 * N * 4);
+        p.part = take((size_t)(divup(V, 64) + divup(V, p.rows) * 8) * 3 * N * 4);
         p.labelLogits = take((size_t)N * 4);
     }
     p.total = at;
@@ -939,9 +1006,9 @@ template <bool BWD>
 void launch_logits(int mb, const WideArgs& a, hipStream_t s) {
     const dim3 grid(a.vTiles * a.nTiles), block(256);
     switch (mb) {
-        case 8: MCN_LAUNCH((k_fcl_logits<8, BWD>), grid, block, tile_lds(8), s, a); break;
-        case 4: MCN_LAUNCH((k_fcl_logits<4, BWD>), grid, block, tile_lds(4), s, a); break;
-        default: MCN_LAUNCH((k_fcl_logits<2, BWD>), grid, block, tile_lds(2), s, a); break;
+        case 8: MCN_LAUNCH((k_fcl_logits<4, BWD, true>), grid, block, SHARED_LDS, s, a); break;
+        case 4: MCN_LAUNCH((k_fcl_logits<4, BWD, false>), grid, block, tile_lds(4), s, a); break;
+        default: MCN_LAUNCH((k_fcl_logits<2, BWD, false>), grid, block, tile_lds(2), s, a); break;
     }
 }
 
@@ -965,7 +1032,7 @@ int wide_piece(const WidePlan& q, WideArgs& a, const float* W, int D, int v0, ch
     a.rows = std::min(q.rows, a.V - v0);
     a.nTiles = q.nTiles;
     const int mb = tile_choice(divup(a.rows, 32), q.nTiles), padded = padded_rows(a.rows, mb);
-    a.vTiles = padded / (32 * mb);
+    a.vTiles = padded / (32 * std::min(mb, 4));
     a.Kv = padded / 32;
     MCN_LAUNCH(k_fcl_pack_w, dim3(a.Kv), dim3(512), PACK_LDS, s, W + (size_t)v0 * D, a.bias ? a.bias + v0 : nullptr, (int*)(ws + q.classExp),
                ws + q.wByClass, D, a.rows, q.Kd);
