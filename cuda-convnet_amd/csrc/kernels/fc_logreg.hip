@@ -12,6 +12,7 @@ namespace {
 
 constexpr int BV = 64, BN = 64, BK = 32;  // k_fcl_tile: classes x cases, features per step
 constexpr size_t PIECE_ELEMS = (size_t)1 << 24;
+constexpr int PIECE_MB = 128;  // fragments of a piece; 512 x 100000 x 1024, both calls: 64 MB 1.77 ms, 128 MB 1.65 ms, 224 MB 1.62 ms
 
 struct FclArgs {
     const float *W, *X, *bias, *labels;
@@ -281,9 +282,9 @@ template <int MB>
 struct Frags {
     f16x8 a[MB][2], b[4][2];
 };
-// LDS stages: as many as 144 KB hold, one block per CU.  A tile of 256 rows spends 1536 matrix cycles on a step of 48 KB, which two
-// stages in flight cover; a small one 384 on 24 KB, and needs five.
-constexpr int tile_stages(int mb) { return mb == 8 ? 3 : mb == 4 ? 4 : 6; }
+// LDS stages of a block that has its CU to itself: as many as 144 KB hold.  A 64 x 128 tile spends 384 matrix cycles on a step of 24 KB,
+// and needs five stages in flight for it.
+constexpr int tile_stages(int mb) { return mb == 4 ? 4 : 6; }
 constexpr int tile_units(int mb) { return 2 * mb + 8; }
 constexpr int tile_lds(int mb) { return tile_stages(mb) * tile_units(mb) * PAIR; }
 
@@ -423,7 +424,9 @@ __device__ __forceinline__ void product_tile(const char* A, size_t aRow, const c
 // multiplies them, and two stages of LDS.  For the logits, whose epilogue (an exponential per entry) takes as long as their products:
 // one block's epilogue runs next to the other's products.
 constexpr int SHARED_LDS = 2 * tile_units(4) * PAIR;
-__device__ __forceinline__ void product_tile_shared(const char* A, size_t aRow, const char* B, size_t bRow, int k0, int k1, char* lds, Acc<4>& acc) {
+template <bool TURNED, class Scale>
+__device__ __forceinline__ void product_tile_shared(const char* A, size_t aRow, const char* B, size_t bRow, int k0, int k1, char* lds, Acc<4>& acc,
+                                                    const Scale& scale) {
     constexpr int UNITS = tile_units(4), STAGE = UNITS * PAIR, MINE = UNITS / 4;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave >> 1, wn = wave & 1;
@@ -436,39 +439,51 @@ __device__ __forceinline__ void product_tile_shared(const char* A, size_t aRow, 
     int n = k1 - k0;
     if (n <= 0) return;
     const char* src[MINE];
+    size_t adv = wave < 2 || !TURNED ? (size_t)PAIR : 2 * bRow;  // (two waves copy A's units, two B's)
 #pragma unroll
     for (int i = 0; i < MINE; i++) {
         const int u = wave * MINE + i, w = u - 8;
-        src[i] = (u < 8 ? A + (size_t)u * aRow : B + (size_t)w * bRow) + (size_t)k0 * PAIR;
+        src[i] = u < 8    ? A + (size_t)u * aRow + (size_t)k0 * PAIR
+                 : TURNED ? B + (size_t)(2 * k0 + (w >> 2)) * bRow + (size_t)(w & 3) * PAIR
+                          : B + (size_t)w * bRow + (size_t)k0 * PAIR;
         asm volatile("" : "+s"(src[i]));
     }
+    asm volatile("" : "+s"(adv));
     asm volatile("" : "+s"(n));
     const unsigned ldsBase = __builtin_amdgcn_readfirstlane((unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)lds) + wave * MINE * PAIR;
     const unsigned laneOff = lane * 16;
-    const char* mine = lds + lane * 8;
+    const int offA = wm * 4 * PAIR + lane * 8;
+    const int offB = (8 + (TURNED ? wn * 2 : wn * 4)) * PAIR + (TURNED ? (lane & 3) * 128 + ((lane >> 4) * 4 + ((lane & 15) >> 2)) * 8 : lane * 8);
     unsigned fill = 0, take = 0;
     auto copy = [&] {
 #pragma unroll
         for (int o = 0; o < 2 * MINE; o++) copy_pair_half(src[o >> 1], ldsBase + fill + (o >> 1) * PAIR, laneOff, o & 1);
 #pragma unroll
-        for (int i = 0; i < MINE; i++) src[i] += PAIR;
+        for (int i = 0; i < MINE; i++) src[i] += adv;
         fill ^= STAGE;
     };
     copy();
     for (int t = 0; t < n; t++) {
         wait_copies_and_meet<0>();  // stage t has landed, and everyone has read the other buffer
         Frags<4> f;
-        const char* s = mine + take;
+        const char* s = lds + take;
         take ^= STAGE;
 #pragma unroll
         for (int q = 0; q < 2; q++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) f.b[j][q] = read_frag(s + (8 + wn * 4 + j) * PAIR + q * FRAG);
+            for (int j = 0; j < 4; j++)
+                if constexpr (TURNED) {
+                    const char* p = s + offB + (j >> 1) * PAIR + q * FRAG + (j & 1) * 512;
+                    f.b[j][q] = read_frag_turned(p, p + 4 * PAIR);
+                } else {
+                    f.b[j][q] = read_frag(s + offB + j * PAIR + q * FRAG);
+                }
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int q = 0; q < 2; q++) f.a[i][q] = read_frag(s + (wm * 4 + i) * PAIR + q * FRAG);
+            for (int q = 0; q < 2; q++) f.a[i][q] = read_frag(s + offA + i * PAIR + q * FRAG);
         if (t + 1 < n) copy();
+        scale(t, acc);
 #pragma unroll
         for (int m = 0; m < 48; m++) {
             const int i = m / 12, k = m % 12 / 4, j = m % 4;
@@ -657,7 +672,7 @@ __global__ __launch_bounds__(256, SHARED ? 2 : 1) void k_fcl_logits(WideArgs p) 
     const size_t row = (size_t)p.Kd * PAIR;
     Acc<MB> acc;
     if constexpr (SHARED)
-        product_tile_shared(p.wByClass + (size_t)tv * 2 * MB * row, row, p.xByCase + (size_t)tn * 8 * row, row, 0, p.kSteps, lds, acc);
+        product_tile_shared<false>(p.wByClass + (size_t)tv * 2 * MB * row, row, p.xByCase + (size_t)tn * 8 * row, row, 0, p.kSteps, lds, acc, NoScale());
     else
         product_tile<MB, false>(p.wByClass + (size_t)tv * 2 * MB * row, row, p.xByCase + (size_t)tn * 8 * row, row, 0, p.kSteps, lds, acc, NoScale());
     const int vBase = tv * 32 * MB + wm * 16 * MB, nBase = tn * TILE + wn * 64;
@@ -807,8 +822,8 @@ __global__ __launch_bounds__(256, SHARED ? 2 : 1) void k_fcl_logits(WideArgs p) 
 }
 
 // ---- weight gradient of a piece: (features x classes) tiles, so that a lane's four rows are four neighbours of one row of W
-template <int MB>
-__global__ __launch_bounds__(256, 1) void k_fcl_wgrad(const char* xByFeat, const char* dz, const int* __restrict__ featExp, float* __restrict__ dW,
+template <int MB, bool SHARED>
+__global__ __launch_bounds__(256, SHARED ? 2 : 1) void k_fcl_wgrad(const char* xByFeat, const char* dz, const int* __restrict__ featExp, float* __restrict__ dW,
                                                       int D, int rows, int Kn, int Kv, int dTiles, int vTiles, float scaleTargets, float scaleOutput) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     int tv, td;
@@ -817,7 +832,8 @@ __global__ __launch_bounds__(256, 1) void k_fcl_wgrad(const char* xByFeat, const
     const int c = lane & 15, g = lane >> 4;
     const size_t row = (size_t)Kn * PAIR;
     Acc<MB> acc;
-    product_tile<MB, true>(xByFeat + (size_t)td * 2 * MB * row, row, dz + (size_t)tv * 4 * PAIR, (size_t)Kv * PAIR, 0, Kn, lds, acc, NoScale());
+    if constexpr (SHARED) product_tile_shared<true>(xByFeat + (size_t)td * 2 * MB * row, row, dz + (size_t)tv * 4 * PAIR, (size_t)Kv * PAIR, 0, Kn, lds, acc, NoScale());
+    else product_tile<MB, true>(xByFeat + (size_t)td * 2 * MB * row, row, dz + (size_t)tv * 4 * PAIR, (size_t)Kv * PAIR, 0, Kn, lds, acc, NoScale());
 #pragma unroll
     for (int i = 0; i < MB; i++) {
         const int d = td * 32 * MB + wm * 16 * MB + i * 16 + g * 4;
@@ -880,8 +896,8 @@ struct CarryScale {
 };
 
 // ---- input gradient: the sum over the classes is split; slab s of (Dp, Np) adds up its share of every piece, in order
-template <int MB>
-__global__ __launch_bounds__(256, 1) void k_fcl_igrad(const char* dz, const char* wByClass, const int* __restrict__ classExp, float* __restrict__ slabs,
+template <int MB, bool SHARED>
+__global__ __launch_bounds__(256, SHARED ? 2 : 1) void k_fcl_igrad(const char* dz, const char* wByClass, const int* __restrict__ classExp, float* __restrict__ slabs,
                                                       int Np, int Dp, int Kv, int Kd, int kPerSplit, int nTiles, int dTiles, int first) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     // the tiles of one split on one XCD: they read the same classes of dz and W
@@ -894,7 +910,8 @@ __global__ __launch_bounds__(256, 1) void k_fcl_igrad(const char* dz, const char
     const int k0 = s * kPerSplit, k1 = min(Kv, k0 + kPerSplit);
     Acc<MB> acc;
     const CarryScale carry(classExp + k0, k1 - k0);
-    product_tile<MB, true>(dz + (size_t)tn * 2 * MB * row, row, wByClass + (size_t)td * 4 * PAIR, (size_t)Kd * PAIR, k0, k1, lds, acc, carry);
+    if constexpr (SHARED) product_tile_shared<true>(dz + (size_t)tn * 2 * MB * row, row, wByClass + (size_t)td * 4 * PAIR, (size_t)Kd * PAIR, k0, k1, lds, acc, carry);
+    else product_tile<MB, true>(dz + (size_t)tn * 2 * MB * row, row, wByClass + (size_t)td * 4 * PAIR, (size_t)Kd * PAIR, k0, k1, lds, acc, carry);
     const int e = carry.cur == EXP_ZERO ? 0 : -(carry.cur + DZ_EXP);
 #pragma unroll
     for (int i = 0; i < MB; i++)
@@ -931,32 +948,26 @@ __global__ __launch_bounds__(256) void k_fcl_finish(const float* __restrict__ sl
     dB[v] = (scaleBiasTargets != 0.f ? scaleBiasTargets * dB[v] : 0.f) + scaleBiasOutput * coeff * s;
 }
 
-// Rows of a product's tile / 32: the whole launch runs in rounds of one tile per CU, and a tile costs its rows plus a fixed part (the
-// fill of its stages, its epilogue) of about 32 rows.  With 256 rows an LDS byte feeds 1.5 times the matrix work that it does with 128.
-int tile_choice(int rows32, int colTiles) {
-    int best = 2;
-    long cost = -1;
-    for (int mb : {8, 4, 2}) {
-        const long c = (long)divup(divup(rows32, mb) * colTiles, 256) * (mb + 1);
-        if (cost < 0 || c < cost) {
-            cost = c;
-            best = mb;
-        }
-    }
-    return best;
+// Which tile a product takes: SHARED 128 x 128, two blocks per CU; WHOLE 128 x 128 or HALF 64 x 128, one block per CU with its stages
+// further ahead.  A launch runs in rounds of 512 or 256 blocks, and a tile costs its rows / 32 (twice that for two sharing a CU) and a
+// fixed part, the fill of its stages and its epilogue, of about one more.  512 x 100000 x 1024: SHARED logits 330 us, WHOLE tiles of
+// twice the rows 390 us; 512 x 10575 x 128, 83 row tiles: logits HALF 13 us, SHARED 25 us.
+enum TileKind { SHARED, WHOLE, HALF };
+TileKind tile_choice(int rows32, int colTiles) {
+    const long whole = (long)divup(rows32, 4) * colTiles, half = (long)divup(rows32, 2) * colTiles;
+    const long cost[3] = {(whole + 511) / 512 * 9, (whole + 255) / 256 * 5, (half + 255) / 256 * 3};
+    return cost[HALF] < cost[WHOLE] && cost[HALF] < cost[SHARED] ? HALF : cost[WHOLE] < cost[SHARED] ? WHOLE : SHARED;
 }
+int tile_rows32(TileKind k) { return k == HALF ? 2 : 4; }
+int tile_bytes(TileKind k) { return k == SHARED ? SHARED_LDS : tile_lds(tile_rows32(k)); }
 
 // Sizes and workspace of the wide path: a function of the shape alone.
 struct WidePlan {
     int Np, Dp, Kd, kSteps, Kn, nTiles, dTiles;  // Kd: k blocks of W's and x's fragments, padded; kSteps: those that hold anything
     int rows, Kv;                                // classes per piece; k blocks of a whole piece, padded
-    int mbWgrad, mbIgrad;
     int splits;                                  // input gradient
     size_t classExp, caseExp, featExp, xByCase, xByFeat, wByClass, dz, dbPart, slabs, part, labelLogits, total;
 };
-// rows of a piece padded to whole tiles of either kind
-int padded_rows(int rows, int mb) { return divup(rows, std::max(TILE, 32 * mb)) * std::max(TILE, 32 * mb); }
-
 bool wide_usable(int D, int V, int N) { return N > 48; }
 
 size_t al256(size_t b) { return (b + 255) / 256 * 256; }
@@ -967,21 +978,17 @@ WidePlan wide_plan(int D, int V, int N, bool bwd) {
     p.dTiles = divup(D, TILE);
     p.kSteps = divup(D, 32);
     p.Kd = p.dTiles * 4;
-    // a piece's fragments should stay in the 256 MB last-level cache between the launches that write and read them; whole rounds of
-    // 256-row tiles where the classes fill some
-    const size_t perRow = (size_t)p.Kd * 128 + (bwd ? (size_t)p.nTiles * TILE * 4 : 0);
-    const int most = (int)std::max<size_t>(TILE, std::min<size_t>(((size_t)128 << 20) / perRow / 256 * 256, (size_t)1 << 17));
-    const int round = std::max(1, 256 / p.nTiles) * 256;
-    p.rows = std::min(V, most > round ? most / round * round : most);
-    const int v32 = divup(p.rows, 32);
-    p.Kv = std::max({padded_rows(p.rows, 8), padded_rows(p.rows, 4)}) / 32;
-    p.mbIgrad = 4;
-    if (p.nTiles % 2 == 0) p.mbIgrad = 8;
-    p.mbWgrad = tile_choice(divup(D, 32), divup(v32, 4));
-    p.Np = divup(N, std::max(TILE, 32 * p.mbIgrad)) * std::max(TILE, 32 * p.mbIgrad);
-    p.Dp = divup(D, std::max(TILE, 32 * p.mbWgrad)) * std::max(TILE, 32 * p.mbWgrad);
+    p.Np = p.nTiles * TILE;
+    p.Dp = p.dTiles * TILE;
     p.Kn = p.Np / 32;
-    p.splits = std::max(1, std::min(p.Kv / 8, 256 / (p.Np / (32 * p.mbIgrad) * p.dTiles)));
+    // a piece's fragments should stay in the 256 MB last-level cache between the launches that write and read them; whole rounds of
+    // shared tiles where the classes fill some
+    const size_t perRow = (size_t)p.Kd * 128 + (bwd ? (size_t)p.Np * 4 : 0);
+    const int most = (int)std::max<size_t>(TILE, std::min<size_t>(((size_t)PIECE_MB << 20) / perRow / TILE * TILE, (size_t)1 << 17));
+    const int round = std::max(1, 512 / p.nTiles) * TILE;
+    p.rows = std::min(V, most > round ? most / round * round : most);
+    p.Kv = divup(p.rows, TILE) * 4;
+    p.splits = std::max(1, std::min(p.Kv / 8, 512 / (p.nTiles * p.dTiles)));
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t o = at; at += al256(bytes); return o; };
     p.classExp = take((size_t)p.Kv * 4);
@@ -993,9 +1000,9 @@ WidePlan wide_plan(int D, int V, int N, bool bwd) {
         p.xByFeat = take((size_t)p.Dp / 16 * p.Kn * PAIR);
         p.dz = take((size_t)p.Np / 16 * p.Kv * PAIR);
         p.dbPart = take((size_t)p.nTiles * V * 4);
-        p.slabs = take((size_t)p.splits * p.dTiles * TILE * p.Np * 4);
+        p.slabs = take((size_t)p.splits * p.Dp * p.Np * 4);
     } else {
-        p.part = take((size_t)(divup(V, 64) + divup(V, p.rows) * 8) * 3 * N * 4);
+        p.part = take((size_t)(divup(V, 64) + divup(V, p.rows) * 2) * 3 * N * 4);
         p.labelLogits = take((size_t)N * 4);
     }
     p.total = at;
@@ -1003,13 +1010,11 @@ WidePlan wide_plan(int D, int V, int N, bool bwd) {
 }
 
 template <bool BWD>
-void launch_logits(int mb, const WideArgs& a, hipStream_t s) {
+void launch_logits(TileKind kind, const WideArgs& a, hipStream_t s) {
     const dim3 grid(a.vTiles * a.nTiles), block(256);
-    switch (mb) {
-        case 8: MCN_LAUNCH((k_fcl_logits<4, BWD, true>), grid, block, SHARED_LDS, s, a); break;
-        case 4: MCN_LAUNCH((k_fcl_logits<4, BWD, false>), grid, block, tile_lds(4), s, a); break;
-        default: MCN_LAUNCH((k_fcl_logits<2, BWD, false>), grid, block, tile_lds(2), s, a); break;
-    }
+    if (kind == SHARED) MCN_LAUNCH((k_fcl_logits<4, BWD, true>), grid, block, tile_bytes(SHARED), s, a);
+    else if (kind == WHOLE) MCN_LAUNCH((k_fcl_logits<4, BWD, false>), grid, block, tile_bytes(WHOLE), s, a);
+    else MCN_LAUNCH((k_fcl_logits<2, BWD, false>), grid, block, tile_bytes(HALF), s, a);
 }
 
 WideArgs wide_args(const WidePlan& q, const float* bias, const float* labels, int V, int N, char* ws) {
@@ -1027,16 +1032,16 @@ WideArgs wide_args(const WidePlan& q, const float* bias, const float* labels, in
     return a;
 }
 // one piece: its packed rows, tiles and k blocks
-int wide_piece(const WidePlan& q, WideArgs& a, const float* W, int D, int v0, char* ws, hipStream_t s) {
+TileKind wide_piece(const WidePlan& q, WideArgs& a, const float* W, int D, int v0, char* ws, hipStream_t s) {
     a.v0 = v0;
     a.rows = std::min(q.rows, a.V - v0);
     a.nTiles = q.nTiles;
-    const int mb = tile_choice(divup(a.rows, 32), q.nTiles), padded = padded_rows(a.rows, mb);
-    a.vTiles = padded / (32 * std::min(mb, 4));
-    a.Kv = padded / 32;
+    a.Kv = divup(a.rows, TILE) * 4;
+    const TileKind kind = tile_choice(a.Kv, q.nTiles);
+    a.vTiles = a.Kv / tile_rows32(kind);
     MCN_LAUNCH(k_fcl_pack_w, dim3(a.Kv), dim3(512), PACK_LDS, s, W + (size_t)v0 * D, a.bias ? a.bias + v0 : nullptr, (int*)(ws + q.classExp),
                ws + q.wByClass, D, a.rows, q.Kd);
-    return mb;
+    return kind;
 }
 
 int wide_cost(const float* W, const float* X, const float* bias, const float* labels, float* stats, float* logp, float* correct, int D, int V,
@@ -1048,9 +1053,9 @@ int wide_cost(const float* W, const float* X, const float* bias, const float* la
                D, V, N, q.Kd, q.Kn, q.Np / 16);
     int tiles = 0;
     for (int v0 = 0; v0 < V; v0 += q.rows) {
-        const int mb = wide_piece(q, a, W, D, v0, ws, s);
+        const TileKind kind = wide_piece(q, a, W, D, v0, ws, s);
         a.part = (float*)(ws + q.part) + (size_t)tiles * 3 * N;
-        launch_logits<false>(mb, a, s);
+        launch_logits<false>(kind, a, s);
         tiles += a.vTiles;
         if (int rc = MCN_LAUNCH_CHECK("fcLogregCost")) return rc;
     }
@@ -1071,25 +1076,28 @@ int wide_grad(const float* W, const float* X, const float* bias, const float* la
     MCN_LAUNCH(k_fcl_pack_x, dim3(q.Np / 16 + (dW ? q.Dp / 16 : 0)), dim3(512), 0, s, X, labels, (int*)(ws + q.caseExp), (int*)(ws + q.featExp),
                ws + q.xByCase, ws + q.xByFeat, D, V, N, q.Kd, q.Kn, q.Np / 16);
     for (int v0 = 0; v0 < V; v0 += q.rows) {
-        const int mb = wide_piece(q, a, W, D, v0, ws, s);
-        launch_logits<true>(mb, a, s);
+        const TileKind kind = wide_piece(q, a, W, D, v0, ws, s);
+        launch_logits<true>(kind, a, s);
         if (dW) {
-            const int vTiles = a.Kv / 4, dTiles = q.Dp / (32 * q.mbWgrad);
+            const int vTiles = a.Kv / 4;
+            const TileKind k = tile_choice(q.dTiles * 4, vTiles);
+            const int dTiles = q.dTiles * 4 / tile_rows32(k);
             const dim3 grid(vTiles * dTiles), block(256);
             const float sO = scaleWeightOutput * coeff;
             float* out = dW + (size_t)v0 * D;
-#define WGRAD(MB) MCN_LAUNCH((k_fcl_wgrad<MB>), grid, block, tile_lds(MB), s, ws + q.xByFeat, a.dz, featExp, out, D, a.rows, q.Kn, a.Kv, dTiles, vTiles, scaleWeightTargets, sO)
-            if (q.mbWgrad == 8) WGRAD(8);
-            else if (q.mbWgrad == 4) WGRAD(4);
-            else WGRAD(2);
+#define WGRAD(MB, SH) MCN_LAUNCH((k_fcl_wgrad<MB, SH>), grid, block, tile_bytes(k), s, ws + q.xByFeat, a.dz, featExp, out, D, a.rows, q.Kn, a.Kv, dTiles, vTiles, scaleWeightTargets, sO)
+            if (k == SHARED) WGRAD(4, true);
+            else if (k == WHOLE) WGRAD(4, false);
+            else WGRAD(2, false);
 #undef WGRAD
         }
         if (dX) {
-            const int nTiles = q.Np / (32 * q.mbIgrad), kPer = divup(a.Kv, q.splits);
-            const dim3 grid(q.splits * nTiles * q.dTiles), block(256);
-#define IGRAD(MB) MCN_LAUNCH((k_fcl_igrad<MB>), grid, block, tile_lds(MB), s, a.dz, a.wByClass, a.classExp, slabs, q.Np, q.dTiles * TILE, a.Kv, q.Kd, kPer, nTiles, q.dTiles, v0 == 0)
-            if (q.mbIgrad == 8) IGRAD(8);
-            else IGRAD(4);
+            // (a short last piece has fewer, not shorter, shares: each adds to its slab)
+            const int tiles = q.nTiles * q.dTiles, kPer = std::max(std::min(8, a.Kv), divup(a.Kv, q.splits)), splits = divup(a.Kv, kPer);
+            const dim3 grid(splits * tiles), block(256);
+#define IGRAD(SH, KIND) MCN_LAUNCH((k_fcl_igrad<4, SH>), grid, block, tile_bytes(KIND), s, a.dz, a.wByClass, a.classExp, slabs, q.Np, q.Dp, a.Kv, q.Kd, kPer, q.nTiles, q.dTiles, v0 == 0)
+            if (splits * tiles > 256) IGRAD(true, SHARED);
+            else IGRAD(false, WHOLE);
 #undef IGRAD
         }
         if (int rc = MCN_LAUNCH_CHECK("fcLogregGrad")) return rc;
@@ -1097,7 +1105,7 @@ int wide_grad(const float* W, const float* X, const float* bias, const float* la
     if (dX || dB) {
         const int dxBlocks = dX ? (int)divup_sz((size_t)D * N, 256) : 0;
         MCN_LAUNCH(k_fcl_finish, dim3(dxBlocks + (dB ? divup(V, 256) : 0)), dim3(256), 0, s, slabs, (const float*)(ws + q.dbPart), dX, dB, D, V, N, q.Np,
-                   q.dTiles * TILE, q.splits, q.nTiles, dxBlocks, coeff, scaleInputTargets, scaleBiasTargets, scaleBiasOutput);
+                   q.Dp, q.splits, q.nTiles, dxBlocks, coeff, scaleInputTargets, scaleBiasTargets, scaleBiasOutput);
     }
     return MCN_LAUNCH_CHECK("fcLogregGrad");
 }
