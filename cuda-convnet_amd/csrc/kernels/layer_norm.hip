@@ -9,56 +9,48 @@
 
 namespace {
 
-constexpr int T = 256;       // threads of a block
-constexpr int MAX_SPLIT = 64;
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
-// Shape of one launch: a block covers colLanes * VW columns and one range of rows; rowLanes = T / colLanes.
-struct LnShape {
-    int F, N;
-    int logColLanes;      // colLanes = 1 << logColLanes
-    int colTiles, splits, rowsPerSplit;
-};
+constexpr int T_SPLIT = 256, T_WHOLE = 256;  // threads of a block
+constexpr int JOIN = 4, AHEAD = 4;           // split: partial sums a lane joins; rows it has asked for by then
+constexpr int CUS = 256;
 
-LnShape ln_shape(int F, int N, int vw) {
-    LnShape s;
-    s.F = F;
-    s.N = N;
-    const int lanes = divup(N, vw);
-    s.logColLanes = 0;
-    while ((1 << s.logColLanes) < lanes && (1 << s.logColLanes) < 64 / vw) s.logColLanes++;
-    const int colLanes = 1 << s.logColLanes, rowLanes = T / colLanes;
-    s.colTiles = divup(lanes, colLanes);
-    // enough blocks for the chip, at least four rows a lane in each
-    s.splits = std::max(1, std::min({MAX_SPLIT, divup(1024, s.colTiles), divup(F, 4 * rowLanes)}));
-    s.rowsPerSplit = divup(F, s.splits);
-    s.splits = divup(F, s.rowsPerSplit);
-    return s;
-}
-
+// VW neighbouring columns of one row; at the right edge of the matrix only `cnt` of them exist.  Rows start at any multiple of four
+// bytes: the hardware takes 16-byte accesses at such addresses.
 template <int VW>
-struct Vec {
+struct Cols {
     float v[VW];
 };
 template <int VW>
-__device__ __forceinline__ Vec<VW> load_cols(const float* __restrict__ p) {
-    Vec<VW> r;
+__device__ __forceinline__ Cols<VW> load_cols(const float* p, int cnt) {
+    Cols<VW> r = {};
     if constexpr (VW == 4) {
-        const f32x4 t = *reinterpret_cast<const f32x4*>(p);
-        for (int j = 0; j < 4; j++) r.v[j] = t[j];
-    } else {
-        r.v[0] = *p;
+        if (cnt == 4) {
+            const f32x4u t = *reinterpret_cast<const f32x4u*>(p);
+#pragma unroll
+            for (int j = 0; j < 4; j++) r.v[j] = t[j];
+            return r;
+        }
     }
+#pragma unroll
+    for (int j = 0; j < VW; j++)
+        if (j < cnt) r.v[j] = p[j];
     return r;
 }
 template <int VW>
-__device__ __forceinline__ void store_cols(float* __restrict__ p, const Vec<VW>& r) {
+__device__ __forceinline__ void store_cols(float* p, const Cols<VW>& r, int cnt) {
     if constexpr (VW == 4) {
-        f32x4 t;
-        for (int j = 0; j < 4; j++) t[j] = r.v[j];
-        *reinterpret_cast<f32x4*>(p) = t;
-    } else {
-        *p = r.v[0];
+        if (cnt == 4) {
+            f32x4u t;
+#pragma unroll
+            for (int j = 0; j < 4; j++) t[j] = r.v[j];
+            *reinterpret_cast<f32x4u*>(p) = t;
+            return;
+        }
     }
+#pragma unroll
+    for (int j = 0; j < VW; j++)
+        if (j < cnt) p[j] = r.v[j];
 }
 
 __device__ __forceinline__ void join(float& n, float& mean, float& m2, float n2, float mean2, float m22) {
@@ -71,225 +63,469 @@ __device__ __forceinline__ void join(float& n, float& mean, float& m2, float n2,
     n = t;
 }
 
-// Stage 1: mean and sum of squared deviations of one range of rows, into part[split][2][N].
-template <int VW>
-__global__ __launch_bounds__(T) void k_ln_stats(const float* __restrict__ x, float* __restrict__ part, LnShape s) {
-    __shared__ float sh[2][T][VW];
-    const int colLanes = 1 << s.logColLanes, rowLanes = T >> s.logColLanes;
-    const int cl = threadIdx.x & (colLanes - 1), rl = threadIdx.x >> s.logColLanes;
-    const int col = (blockIdx.x * colLanes + cl) * VW;
-    const int r0 = blockIdx.y * s.rowsPerSplit, r1 = min(s.F, r0 + s.rowsPerSplit);
-    const bool live = col < s.N;
-    float mean[VW] = {}, m2[VW] = {}, cnt = 0.f;
-    if (live)
-        for (int r = r0 + rl; r < r1; r += rowLanes) {
-            const Vec<VW> v = load_cols<VW>(x + (size_t)r * s.N + col);
-            const float w = 1.f / (cnt + 1.f);
-#pragma unroll
-            for (int j = 0; j < VW; j++) {
-                const float d = v.v[j] - mean[j];
-                mean[j] += d * w;
-                m2[j] += d * (v.v[j] - mean[j]);
-            }
-            cnt += 1.f;
-        }
-#pragma unroll
-    for (int j = 0; j < VW; j++) {
-        sh[0][threadIdx.x][j] = mean[j];
-        sh[1][threadIdx.x][j] = m2[j];
+// Where a thread of a T-thread block stands: columns col .. col + cnt - 1, rows rl, rl + rowLanes, ...
+template <int VW, int T>
+struct Place {
+    int cl, rl, rowLanes, col, cnt;
+    __device__ __forceinline__ Place(int tile, int logLanes, int N) {
+        const int lanes = 1 << logLanes;
+        cl = threadIdx.x & (lanes - 1);
+        rl = threadIdx.x >> logLanes;
+        rowLanes = T >> logLanes;
+        col = (tile * lanes + cl) * VW;
+        cnt = max(0, min(VW, N - col));
     }
-    __syncthreads();
-    const int rows = r1 - r0;
-    for (int half = rowLanes >> 1; half > 0; half >>= 1) {
-        if (rl < half) {
-            const int o = threadIdx.x + (half << s.logColLanes);
-            // rows held by row lanes rl, rl + half, ... so far: every lane's share of the range follows from its index
-            float na = 0.f, nb = 0.f;
-            for (int k = rl; k < rowLanes; k += 2 * half) na += (float)(k < rows ? (rows - k + rowLanes - 1) / rowLanes : 0);
-            for (int k = rl + half; k < rowLanes; k += 2 * half) nb += (float)(k < rows ? (rows - k + rowLanes - 1) / rowLanes : 0);
+};
+// Sums of NV values a thread over the row lanes of its columns; every thread gets them.  Lanes of a wave, then the waves, in a fixed order.
+template <int NV, int T>
+__device__ __forceinline__ void sum_rows(float (&v)[NV], int cl, int logLanes, float (*sh)[64][NV]) {
+    for (int o = 1 << logLanes; o < 64; o <<= 1)
 #pragma unroll
-            for (int j = 0; j < VW; j++) {
-                float n = na, a = sh[0][threadIdx.x][j], b = sh[1][threadIdx.x][j];
-                join(n, a, b, nb, sh[0][o][j], sh[1][o][j]);
-                sh[0][threadIdx.x][j] = a;
-                sh[1][threadIdx.x][j] = b;
-            }
-        }
+        for (int k = 0; k < NV; k++) v[k] += __shfl_xor(v[k], o, 64);
+    if constexpr (T > 64) {
+        const int wave = threadIdx.x >> 6;
         __syncthreads();
-    }
-    if (rl == 0 && live) {
-        Vec<VW> a, b;
-        for (int j = 0; j < VW; j++) { a.v[j] = sh[0][threadIdx.x][j]; b.v[j] = sh[1][threadIdx.x][j]; }
-        float* p = part + (size_t)blockIdx.y * 2 * s.N + col;
-        store_cols<VW>(p, a);
-        store_cols<VW>(p + s.N, b);
+        if ((int)(threadIdx.x & 63) < (1 << logLanes))
+#pragma unroll
+            for (int k = 0; k < NV; k++) sh[wave][cl][k] = v[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < NV; k++) v[k] = 0.f;
+#pragma unroll
+        for (int w = 0; w < T / 64; w++)
+#pragma unroll
+            for (int k = 0; k < NV; k++) v[k] += sh[w][cl][k];
     }
 }
 
-// Stage 2: joins the ranges and writes y; the blocks of the first range also leave the case statistics.
-template <int VW>
-__global__ __launch_bounds__(T) void k_ln_apply(const float* x, const float* __restrict__ gain, const float* __restrict__ bias, float* y,
-                                                float* __restrict__ caseStats, const float* __restrict__ part, float eps, LnShape s) {
-    const int colLanes = 1 << s.logColLanes, rowLanes = T >> s.logColLanes;
-    const int cl = threadIdx.x & (colLanes - 1), rl = threadIdx.x >> s.logColLanes;
-    const int col = (blockIdx.x * colLanes + cl) * VW;
-    if (col >= s.N) return;
-    float mean[VW] = {}, m2[VW] = {}, cnt = 0.f;
-    for (int k = 0; k < s.splits; k++) {
-        const float rows = (float)(min(s.F, (k + 1) * s.rowsPerSplit) - k * s.rowsPerSplit);
-        const Vec<VW> a = load_cols<VW>(part + (size_t)k * 2 * s.N + col), b = load_cols<VW>(part + ((size_t)k * 2 + 1) * s.N + col);
-        float n = 0.f;
+// ---- forward, a block holds all rows of its columns in registers (R a thread): one read, the variance from exact deviations
+template <int VW, int R>
+__global__ __launch_bounds__(T_WHOLE) void k_ln_whole(const float* x, const float* __restrict__ gain, const float* __restrict__ bias, float* y,
+                                                      float* __restrict__ caseStats, float eps, int F, int N, int logLanes, int tiles) {
+    constexpr int T = T_WHOLE;
+    __shared__ float sh[T / 64][64][VW];
+    int grp, sub;
+    mcn_xcd_group(blockIdx.x, 8, gridDim.x / 8, grp, sub);  // eight neighbouring tiles on one XCD: they share cache lines (the grid is a multiple of eight)
+    const int tile = grp * 8 + sub;
+    if (tile >= tiles) return;
+    const Place<VW, T> p(tile, logLanes, N);
+    Cols<VW> v[R];
+    const size_t first = (size_t)p.rl * N + p.col, step = (size_t)p.rowLanes * N;
+    const float* xp = x + first;
+#pragma unroll
+    for (int i = 0; i < R; i++, xp += step) v[i] = p.rl + i * p.rowLanes < F ? load_cols<VW>(xp, p.cnt) : Cols<VW>{};
+    float mean[VW] = {}, m2[VW] = {};
+#pragma unroll
+    for (int i = 0; i < R; i++)
+#pragma unroll
+        for (int j = 0; j < VW; j++) mean[j] += v[i].v[j];
+    sum_rows<VW, T>(mean, p.cl, logLanes, sh);
+#pragma unroll
+    for (int j = 0; j < VW; j++) mean[j] /= (float)F;
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        const bool in = p.rl + i * p.rowLanes < F;
 #pragma unroll
         for (int j = 0; j < VW; j++) {
-            n = cnt;
-            join(n, mean[j], m2[j], rows, a.v[j], b.v[j]);
+            v[i].v[j] -= mean[j];
+            m2[j] += in ? v[i].v[j] * v[i].v[j] : 0.f;
         }
-        cnt = n;
     }
-    Vec<VW> mu, rs;
+    sum_rows<VW, T>(m2, p.cl, logLanes, sh);
+    Cols<VW> mu, rs;
+#pragma unroll
+    for (int j = 0; j < VW; j++) {
+        mu.v[j] = mean[j];
+        rs.v[j] = 1.f / sqrtf(m2[j] / (float)F + eps);
+    }
+    if (caseStats && p.rl == 0) {
+        store_cols<VW>(caseStats + p.col, mu, p.cnt);
+        store_cols<VW>(caseStats + N + p.col, rs, p.cnt);
+    }
+    float* yp = y + first;
+#pragma unroll
+    for (int i = 0; i < R; i++, yp += step) {
+        const int r = p.rl + i * p.rowLanes;
+        if (r >= F) break;
+        const float g = gain ? gain[r] : 1.f, b = bias ? bias[r] : 0.f;
+#pragma unroll
+        for (int j = 0; j < VW; j++) v[i].v[j] = g * (v[i].v[j] * rs.v[j]) + b;
+        store_cols<VW>(yp, v[i], p.cnt);
+    }
+}
+
+// ---- backward, the same way: both matrices in registers.  A block goes through its tiles one after the other with its rows fixed, so
+// the row sums for gains and biases stay in registers too and leave once per block: rowPart[block][2][F].
+template <int VW, int R>
+__global__ __launch_bounds__(T_WHOLE) void k_ln_undo_whole(const float* g, const float* x, const float* __restrict__ gain,
+                                                     const float* __restrict__ caseStats, float* target, float* __restrict__ rowPart,
+                                                     float scaleTargets, float scaleOutput, int F, int N, int logLanes, int tiles) {
+    constexpr int T = T_WHOLE;
+    __shared__ float sh[T / 64][64][2 * VW];
+    int grp, sub;
+    mcn_xcd_group(blockIdx.x, 8, gridDim.x / 8, grp, sub);  // (the grid is a multiple of eight)
+    const int block = grp * 8 + sub, rowLanes = T >> logLanes, rl = threadIdx.x >> logLanes;
+    float sg[R] = {}, sb[R] = {};
+    const float invF = 1.f / (float)F;
+    const size_t step = (size_t)rowLanes * N;
+    for (int tile = block; tile < tiles; tile += gridDim.x) {
+        const Place<VW, T> p(tile, logLanes, N);
+        const size_t first = (size_t)rl * N + p.col;
+        Cols<VW> gv[R], xv[R];
+        const float *gp = g + first, *xp = x + first;
+#pragma unroll
+        for (int i = 0; i < R; i++, gp += step, xp += step) {
+            const bool in = rl + i * rowLanes < F;
+            gv[i] = in ? load_cols<VW>(gp, p.cnt) : Cols<VW>{};
+            xv[i] = in ? load_cols<VW>(xp, p.cnt) : Cols<VW>{};
+        }
+        const Cols<VW> mu = load_cols<VW>(caseStats + p.col, p.cnt), rs = load_cols<VW>(caseStats + N + p.col, p.cnt);
+        float s[2 * VW] = {};
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            const int r = rl + i * rowLanes;
+            const float ga = gain && r < F ? gain[r] : 1.f;
+#pragma unroll
+            for (int j = 0; j < VW; j++) {
+                const float xh = (xv[i].v[j] - mu.v[j]) * rs.v[j];
+                sg[i] += gv[i].v[j] * xh;
+                sb[i] += gv[i].v[j];
+                const float h = ga * gv[i].v[j];
+                s[j] += h;
+                s[VW + j] += h * xh;
+                xv[i].v[j] = xh;
+                gv[i].v[j] = h;
+            }
+        }
+        if (!target) continue;
+        sum_rows<2 * VW, T>(s, p.cl, logLanes, sh);
+#pragma unroll
+        for (int j = 0; j < 2 * VW; j++) s[j] *= invF;
+        float* tp = target + first;
+#pragma unroll
+        for (int i = 0; i < R; i++, tp += step) {
+            if (rl + i * rowLanes >= F) break;
+            Cols<VW> o;
+#pragma unroll
+            for (int j = 0; j < VW; j++) o.v[j] = scaleOutput * (rs.v[j] * (gv[i].v[j] - s[j] - xv[i].v[j] * s[VW + j]));
+            if (scaleTargets != 0.f) {
+                const Cols<VW> t = load_cols<VW>(tp, p.cnt);
+#pragma unroll
+                for (int j = 0; j < VW; j++) o.v[j] += scaleTargets * t.v[j];
+            }
+            store_cols<VW>(tp, o, p.cnt);
+        }
+    }
+    if (!rowPart) return;
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        const int r = rl + i * rowLanes;
+        for (int o = (1 << logLanes) >> 1; o > 0; o >>= 1) {
+            sg[i] += __shfl_xor(sg[i], o, 64);
+            sb[i] += __shfl_xor(sb[i], o, 64);
+        }
+        if ((threadIdx.x & ((1 << logLanes) - 1)) == 0 && r < F) {
+            float* out = rowPart + (size_t)block * 2 * F + r;
+            out[0] = sg[i];
+            out[F] = sb[i];
+        }
+    }
+}
+
+// ---- more rows than a block's registers hold: ranges of rows, joined by a second launch that reads the matrices again
+struct Split {
+    int F, N, logLanes, colTiles, splits, rowsPerSplit;
+};
+
+template <int VW>
+__global__ __launch_bounds__(T_SPLIT) void k_ln_split_stats(const float* __restrict__ x, float* __restrict__ part, Split s) {
+    constexpr int T = T_SPLIT, R = 8;
+    __shared__ float sh[T / 64][64][VW];
+    const Place<VW, T> p(blockIdx.x, s.logLanes, s.N);
+    const int r0 = blockIdx.y * s.rowsPerSplit, r1 = min(s.F, r0 + s.rowsPerSplit), chunk = p.rowLanes * R;
+    float n = 0.f, mean[VW] = {}, m2[VW] = {};
+    for (int c = r0; c < r1; c += chunk) {  // (the same number of chunks for every thread: barriers below)
+        Cols<VW> v[R];
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            const int r = c + p.rl + i * p.rowLanes;
+            v[i] = r < r1 ? load_cols<VW>(x + (size_t)r * s.N + p.col, p.cnt) : Cols<VW>{};
+        }
+        float a[VW] = {}, b[VW] = {};
+#pragma unroll
+        for (int i = 0; i < R; i++)
+#pragma unroll
+            for (int j = 0; j < VW; j++) a[j] += v[i].v[j];
+        sum_rows<VW, T>(a, p.cl, s.logLanes, sh);
+        const float rows = (float)min(chunk, r1 - c);
+#pragma unroll
+        for (int j = 0; j < VW; j++) a[j] /= rows;
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            const bool in = c + p.rl + i * p.rowLanes < r1;
+#pragma unroll
+            for (int j = 0; j < VW; j++) {
+                const float d = v[i].v[j] - a[j];
+                b[j] += in ? d * d : 0.f;
+            }
+        }
+        sum_rows<VW, T>(b, p.cl, s.logLanes, sh);
+        float t = n;
+#pragma unroll
+        for (int j = 0; j < VW; j++) {
+            t = n;
+            join(t, mean[j], m2[j], rows, a[j], b[j]);
+        }
+        n = t;
+    }
+    if (p.rl == 0) {
+        Cols<VW> a, b;
+#pragma unroll
+        for (int j = 0; j < VW; j++) { a.v[j] = mean[j]; b.v[j] = m2[j]; }
+        float* out = part + (size_t)blockIdx.y * 2 * s.N + p.col;
+        store_cols<VW>(out, a, p.cnt);
+        store_cols<VW>(out + s.N, b, p.cnt);
+    }
+}
+
+// joins the ranges and writes y; the blocks of the first range also leave the case statistics
+template <int VW>
+__global__ __launch_bounds__(T_SPLIT) void k_ln_split_apply(const float* x, const float* __restrict__ gain, const float* __restrict__ bias,
+                                                            float* y, float* __restrict__ caseStats, const float* __restrict__ part, float eps,
+                                                            Split s) {
+    const Place<VW, T_SPLIT> p(blockIdx.x, s.logLanes, s.N);
+    __shared__ float sh[T_SPLIT / 64][64][VW];
+    const int r0 = blockIdx.y * s.rowsPerSplit, r1 = min(s.F, r0 + s.rowsPerSplit);
+    // everything this thread will need first, before the sums make it wait: one trip to memory instead of three
+    Cols<VW> a[JOIN], b[JOIN], v[AHEAD];
+#pragma unroll
+    for (int i = 0; i < JOIN; i++) {
+        const int k = p.rl + i * p.rowLanes;
+        a[i] = k < s.splits ? load_cols<VW>(part + (size_t)k * 2 * s.N + p.col, p.cnt) : Cols<VW>{};
+        b[i] = k < s.splits ? load_cols<VW>(part + ((size_t)k * 2 + 1) * s.N + p.col, p.cnt) : Cols<VW>{};
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++) {
+        const int r = r0 + p.rl + i * p.rowLanes;
+        v[i] = r < r1 ? load_cols<VW>(x + (size_t)r * s.N + p.col, p.cnt) : Cols<VW>{};
+    }
+    auto rowsOf = [&](int i) {
+        const int k = p.rl + i * p.rowLanes;
+        return k < s.splits ? (float)(min(s.F, (k + 1) * s.rowsPerSplit) - k * s.rowsPerSplit) : 0.f;
+    };
+    float mean[VW] = {}, m2[VW] = {};
+#pragma unroll
+    for (int i = 0; i < JOIN; i++)
+#pragma unroll
+        for (int j = 0; j < VW; j++) mean[j] += rowsOf(i) * a[i].v[j];
+    sum_rows<VW, T_SPLIT>(mean, p.cl, s.logLanes, sh);
+#pragma unroll
+    for (int j = 0; j < VW; j++) mean[j] /= (float)s.F;
+#pragma unroll
+    for (int i = 0; i < JOIN; i++)
+#pragma unroll
+        for (int j = 0; j < VW; j++) {
+            const float d = a[i].v[j] - mean[j];
+            m2[j] += b[i].v[j] + rowsOf(i) * d * d;
+        }
+    sum_rows<VW, T_SPLIT>(m2, p.cl, s.logLanes, sh);
+    Cols<VW> mu, rs;
 #pragma unroll
     for (int j = 0; j < VW; j++) {
         mu.v[j] = mean[j];
         rs.v[j] = 1.f / sqrtf(m2[j] / (float)s.F + eps);
     }
-    if (caseStats && blockIdx.y == 0 && rl == 0) {
-        store_cols<VW>(caseStats + col, mu);
-        store_cols<VW>(caseStats + s.N + col, rs);
+    if (caseStats && blockIdx.y == 0 && p.rl == 0) {
+        store_cols<VW>(caseStats + p.col, mu, p.cnt);
+        store_cols<VW>(caseStats + s.N + p.col, rs, p.cnt);
     }
-    const int r0 = blockIdx.y * s.rowsPerSplit, r1 = min(s.F, r0 + s.rowsPerSplit);
-    for (int r = r0 + rl; r < r1; r += rowLanes) {
-        Vec<VW> v = load_cols<VW>(x + (size_t)r * s.N + col);
-        const float g = gain ? gain[r] : 1.f, b = bias ? bias[r] : 0.f;
+    for (int c = r0 + p.rl; c < r1; c += AHEAD * p.rowLanes) {
 #pragma unroll
-        for (int j = 0; j < VW; j++) v.v[j] = g * ((v.v[j] - mu.v[j]) * rs.v[j]) + b;
-        store_cols<VW>(y + (size_t)r * s.N + col, v);
+        for (int i = 0; i < AHEAD; i++) {
+            const int r = c + i * p.rowLanes;
+            if (r >= r1) break;
+            const float g = gain ? gain[r] : 1.f, t = bias ? bias[r] : 0.f;
+#pragma unroll
+            for (int j = 0; j < VW; j++) v[i].v[j] = g * ((v[i].v[j] - mu.v[j]) * rs.v[j]) + t;
+            store_cols<VW>(y + (size_t)r * s.N + p.col, v[i], p.cnt);
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            const int r = c + (i + AHEAD) * p.rowLanes;
+            if (r < r1) v[i] = load_cols<VW>(x + (size_t)r * s.N + p.col, p.cnt);
+        }
     }
 }
 
-// Backward, stage 1: per range of rows the column sums of h and h xh (colPart[split][2][N]), and per tile of columns the row sums of
-// g xh and g (rowPart[tile][2][F]).
+// backward: per range the column sums of h and h xh (colPart[split][2][N]), per tile of columns the row sums of g xh and g
+// (rowPart[tile][2][F])
 template <int VW>
-__global__ __launch_bounds__(T) void k_ln_undo_sums(const float* __restrict__ g, const float* __restrict__ x, const float* __restrict__ gain,
-                                                    const float* __restrict__ caseStats, float* __restrict__ colPart,
-                                                    float* __restrict__ rowPart, LnShape s) {
-    __shared__ float sh[2][T][VW];
-    const int colLanes = 1 << s.logColLanes, rowLanes = T >> s.logColLanes;
-    const int cl = threadIdx.x & (colLanes - 1), rl = threadIdx.x >> s.logColLanes;
-    const int col = (blockIdx.x * colLanes + cl) * VW;
+__global__ __launch_bounds__(T_SPLIT) void k_ln_undo_split_sums(const float* __restrict__ g, const float* __restrict__ x,
+                                                                const float* __restrict__ gain, const float* __restrict__ caseStats,
+                                                                float* __restrict__ colPart, float* __restrict__ rowPart, Split s) {
+    __shared__ float sh[T_SPLIT / 64][64][2 * VW];
+    const Place<VW, T_SPLIT> p(blockIdx.x, s.logLanes, s.N);
     const int r0 = blockIdx.y * s.rowsPerSplit, r1 = min(s.F, r0 + s.rowsPerSplit);
-    const bool live = col < s.N;
-    Vec<VW> mu = {}, rs = {};
-    if (live) {
-        mu = load_cols<VW>(caseStats + col);
-        rs = load_cols<VW>(caseStats + s.N + col);
-    }
-    float s1[VW] = {}, s2[VW] = {};
-    const int steps = (max(r1 - r0, 0) + rowLanes - 1) / rowLanes;  // the same for every lane: the shuffles below need whole groups
+    const Cols<VW> mu = load_cols<VW>(caseStats + p.col, p.cnt), rs = load_cols<VW>(caseStats + s.N + p.col, p.cnt);
+    float v[2 * VW] = {};
+    const int steps = (max(r1 - r0, 0) + p.rowLanes - 1) / p.rowLanes;  // the same for every lane: the shuffles below need whole groups
+#pragma unroll 4
     for (int i = 0; i < steps; i++) {
-        const int r = r0 + rl + i * rowLanes;
+        const int r = r0 + p.rl + i * p.rowLanes;
         float sg = 0.f, sb = 0.f;
-        if (live && r < r1) {
-            const Vec<VW> gv = load_cols<VW>(g + (size_t)r * s.N + col), xv = load_cols<VW>(x + (size_t)r * s.N + col);
+        if (r < r1) {
+            const Cols<VW> gv = load_cols<VW>(g + (size_t)r * s.N + p.col, p.cnt), xv = load_cols<VW>(x + (size_t)r * s.N + p.col, p.cnt);
             const float ga = gain ? gain[r] : 1.f;
 #pragma unroll
             for (int j = 0; j < VW; j++) {
                 const float xh = (xv.v[j] - mu.v[j]) * rs.v[j], gx = gv.v[j] * xh;
-                s1[j] += ga * gv.v[j];
-                s2[j] += ga * gx;
+                v[j] += ga * gv.v[j];
+                v[VW + j] += ga * gx;
                 sg += gx;
                 sb += gv.v[j];
             }
         }
         if (rowPart) {
-            for (int o = colLanes >> 1; o > 0; o >>= 1) {
+            for (int o = (1 << s.logLanes) >> 1; o > 0; o >>= 1) {
                 sg += __shfl_xor(sg, o, 64);
                 sb += __shfl_xor(sb, o, 64);
             }
-            if (cl == 0 && r < r1) {
-                float* p = rowPart + (size_t)blockIdx.x * 2 * s.F + r;
-                p[0] = sg;
-                p[s.F] = sb;
+            if (p.cl == 0 && r < r1) {
+                float* out = rowPart + (size_t)blockIdx.x * 2 * s.F + r;
+                out[0] = sg;
+                out[s.F] = sb;
             }
         }
     }
+    sum_rows<2 * VW, T_SPLIT>(v, p.cl, s.logLanes, sh);
+    if (p.rl == 0) {
+        Cols<VW> a, b;
 #pragma unroll
-    for (int j = 0; j < VW; j++) {
-        sh[0][threadIdx.x][j] = s1[j];
-        sh[1][threadIdx.x][j] = s2[j];
+        for (int j = 0; j < VW; j++) { a.v[j] = v[j]; b.v[j] = v[VW + j]; }
+        float* out = colPart + (size_t)blockIdx.y * 2 * s.N + p.col;
+        store_cols<VW>(out, a, p.cnt);
+        store_cols<VW>(out + s.N, b, p.cnt);
     }
-    __syncthreads();
-    for (int half = rowLanes >> 1; half > 0; half >>= 1) {
-        if (rl < half) {
-            const int o = threadIdx.x + (half << s.logColLanes);
+}
+
+template <int VW>
+__global__ __launch_bounds__(T_SPLIT) void k_ln_undo_split_apply(const float* __restrict__ g, const float* __restrict__ x,
+                                                                 const float* __restrict__ gain, const float* __restrict__ caseStats,
+                                                                 const float* __restrict__ colPart, float* target, float scaleTargets,
+                                                                 float scaleOutput, Split s) {
+    const Place<VW, T_SPLIT> p(blockIdx.x, s.logLanes, s.N);
+    const Cols<VW> mu = load_cols<VW>(caseStats + p.col, p.cnt), rs = load_cols<VW>(caseStats + s.N + p.col, p.cnt);
+    __shared__ float sh[T_SPLIT / 64][64][2 * VW];
+    const int r0 = blockIdx.y * s.rowsPerSplit, r1 = min(s.F, r0 + s.rowsPerSplit);
+    Cols<VW> gv[AHEAD], xv[AHEAD];  // (as in the forward kernel: asked for ahead of the sums)
+    auto ask = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            const int r = c + i * p.rowLanes;
+            if (r < r1) {
+                gv[i] = load_cols<VW>(g + (size_t)r * s.N + p.col, p.cnt);
+                xv[i] = load_cols<VW>(x + (size_t)r * s.N + p.col, p.cnt);
+            }
+        }
+    };
+    float sums[2 * VW] = {};
+    {
+        Cols<VW> a[JOIN], b[JOIN];
+#pragma unroll
+        for (int i = 0; i < JOIN; i++) {
+            const int k = p.rl + i * p.rowLanes;
+            a[i] = k < s.splits ? load_cols<VW>(colPart + (size_t)k * 2 * s.N + p.col, p.cnt) : Cols<VW>{};
+            b[i] = k < s.splits ? load_cols<VW>(colPart + ((size_t)k * 2 + 1) * s.N + p.col, p.cnt) : Cols<VW>{};
+        }
+        ask(r0 + p.rl);
+#pragma unroll
+        for (int i = 0; i < JOIN; i++)
+#pragma unroll
+            for (int j = 0; j < VW; j++) { sums[j] += a[i].v[j]; sums[VW + j] += b[i].v[j]; }
+    }
+    sum_rows<2 * VW, T_SPLIT>(sums, p.cl, s.logLanes, sh);
+    const float invF = 1.f / (float)s.F;
+    float s1[VW], s2[VW];
+#pragma unroll
+    for (int j = 0; j < VW; j++) { s1[j] = sums[j] * invF; s2[j] = sums[VW + j] * invF; }
+    for (int c = r0 + p.rl; c < r1; c += AHEAD * p.rowLanes) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            const int r = c + i * p.rowLanes;
+            if (r >= r1) break;
+            const float ga = gain ? gain[r] : 1.f;
+            Cols<VW> o;
 #pragma unroll
             for (int j = 0; j < VW; j++) {
-                sh[0][threadIdx.x][j] += sh[0][o][j];
-                sh[1][threadIdx.x][j] += sh[1][o][j];
+                const float xh = (xv[i].v[j] - mu.v[j]) * rs.v[j];
+                o.v[j] = scaleOutput * (rs.v[j] * (ga * gv[i].v[j] - s1[j] - xh * s2[j]));
             }
+            float* to = target + (size_t)r * s.N + p.col;
+            if (scaleTargets != 0.f) {
+                const Cols<VW> t = load_cols<VW>(to, p.cnt);
+#pragma unroll
+                for (int j = 0; j < VW; j++) o.v[j] += scaleTargets * t.v[j];
+            }
+            store_cols<VW>(to, o, p.cnt);
         }
-        __syncthreads();
-    }
-    if (rl == 0 && live) {
-        Vec<VW> a, b;
-        for (int j = 0; j < VW; j++) { a.v[j] = sh[0][threadIdx.x][j]; b.v[j] = sh[1][threadIdx.x][j]; }
-        float* p = colPart + (size_t)blockIdx.y * 2 * s.N + col;
-        store_cols<VW>(p, a);
-        store_cols<VW>(p + s.N, b);
+        ask(c + AHEAD * p.rowLanes);
     }
 }
 
-// Backward, stage 2: dx.
-template <int VW>
-__global__ __launch_bounds__(T) void k_ln_undo_apply(const float* __restrict__ g, const float* __restrict__ x, const float* __restrict__ gain,
-                                                     const float* __restrict__ caseStats, const float* __restrict__ colPart, float* target,
-                                                     float scaleTargets, float scaleOutput, LnShape s) {
-    const int colLanes = 1 << s.logColLanes, rowLanes = T >> s.logColLanes;
-    const int cl = threadIdx.x & (colLanes - 1), rl = threadIdx.x >> s.logColLanes;
-    const int col = (blockIdx.x * colLanes + cl) * VW;
-    if (col >= s.N) return;
-    const Vec<VW> mu = load_cols<VW>(caseStats + col), rs = load_cols<VW>(caseStats + s.N + col);
-    float s1[VW] = {}, s2[VW] = {};
-    for (int k = 0; k < s.splits; k++) {
-        const Vec<VW> a = load_cols<VW>(colPart + (size_t)k * 2 * s.N + col), b = load_cols<VW>(colPart + ((size_t)k * 2 + 1) * s.N + col);
-#pragma unroll
-        for (int j = 0; j < VW; j++) { s1[j] += a.v[j]; s2[j] += b.v[j]; }
+// ---- gains' and biases' gradients from the partial row sums: 32 of the 2 F sums x 16 lanes over the partials per block
+__global__ __launch_bounds__(512) void k_ln_undo_rows(const float* __restrict__ rowPart, float* gainGrad, float* biasGrad, float gainTargets,
+                                                      float gainOutput, float biasTargets, float biasOutput, int F, int parts) {
+    __shared__ float sh[16][33];
+    const int c = threadIdx.x & 31, l = threadIdx.x >> 5, i = blockIdx.x * 32 + c;
+    float v = 0.f;
+    if (i < 2 * F) {
+#pragma unroll 4
+        for (int t = l; t < parts; t += 16) v += rowPart[(size_t)t * 2 * F + i];
     }
-    const float invF = 1.f / (float)s.F;
-#pragma unroll
-    for (int j = 0; j < VW; j++) { s1[j] *= invF; s2[j] *= invF; }
-    const int r0 = blockIdx.y * s.rowsPerSplit, r1 = min(s.F, r0 + s.rowsPerSplit);
-    for (int r = r0 + rl; r < r1; r += rowLanes) {
-        const size_t at = (size_t)r * s.N + col;
-        const Vec<VW> gv = load_cols<VW>(g + at), xv = load_cols<VW>(x + at);
-        const float ga = gain ? gain[r] : 1.f;
-        Vec<VW> o;
-#pragma unroll
-        for (int j = 0; j < VW; j++) {
-            const float xh = (xv.v[j] - mu.v[j]) * rs.v[j];
-            o.v[j] = scaleOutput * (rs.v[j] * (ga * gv.v[j] - s1[j] - xh * s2[j]));
-        }
-        if (scaleTargets != 0.f) {
-            const Vec<VW> t = load_cols<VW>(target + at);
-#pragma unroll
-            for (int j = 0; j < VW; j++) o.v[j] += scaleTargets * t.v[j];
-        }
-        store_cols<VW>(target + at, o);
-    }
-}
-
-// Backward, stage 3: the gains' and biases' gradients from the tiles' row sums.
-__global__ __launch_bounds__(T) void k_ln_undo_rows(const float* __restrict__ rowPart, float* gainGrad, float* biasGrad, float gainTargets,
-                                                    float gainOutput, float biasTargets, float biasOutput, int F, int tiles) {
-    const int i = blockIdx.x * T + threadIdx.x;
-    if (i >= 2 * F) return;
+    sh[l][c] = v;
+    __syncthreads();
+    if (l != 0 || i >= 2 * F) return;
+    for (int k = 1; k < 16; k++) v += sh[k][c];
     const bool isBias = i >= F;
     float* out = isBias ? biasGrad : gainGrad;
     if (!out) return;
-    float v = 0.f;
-    for (int t = 0; t < tiles; t++) v += rowPart[(size_t)t * 2 * F + i];
     const float sT = isBias ? biasTargets : gainTargets, sO = isBias ? biasOutput : gainOutput;
     const int f = isBias ? i - F : i;
     out[f] = (sT != 0.f ? sT * out[f] : 0.f) + sO * v;
+}
+
+// How a shape is laid out.
+struct Plan {
+    bool whole;
+    int vw, logLanes, tiles;  // whole
+    int blocks;               // backward, whole
+    Split split;
+};
+constexpr int FWD_ROWS = 16, BWD_ROWS = 8;       // rows a thread of the whole kernels holds
+// rows: FWD_ROWS or BWD_ROWS
+Plan ln_plan(int F, int N, int rows) {
+    Plan p = {};
+    p.vw = N >= 4 ? 4 : 1;
+    const int lanes = divup(N, p.vw), most = T_WHOLE * rows;
+    // whole: four column lanes (64 bytes of a row) are the fastest where there are tiles for every CU and the rows fit, fewer else
+    int lg = p.vw == 1 ? (N == 1 ? 0 : N == 2 ? 1 : 2) : 2;
+    while (p.vw == 4 && lg > 0 && (divup(lanes, 1 << lg) < CUS || ((size_t)F << lg) > (size_t)most)) lg--;
+    p.logLanes = lg;
+    p.tiles = divup(lanes, 1 << lg);
+    // one lane a row (16 bytes) only pays where the matrix is small
+    p.whole = ((size_t)F << lg) <= (size_t)most && (lg > 0 || p.tiles <= CUS);
+    p.blocks = std::min(divup(p.tiles, 8) * 8, 4 * CUS);
+    Split& s = p.split;
+    s.F = F;
+    s.N = N;
+    s.logLanes = 0;
+    while ((1 << s.logLanes) < lanes && s.logLanes < 4) s.logLanes++;
+    s.colTiles = divup(lanes, 1 << s.logLanes);
+    const int rowLanes = T_SPLIT >> s.logLanes;
+    s.splits = std::max(1, std::min({64, JOIN * rowLanes, divup(4 * CUS, s.colTiles), divup(F, 4 * rowLanes)}));
+    s.rowsPerSplit = divup(F, s.splits);
+    s.splits = divup(F, s.rowsPerSplit);
+    return p;
 }
 
 inline bool al16(const void* p) { return ((uintptr_t)p % 16) == 0; }
@@ -305,16 +541,12 @@ int ln_require_workspace(const void* ws, size_t have, size_t need, const char* w
     return MCN_OK;
 }
 
-size_t al4(size_t n) { return (n + 3) / 4 * 4; }
-
 }  // namespace
 
-// The workspace does not depend on the pointers' alignment: the larger of the two forms.
 MCN_API size_t mcn_layer_norm_workspace_bytes(int numFeatures, int numCases) {
     if (!ln_sizes_ok(numFeatures, numCases)) return 0;
-    size_t b = 0;
-    for (int vw = 1; vw <= 4; vw += 3) b = std::max(b, (size_t)ln_shape(numFeatures, numCases, vw).splits * 2 * numCases * sizeof(float));
-    return b;
+    const Plan p = ln_plan(numFeatures, numCases, FWD_ROWS);
+    return p.whole ? 0 : (size_t)p.split.splits * 2 * numCases * sizeof(float);
 }
 
 MCN_API int mcn_layer_norm(const float* inputs, const float* gains, const float* biases, float* target, float* caseStats, int numFeatures,
@@ -323,28 +555,37 @@ MCN_API int mcn_layer_norm(const float* inputs, const float* gains, const float*
     MCN_REQUIRE(eps > 0.f, "layerNorm: eps %g is not positive", (double)eps);
     if (int rc = ln_require_workspace(workspace, workspaceBytes, mcn_layer_norm_workspace_bytes(numFeatures, numCases), "layerNorm")) return rc;
     hipStream_t st = (hipStream_t)stream;
-    float* part = (float*)workspace;
-    const bool vec = numCases % 4 == 0 && al16(inputs) && al16(target) && al16(caseStats);
-    const LnShape s = ln_shape(numFeatures, numCases, vec ? 4 : 1);
-    const dim3 grid(s.colTiles, s.splits);
-    if (vec) {
-        MCN_LAUNCH(k_ln_stats<4>, grid, dim3(T), 0, st, inputs, part, s);
-        MCN_LAUNCH(k_ln_apply<4>, grid, dim3(T), 0, st, inputs, gains, biases, target, caseStats, part, eps, s);
+    const int F = numFeatures, N = numCases;
+    const Plan p = ln_plan(F, N, FWD_ROWS);
+    if (p.whole) {
+        const dim3 grid(divup(p.tiles, 8) * 8);
+#define WHOLE(VW, R) MCN_LAUNCH((k_ln_whole<VW, R>), grid, dim3(T_WHOLE), 0, st, inputs, gains, biases, target, caseStats, eps, F, N, p.logLanes, p.tiles)
+        const bool few = ((size_t)F << p.logLanes) <= T_WHOLE * 4;
+        if (p.vw == 4 && few) WHOLE(4, 4);
+        else if (p.vw == 4) WHOLE(4, FWD_ROWS);
+        else if (few) WHOLE(1, 4);
+        else WHOLE(1, FWD_ROWS);
+#undef WHOLE
     } else {
-        MCN_LAUNCH(k_ln_stats<1>, grid, dim3(T), 0, st, inputs, part, s);
-        MCN_LAUNCH(k_ln_apply<1>, grid, dim3(T), 0, st, inputs, gains, biases, target, caseStats, part, eps, s);
+        const Split& s = p.split;
+        const dim3 grid(s.colTiles, s.splits);
+        float* part = (float*)workspace;
+        if (p.vw == 4) {
+            MCN_LAUNCH(k_ln_split_stats<4>, grid, dim3(T_SPLIT), 0, st, inputs, part, s);
+            MCN_LAUNCH(k_ln_split_apply<4>, grid, dim3(T_SPLIT), 0, st, inputs, gains, biases, target, caseStats, part, eps, s);
+        } else {
+            MCN_LAUNCH(k_ln_split_stats<1>, grid, dim3(T_SPLIT), 0, st, inputs, part, s);
+            MCN_LAUNCH(k_ln_split_apply<1>, grid, dim3(T_SPLIT), 0, st, inputs, gains, biases, target, caseStats, part, eps, s);
+        }
     }
     return MCN_LAUNCH_CHECK("layerNorm");
 }
 
 MCN_API size_t mcn_layer_norm_undo_workspace_bytes(int numFeatures, int numCases) {
     if (!ln_sizes_ok(numFeatures, numCases)) return 0;
-    size_t b = 0;
-    for (int vw = 1; vw <= 4; vw += 3) {
-        const LnShape s = ln_shape(numFeatures, numCases, vw);
-        b = std::max(b, (al4((size_t)s.splits * 2 * numCases) + (size_t)s.colTiles * 2 * numFeatures) * sizeof(float));
-    }
-    return b;
+    const Plan p = ln_plan(numFeatures, numCases, BWD_ROWS);
+    const size_t parts = p.whole ? p.blocks : p.split.colTiles;
+    return (parts * 2 * numFeatures + (p.whole ? 0 : (size_t)p.split.splits * 2 * numCases)) * sizeof(float);
 }
 
 MCN_API int mcn_layer_norm_undo(const float* outGrads, const float* inputs, const float* gains, const float* caseStats, float* target,
@@ -356,24 +597,36 @@ MCN_API int mcn_layer_norm_undo(const float* outGrads, const float* inputs, cons
     MCN_REQUIRE(target != outGrads && target != inputs, "layerNormUndo: the target is one of the operands");
     if (int rc = ln_require_workspace(workspace, workspaceBytes, mcn_layer_norm_undo_workspace_bytes(numFeatures, numCases), "layerNormUndo")) return rc;
     hipStream_t st = (hipStream_t)stream;
-    const bool vec = numCases % 4 == 0 && al16(outGrads) && al16(inputs) && al16(caseStats) && al16(target);
-    const LnShape s = ln_shape(numFeatures, numCases, vec ? 4 : 1);
-    float* colPart = (float*)workspace;
+    const int F = numFeatures, N = numCases;
+    const Plan p = ln_plan(F, N, BWD_ROWS);
     const bool rows = gainGrads || biasGrads;
-    float* rowPart = rows ? colPart + al4((size_t)s.splits * 2 * numCases) : nullptr;
-    const dim3 grid(s.colTiles, s.splits);
-    if (vec)
-        MCN_LAUNCH(k_ln_undo_sums<4>, grid, dim3(T), 0, st, outGrads, inputs, gains, caseStats, colPart, rowPart, s);
-    else
-        MCN_LAUNCH(k_ln_undo_sums<1>, grid, dim3(T), 0, st, outGrads, inputs, gains, caseStats, colPart, rowPart, s);
-    if (target) {
-        if (vec)
-            MCN_LAUNCH(k_ln_undo_apply<4>, grid, dim3(T), 0, st, outGrads, inputs, gains, caseStats, colPart, target, scaleTargets, scaleOutput, s);
-        else
-            MCN_LAUNCH(k_ln_undo_apply<1>, grid, dim3(T), 0, st, outGrads, inputs, gains, caseStats, colPart, target, scaleTargets, scaleOutput, s);
+    float* rowPart = rows ? (float*)workspace : nullptr;
+    int parts;
+    if (p.whole) {
+        parts = p.blocks;
+#define WHOLE(VW, R) MCN_LAUNCH((k_ln_undo_whole<VW, R>), dim3(p.blocks), dim3(T_WHOLE), 0, st, outGrads, inputs, gains, caseStats, target, \
+                                rowPart, scaleTargets, scaleOutput, F, N, p.logLanes, p.tiles)
+        const bool few = ((size_t)F << p.logLanes) <= T_WHOLE * 2;
+        if (p.vw == 4 && few) WHOLE(4, 2);
+        else if (p.vw == 4) WHOLE(4, BWD_ROWS);
+        else if (few) WHOLE(1, 2);
+        else WHOLE(1, BWD_ROWS);
+#undef WHOLE
+    } else {
+        const Split& s = p.split;
+        const dim3 grid(s.colTiles, s.splits);
+        parts = s.colTiles;
+        float* colPart = (float*)workspace + (size_t)parts * 2 * F;
+        if (p.vw == 4) {
+            MCN_LAUNCH(k_ln_undo_split_sums<4>, grid, dim3(T_SPLIT), 0, st, outGrads, inputs, gains, caseStats, colPart, rowPart, s);
+            if (target) MCN_LAUNCH(k_ln_undo_split_apply<4>, grid, dim3(T_SPLIT), 0, st, outGrads, inputs, gains, caseStats, colPart, target, scaleTargets, scaleOutput, s);
+        } else {
+            MCN_LAUNCH(k_ln_undo_split_sums<1>, grid, dim3(T_SPLIT), 0, st, outGrads, inputs, gains, caseStats, colPart, rowPart, s);
+            if (target) MCN_LAUNCH(k_ln_undo_split_apply<1>, grid, dim3(T_SPLIT), 0, st, outGrads, inputs, gains, caseStats, colPart, target, scaleTargets, scaleOutput, s);
+        }
     }
     if (rows)
-        MCN_LAUNCH(k_ln_undo_rows, dim3((unsigned)divup_sz((size_t)2 * numFeatures, T)), dim3(T), 0, st, rowPart, gainGrads, biasGrads, scaleGainTargets,
-                   scaleGainOutput, scaleBiasTargets, scaleBiasOutput, numFeatures, s.colTiles);
+        MCN_LAUNCH(k_ln_undo_rows, dim3((unsigned)divup_sz((size_t)2 * F, 32)), dim3(512), 0, st, rowPart, gainGrads, biasGrads, scaleGainTargets,
+                   scaleGainOutput, scaleBiasTargets, scaleBiasOutput, F, parts);
     return MCN_LAUNCH_CHECK("layerNormUndo");
 }
