@@ -242,42 +242,46 @@ __global__ __launch_bounds__(T_SPLIT) void k_ln_split_stats(const float* __restr
     constexpr int T = T_SPLIT, R = 8;
     __shared__ float sh[T / 64][64][VW];
     const Place<VW, T> p(blockIdx.x, s.logLanes, s.N);
-    const int r0 = blockIdx.y * s.rowsPerSplit, r1 = min(s.F, r0 + s.rowsPerSplit), chunk = p.rowLanes * R;
+    const int r0 = blockIdx.y * s.rowsPerSplit, r1 = min(s.F, r0 + s.rowsPerSplit);
+    // a thread: R rows at a time, their mean and deviations exactly, then joined to what it has
     float n = 0.f, mean[VW] = {}, m2[VW] = {};
-    for (int c = r0; c < r1; c += chunk) {  // (the same number of chunks for every thread: barriers below)
+    for (int c = r0 + p.rl; c < r1; c += R * p.rowLanes) {
         Cols<VW> v[R];
+        const int have = min(R, (r1 - c + p.rowLanes - 1) / p.rowLanes);
 #pragma unroll
-        for (int i = 0; i < R; i++) {
-            const int r = c + p.rl + i * p.rowLanes;
-            v[i] = r < r1 ? load_cols<VW>(x + (size_t)r * s.N + p.col, p.cnt) : Cols<VW>{};
-        }
-        float a[VW] = {}, b[VW] = {};
-#pragma unroll
-        for (int i = 0; i < R; i++)
-#pragma unroll
-            for (int j = 0; j < VW; j++) a[j] += v[i].v[j];
-        sum_rows<VW, T>(a, p.cl, s.logLanes, sh);
-        const float rows = (float)min(chunk, r1 - c);
-#pragma unroll
-        for (int j = 0; j < VW; j++) a[j] /= rows;
-#pragma unroll
-        for (int i = 0; i < R; i++) {
-            const bool in = c + p.rl + i * p.rowLanes < r1;
-#pragma unroll
-            for (int j = 0; j < VW; j++) {
-                const float d = v[i].v[j] - a[j];
-                b[j] += in ? d * d : 0.f;
-            }
-        }
-        sum_rows<VW, T>(b, p.cl, s.logLanes, sh);
+        for (int i = 0; i < R; i++) v[i] = i < have ? load_cols<VW>(x + (size_t)(c + i * p.rowLanes) * s.N + p.col, p.cnt) : Cols<VW>{};
+        const float rows = (float)have, inv = 1.f / rows;
         float t = n;
 #pragma unroll
         for (int j = 0; j < VW; j++) {
+            float a = 0.f, b = 0.f;
+#pragma unroll
+            for (int i = 0; i < R; i++) a += v[i].v[j];
+            a *= inv;
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                const float d = v[i].v[j] - a;
+                b += i < have ? d * d : 0.f;
+            }
             t = n;
-            join(t, mean[j], m2[j], rows, a[j], b[j]);
+            join(t, mean[j], m2[j], rows, a, b);
         }
         n = t;
     }
+    // then the row lanes: the mean of all, and the deviations about it
+    const float invAll = 1.f / (float)(r1 - r0);
+    float all[VW];
+#pragma unroll
+    for (int j = 0; j < VW; j++) all[j] = n * mean[j];
+    sum_rows<VW, T>(all, p.cl, s.logLanes, sh);
+#pragma unroll
+    for (int j = 0; j < VW; j++) {
+        all[j] *= invAll;
+        const float d = mean[j] - all[j];
+        m2[j] += n * d * d;
+        mean[j] = all[j];
+    }
+    sum_rows<VW, T>(m2, p.cl, s.logLanes, sh);
     if (p.rl == 0) {
         Cols<VW> a, b;
 #pragma unroll
