@@ -10,16 +10,18 @@
 
 namespace {
 
-constexpr int BV = 64, BN = 64, BK = 32;  // k_fcl_tile: classes x cases, features per step
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // (16-byte accesses at any multiple of four bytes)
+
+constexpr int NARROW = 64;  // k_fcl_narrow: most cases
+constexpr size_t NARROW_GRAD = (size_t)1 << 23;  // ... and weights, for the gradients
 constexpr size_t PIECE_ELEMS = (size_t)1 << 24;
 constexpr int PIECE_MB = 128;  // fragments of a piece; 512 x 100000 x 1024, both calls: 64 MB 1.77 ms, 128 MB 1.65 ms, 224 MB 1.62 ms
 
-struct FclArgs {
+struct NarrowArgs {
     const float *W, *X, *bias, *labels;
     int D, V, N;
     int v0, vRows;        // the piece: classes [v0, v0 + vRows)
-    int nTiles;
-    float* part;          // forward: [vTiles][3][N]
+    float* part;          // forward: [tiles][3][N]
     float* labelLogits;   // forward: [N]
     const float* stats;   // backward: [2][N]
     float* dz;            // backward: [vRows][N]
@@ -50,129 +52,165 @@ __device__ __forceinline__ bool label_of(float l, int V, int& label) {
     return ok;
 }
 
-template <bool BWD>
-__global__ __launch_bounds__(256) void k_fcl_tile(FclArgs p) {
-    __shared__ float As[BV][BK + 4];
-    __shared__ float Bs[BK][BN + 4];
-    __shared__ float red[3][4][BN];
-    const int tn = blockIdx.x % p.nTiles, tv = blockIdx.x / p.nTiles;
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    const int vBase = tv * BV, nBase = tn * BN;
-    f32x4 acc[4] = {};
-    for (int k0 = 0; k0 < p.D; k0 += BK) {
+// exp(x) for x <= 0, to about one unit in the last place: 2^(x log2 e) with the product's rounding error carried along.  Below -104 the
+// result is no normal number, and 0 will do; a NaN comes through.
+__device__ __forceinline__ float exp_neg(float x) {
+    constexpr float L = 1.44269504f, L_LOW = 1.925963033500e-8f, LN2 = 0.693147181f;  // log2 e = L + L_LOW
+    x = x < -104.f ? -104.f : x;
+    const float h = x * L, l = fmaf(x, L_LOW, fmaf(x, L, -h));
+    const float e = __builtin_amdgcn_exp2f(h);
+    return fmaf(e * LN2, l, e);
+}
+
+// Few cases (at most 16 NB): bound by reading W once, so fp32 matrix instructions do, straight from the operands' own layouts.  A block
+// takes 16 RG classes, its four waves a quarter of the features each (16 at a time: a lane reads 16 bytes of its class's row, and the
+// four matrix instructions that follow take one feature of every lane's four); their sums are joined in LDS.  RG = 1 while the classes
+// do not fill the chip, 4 beyond, where it keeps the number of tiles to join down.
+template <bool BWD, int NB, int RG>
+__global__ __launch_bounds__(256) void k_fcl_narrow(NarrowArgs p) {
+    __shared__ f32x4 red[4][RG][NB][64];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int vBase = blockIdx.x * 16 * RG;
+    const float* rowPtr[RG];
 #pragma unroll
-        for (int u = 0; u < BV * BK / 256; u++) {
-            const int e = tid + 256 * u, r = e / BK, k = e % BK;
-            const bool in = vBase + r < p.vRows && k0 + k < p.D;
-            As[r][k] = in ? p.W[(size_t)(p.v0 + vBase + r) * p.D + k0 + k] : 0.f;
-        }
+    for (int q = 0; q < RG; q++) rowPtr[q] = p.W + (size_t)(p.v0 + min(vBase + q * 16 + c, p.vRows - 1)) * p.D;  // (a class behind the last one: read and not used)
+    f32x4 acc[RG][NB] = {};
+    const int steps = (p.D + 15) / 16;
+#pragma unroll 4
+    for (int t = wave; t < steps; t += 4) {
+        const int k = t * 16 + g * 4;
+        f32x4 a[RG];
+        float b[NB][4];
+        const bool whole = k + 4 <= p.D;
 #pragma unroll
-        for (int u = 0; u < BK * BN / 256; u++) {
-            const int e = tid + 256 * u, k = e / BN, c = e % BN;
-            const bool in = nBase + c < p.N && k0 + k < p.D;
-            Bs[k][c] = in ? p.X[(size_t)(k0 + k) * p.N + nBase + c] : 0.f;
-        }
-        __syncthreads();
+        for (int q = 0; q < RG; q++) {
+            if (whole) {
+                const f32x4u u = *reinterpret_cast<const f32x4u*>(rowPtr[q] + k);
+                a[q] = (f32x4){u[0], u[1], u[2], u[3]};
+            } else {
 #pragma unroll
-        for (int k = 0; k < BK; k += 4) {
-            const float a = As[wave * 16 + (lane & 15)][k + (lane >> 4)];
-#pragma unroll
-            for (int t = 0; t < 4; t++) acc[t] = mfma16(a, Bs[k + (lane >> 4)][t * 16 + (lane & 15)], acc[t]);
-        }
-        __syncthreads();
-    }
-    const int rowInPiece = vBase + wave * 16 + (lane >> 4) * 4;
-    float bv[4];
-    bool live[4];
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-        live[r] = rowInPiece + r < p.vRows;
-        bv[r] = live[r] && p.bias ? p.bias[p.v0 + rowInPiece + r] : 0.f;
-    }
-#pragma unroll
-    for (int t = 0; t < 4; t++) {
-        const int c = t * 16 + (lane & 15), n = nBase + c;
-        int label = -1;
-        if (n < p.N) label_of(p.labels[n], p.V, label);
-        float z[4];
-#pragma unroll
-        for (int r = 0; r < 4; r++) z[r] = acc[t][r] + bv[r];
-        if (BWD) {
-            if (n < p.N) {
-                const float M = p.stats[n], S = p.stats[p.N + n];
-                const float inv = label >= 0 && S != 0.f ? 1.f / S : 0.f;
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-                    if (live[r]) {
-                        const float prob = inv != 0.f ? expf(z[r] - M) * inv : 0.f;
-                        const float hot = label == p.v0 + rowInPiece + r ? 1.f : 0.f;
-                        p.dz[(size_t)(rowInPiece + r) * p.N + n] = label >= 0 && S != 0.f ? p.coeff * (hot - prob) : 0.f;
-                    }
+                for (int j = 0; j < 4; j++) a[q][j] = k + j < p.D ? rowPtr[q][k + j] : 0.f;
             }
-            continue;
         }
-        float m = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < NB; n++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) b[n][j] = n * 16 + c < p.N && k + j < p.D ? p.X[(size_t)(k + j) * p.N + n * 16 + c] : 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int q = 0; q < RG; q++)
+#pragma unroll
+                for (int n = 0; n < NB; n++) acc[q][n] = mfma16(a[q][j], b[n][j], acc[q][n]);
+    }
+#pragma unroll
+    for (int q = 0; q < RG; q++)
+#pragma unroll
+        for (int n = 0; n < NB; n++) red[wave][q][n][lane] = acc[q][n];
+    __syncthreads();
+    if (wave >= NB) return;  // a wave: 16 cases
+    const int n = wave * 16 + c;
+    int label = -1;
+    float M = 0.f, S = 0.f;
+    if (n < p.N && label_of(p.labels[n], p.V, label) && BWD) {
+        M = p.stats[n];
+        S = p.stats[p.N + n];
+    }
+    float z[RG][4], m = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < RG; q++) {
+        const f32x4 s = (red[0][q][wave][lane] + red[1][q][wave][lane]) + (red[2][q][wave][lane] + red[3][q][wave][lane]);
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-            if (live[r] && z[r] > m) m = z[r];
-            if (live[r] && label == p.v0 + rowInPiece + r && n < p.N) p.labelLogits[n] = z[r];
-        }
-        for (int o = 16; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-        float s = 0.f, cnt = 0.f;
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-            if (live[r] && z[r] != -INFINITY) {  // (a masked class adds nothing; a NaN comes through)
-                const bool top = z[r] == m && m < INFINITY;
-                s += top ? 0.f : expf(z[r] - m);
-                cnt += top ? 1.f : 0.f;
-            }
-        for (int o = 16; o < 64; o <<= 1) {
-            s += __shfl_xor(s, o, 64);
-            cnt += __shfl_xor(cnt, o, 64);
-        }
-        if (lane < 16) {
-            red[0][wave][c] = m;
-            red[1][wave][c] = s;
-            red[2][wave][c] = cnt;
+            const int v = vBase + q * 16 + g * 4 + r;
+            const float bv = v < p.vRows ? (p.bias ? p.bias[p.v0 + v] : 0.f) : -INFINITY;
+            z[q][r] = bv == -INFINITY ? -INFINITY : s[r] + bv;  // (a class that is taken out, whatever its weights hold)
+            m = fmaxf(z[q][r], m);
         }
     }
-    if (BWD) return;
-    __syncthreads();
-    if (tid < BN && nBase + tid < p.N) {
-        Stat a = {-INFINITY, 0.f, 0.f};
-        for (int w = 0; w < 4; w++) stat_join(a, red[0][w][tid], red[1][w][tid], red[2][w][tid]);
-        float* out = p.part + (size_t)tv * 3 * p.N + nBase + tid;
-        out[0] = a.m;
-        out[p.N] = a.rest;
-        out[2 * (size_t)p.N] = a.cnt;
+    if (BWD) {
+        const bool counts = S != 0.f;  // (no label, or no class left: nothing; a NaN goes on)
+        const float inv = counts ? 1.f / S : 0.f;
+#pragma unroll
+        for (int q = 0; q < RG; q++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int v = vBase + q * 16 + g * 4 + r;
+                if (v < p.vRows && n < p.N) {
+                    const float hot = label == p.v0 + v ? 1.f : 0.f;
+                    p.dz[(size_t)v * p.N + n] = counts ? p.coeff * (hot - exp_neg(z[q][r] - M) * inv) : 0.f;
+                }
+            }
+        return;
+    }
+    for (int o = 16; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    const float from = m == -INFINITY ? 0.f : m;
+    float rest = 0.f, cnt = 0.f;
+#pragma unroll
+    for (int q = 0; q < RG; q++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const float x = z[q][r] - from;
+            const bool top = x == 0.f && m != -INFINITY;
+            rest += top ? 0.f : exp_neg(x);
+            cnt += top ? 1.f : 0.f;
+            if (label >= 0 && label == p.v0 + vBase + q * 16 + g * 4 + r) p.labelLogits[n] = z[q][r];
+        }
+    for (int o = 16; o < 64; o <<= 1) {
+        rest += __shfl_xor(rest, o, 64);
+        cnt += __shfl_xor(cnt, o, 64);
+    }
+    if (g == 0 && n < p.N) {
+        float* out = p.part + (size_t)blockIdx.x * 3 * p.N + n;
+        out[0] = m;
+        out[p.N] = rest;
+        out[2 * (size_t)p.N] = cnt;
     }
 }
 
 // Joins the tiles of every case: 16 cases x 64 tile lanes per block; first the max, then the sums, so that no exponential waits for
-// another (running joins of 782 tiles took 32 us for 1024 cases).
+// another.  A lane asks for all of its first eight tiles at once and keeps them (up to 512 tiles: one trip to memory).
 __global__ __launch_bounds__(1024) void k_fcl_join(const float* __restrict__ part, const float* __restrict__ labelLogits,
                                                    const float* __restrict__ labels, float* __restrict__ caseStats, float* __restrict__ logProbs,
                                                    float* __restrict__ correct, int V, int N, int tiles) {
+    constexpr int KEPT = 8;
     __shared__ float sh[2][64][17];
     const int c = threadIdx.x & 15, l = threadIdx.x >> 4, n = blockIdx.x * 16 + c;
+    const float* at = part + (size_t)l * 3 * N + n;
+    const size_t step = (size_t)64 * 3 * N;
+    float km[KEPT], kr[KEPT], kc[KEPT];
+#pragma unroll
+    for (int i = 0; i < KEPT; i++) {
+        const bool in = n < N && l + 64 * i < tiles;
+        km[i] = in ? at[i * step] : -INFINITY;
+        kr[i] = in ? at[i * step + N] : 0.f;
+        kc[i] = in ? at[i * step + 2 * (size_t)N] : 0.f;
+    }
     float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < KEPT; i++) m = fmaxf(m, km[i]);
     if (n < N) {
 #pragma unroll 8
-        for (int t = l; t < tiles; t += 64) m = fmaxf(m, part[(size_t)t * 3 * N + n]);
+        for (int t = l + 64 * KEPT; t < tiles; t += 64) m = fmaxf(m, part[(size_t)t * 3 * N + n]);
     }
     sh[0][l][c] = m;
     __syncthreads();
     for (int k = 0; k < 64; k++) m = fmaxf(m, sh[0][k][c]);
     __syncthreads();
     float rest = 0.f, cnt = 0.f;
+    auto add = [&](float tm, float tr, float tc) {
+        const bool top = tm == m;
+        // (a tile without a finite logit holds 0, or a NaN, which stays)
+        rest += top ? tr : (tr + tc) * (tm == -INFINITY ? 1.f : expf(tm - m));
+        cnt += top ? tc : 0.f;
+    };
+#pragma unroll
+    for (int i = 0; i < KEPT; i++) add(km[i], kr[i], kc[i]);
     if (n < N) {
 #pragma unroll 8
-        for (int t = l; t < tiles; t += 64) {
+        for (int t = l + 64 * KEPT; t < tiles; t += 64) {
             const float* q = part + (size_t)t * 3 * N + n;
-            const bool top = q[0] == m;
-            // (a tile without a finite logit holds 0, or a NaN, which stays)
-            rest += top ? q[N] : (q[N] + q[2 * (size_t)N]) * (q[0] == -INFINITY ? 1.f : expf(q[0] - m));
-            cnt += top ? q[2 * (size_t)N] : 0.f;
+            add(q[0], q[N], q[2 * (size_t)N]);
         }
     }
     sh[0][l][c] = rest;
@@ -245,7 +283,6 @@ __global__ __launch_bounds__(256) void k_fcl_cost(const float* __restrict__ labe
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef __fp16 fp16x4 __attribute__((__vector_size__(4 * sizeof(__fp16))));  // (the type the transposing read is declared with)
-typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr int FRAG = 1024, PAIR = 2 * FRAG;  // bytes of a fragment, of its two pieces
 constexpr int TILE = 128;                    // columns of a product's tile
@@ -638,16 +675,6 @@ __global__ __launch_bounds__(512) void k_fcl_pack_w(const float* __restrict__ W,
     }
 }
 
-// exp(x) for x <= 0, to about one unit in the last place: 2^(x log2 e) with the product's rounding error carried along.  Below -104 the
-// result is no normal number, and 0 will do; a NaN comes through.
-__device__ __forceinline__ float exp_neg(float x) {
-    constexpr float L = 1.44269504f, L_LOW = 1.925963033500e-8f, LN2 = 0.693147181f;  // log2 e = L + L_LOW
-    x = x < -104.f ? -104.f : x;
-    const float h = x * L, l = fmaf(x, L_LOW, fmaf(x, L, -h));
-    const float e = __builtin_amdgcn_exp2f(h);
-    return fmaf(e * LN2, l, e);
-}
-
 // ---- logits of a piece
 struct WideArgs {
     const char *wByClass, *xByCase;
@@ -965,10 +992,15 @@ int tile_bytes(TileKind k) { return k == SHARED ? SHARED_LDS : tile_lds(tile_row
 struct WidePlan {
     int Np, Dp, Kd, kSteps, Kn, nTiles, dTiles;  // Kd: k blocks of W's and x's fragments, padded; kSteps: those that hold anything
     int rows, Kv;                                // classes per piece; k blocks of a whole piece, padded
-    int splits;                                  // input gradient
+    int kPerSplit, splits;                       // input gradient: every split of a whole piece holds something, so that the first piece
+                                                 // writes every slab
     size_t classExp, caseExp, featExp, xByCase, xByFeat, wByClass, dz, dbPart, slabs, part, labelLogits, total;
 };
-bool wide_usable(int D, int V, int N) { return N > 48; }
+// When the packed operands pay (us, narrow / wide).  Cost, 512 x 10575: 16 cases 16 / 34, 64 cases 26 / 35; 512 x 100000: 56 / 145, 121 / 147.
+// Gradients, whose narrow form takes dz through mcn_gemm: 512 x 10575 16 cases 51 / 59, 64 cases 60 / 60; 2048 x 10575 179 / 152;
+// 512 x 100000 404 / 314: by the number of weights.
+bool wide_cost_usable(int N) { return N > NARROW; }
+bool wide_grad_usable(int D, int V, int N) { return N > NARROW || (size_t)D * V > NARROW_GRAD; }
 
 size_t al256(size_t b) { return (b + 255) / 256 * 256; }
 
@@ -988,7 +1020,8 @@ WidePlan wide_plan(int D, int V, int N, bool bwd) {
     const int round = std::max(1, 512 / p.nTiles) * TILE;
     p.rows = std::min(V, most > round ? most / round * round : most);
     p.Kv = divup(p.rows, TILE) * 4;
-    p.splits = std::max(1, std::min(p.Kv / 8, 512 / (p.nTiles * p.dTiles)));
+    p.kPerSplit = divup(p.Kv, std::max(1, std::min(p.Kv / 8, 512 / (p.nTiles * p.dTiles))));
+    p.splits = divup(p.Kv, p.kPerSplit);
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t o = at; at += al256(bytes); return o; };
     p.classExp = take((size_t)p.Kv * 4);
@@ -1093,7 +1126,7 @@ int wide_grad(const float* W, const float* X, const float* bias, const float* la
         }
         if (dX) {
             // (a short last piece has fewer, not shorter, shares: each adds to its slab)
-            const int tiles = q.nTiles * q.dTiles, kPer = std::max(std::min(8, a.Kv), divup(a.Kv, q.splits)), splits = divup(a.Kv, kPer);
+            const int tiles = q.nTiles * q.dTiles, kPer = a.Kv == q.Kv ? q.kPerSplit : std::max(8, divup(a.Kv, q.splits)), splits = divup(a.Kv, kPer);
             const dim3 grid(splits * tiles), block(256);
 #define IGRAD(SH, KIND) MCN_LAUNCH((k_fcl_igrad<4, SH>), grid, block, tile_bytes(KIND), s, a.dz, a.wByClass, a.classExp, slabs, q.Np, q.Dp, a.Kv, q.Kd, kPer, q.nTiles, q.dTiles, v0 == 0)
             if (splits * tiles > 256) IGRAD(true, SHARED);
@@ -1112,24 +1145,42 @@ int wide_grad(const float* W, const float* X, const float* bias, const float* la
 
 bool fcl_sizes_ok(int D, int V, int N) { return D > 0 && V > 0 && N > 0 && V <= (1 << 24) && D <= (1 << 20) && N <= (1 << 20); }
 
-int fcl_piece_rows(int V, int D, int N) {
-    const size_t rows = std::min<size_t>(PIECE_ELEMS / (size_t)std::max(N, D), (size_t)1 << 19) / BV * BV;
-    return (int)std::min<size_t>((size_t)V, std::max<size_t>(rows, BV));
-}
-
 size_t al16b(size_t b) { return (b + 15) / 16 * 16; }
 
-size_t fcl_cost_bytes(int D, int V, int N) {
-    if (wide_usable(D, V, N)) return wide_plan(D, V, N, false).total;
-    return al16b((size_t)divup(V, BV) * 3 * N * sizeof(float)) + al16b((size_t)N * sizeof(float));
+// The narrow path: tiles of the forward pass, and the pieces whose dz (and the products that take it) fit the workspace.
+int narrow_groups(int V) { return V > 16 * 1024 ? 4 : 1; }
+int narrow_tiles(int V) { return divup(V, 16 * narrow_groups(V)); }
+int narrow_piece(int V, int D, int N) {
+    const size_t rows = std::min<size_t>(PIECE_ELEMS / (size_t)std::max(N, D), (size_t)1 << 19) / 64 * 64;
+    return (int)std::min<size_t>((size_t)V, std::max<size_t>(rows, 64));
 }
-size_t fcl_inner_bytes(int rows, int D, int N) {
+size_t narrow_inner_bytes(int rows, int D, int N) {
     return al16b(std::max({mcn_gemm_workspace_bytes(rows, D, N, 0, 1), mcn_gemm_workspace_bytes(D, N, rows, 1, 0), mcn_add_sum_workspace_bytes(rows, N, 1)}));
 }
+size_t fcl_cost_bytes(int D, int V, int N) {
+    if (wide_cost_usable(N)) return wide_plan(D, V, N, false).total;
+    return al16b((size_t)narrow_tiles(V) * 3 * N * sizeof(float)) + al16b((size_t)N * sizeof(float));
+}
 size_t fcl_grad_bytes(int D, int V, int N) {
-    if (wide_usable(D, V, N)) return wide_plan(D, V, N, true).total;
-    const int rows = fcl_piece_rows(V, D, N), rest = V % rows;
-    return al16b((size_t)rows * N * sizeof(float)) + std::max(fcl_inner_bytes(rows, D, N), rest ? fcl_inner_bytes(rest, D, N) : 0);
+    if (wide_grad_usable(D, V, N)) return wide_plan(D, V, N, true).total;
+    const int rows = narrow_piece(V, D, N), rest = V % rows;
+    return al16b((size_t)rows * N * sizeof(float)) + std::max(narrow_inner_bytes(rows, D, N), rest ? narrow_inner_bytes(rest, D, N) : 0);
+}
+
+template <bool BWD>
+void launch_narrow(const NarrowArgs& p, hipStream_t s) {
+    const int groups = narrow_groups(p.vRows);
+    const dim3 grid(divup(p.vRows, 16 * groups)), block(256);
+#define NARROW_LAUNCH(NB)                                                                       \
+    if (groups == 1) MCN_LAUNCH((k_fcl_narrow<BWD, NB, 1>), grid, block, 0, s, p); \
+    else MCN_LAUNCH((k_fcl_narrow<BWD, NB, 4>), grid, block, 0, s, p)
+    switch (divup(p.N, 16)) {
+        case 1: NARROW_LAUNCH(1); break;
+        case 2: NARROW_LAUNCH(2); break;
+        case 3: NARROW_LAUNCH(3); break;
+        default: NARROW_LAUNCH(4); break;
+    }
+#undef NARROW_LAUNCH
 }
 
 int fcl_check(const char* what, const void* ws, size_t have, size_t need) {
@@ -1156,14 +1207,14 @@ MCN_API int mcn_fc_logreg_cost(const float* weights, const float* inputs, const 
     MCN_REQUIRE(fcl_sizes_ok(numInputs, numOutputs, numCases), "fcLogregCost: %d inputs, %d outputs, %d cases", numInputs, numOutputs, numCases);
     if (int rc = fcl_check("fcLogregCost", workspace, workspaceBytes, fcl_cost_bytes(numInputs, numOutputs, numCases))) return rc;
     hipStream_t s = (hipStream_t)stream;
-    if (wide_usable(numInputs, numOutputs, numCases)) {
+    if (wide_cost_usable(numCases)) {
         if (int rc = wide_cost(weights, inputs, biases, labels, caseStats, labelLogProbs, correctProbs, numInputs, numOutputs, numCases, (char*)workspace, s)) return rc;
     } else {
-        const int tiles = divup(numOutputs, BV);
-        FclArgs p = {weights, inputs, biases, labels, numInputs, numOutputs, numCases, 0, numOutputs, divup(numCases, BN)};
+        const int tiles = narrow_tiles(numOutputs);
+        NarrowArgs p = {weights, inputs, biases, labels, numInputs, numOutputs, numCases, 0, numOutputs};
         p.part = (float*)workspace;
         p.labelLogits = (float*)((char*)workspace + al16b((size_t)tiles * 3 * numCases * sizeof(float)));
-        MCN_LAUNCH(k_fcl_tile<false>, dim3(tiles * p.nTiles), dim3(256), 0, s, p);
+        launch_narrow<false>(p, s);
         MCN_LAUNCH(k_fcl_join, dim3(divup(numCases, 16)), dim3(1024), 0, s, p.part, p.labelLogits, labels, caseStats, labelLogProbs, correctProbs,
                    numOutputs, numCases, tiles);
     }
@@ -1181,20 +1232,20 @@ MCN_API int mcn_fc_logreg_grad(const float* weights, const float* inputs, const 
     MCN_REQUIRE(fcl_sizes_ok(numInputs, numOutputs, numCases), "fcLogregGrad: %d inputs, %d outputs, %d cases", numInputs, numOutputs, numCases);
     if (int rc = fcl_check("fcLogregGrad", workspace, workspaceBytes, fcl_grad_bytes(numInputs, numOutputs, numCases))) return rc;
     hipStream_t s = (hipStream_t)stream;
-    if (wide_usable(numInputs, numOutputs, numCases))
+    if (wide_grad_usable(numInputs, numOutputs, numCases))
         return wide_grad(weights, inputs, biases, labels, caseStats, inputGrads, weightGrads, biasGrads, numInputs, numOutputs, numCases, coeff,
                          scaleInputTargets, scaleWeightTargets, scaleWeightOutput, scaleBiasTargets, scaleBiasOutput, (char*)workspace, s);
-    const int D = numInputs, N = numCases, piece = fcl_piece_rows(numOutputs, D, N);
+    const int D = numInputs, N = numCases, piece = narrow_piece(numOutputs, D, N);
     float* dz = (float*)workspace;
     void* ws = (char*)workspace + al16b((size_t)piece * N * sizeof(float));
     const size_t wsBytes = workspaceBytes - al16b((size_t)piece * N * sizeof(float));
     for (int v0 = 0; v0 < numOutputs; v0 += piece) {
         const int rows = std::min(piece, numOutputs - v0);
-        FclArgs p = {weights, inputs, biases, labels, D, numOutputs, N, v0, rows, divup(N, BN)};
+        NarrowArgs p = {weights, inputs, biases, labels, D, numOutputs, N, v0, rows};
         p.stats = caseStats;
         p.dz = dz;
         p.coeff = coeff;
-        MCN_LAUNCH(k_fcl_tile<true>, dim3(divup(rows, BV) * p.nTiles), dim3(256), 0, s, p);
+        launch_narrow<true>(p, s);
         if (int rc = MCN_LAUNCH_CHECK("fcLogregGrad")) return rc;
         if (weightGrads)
             if (int rc = mcn_gemm(dz, inputs, weightGrads + (size_t)v0 * D, rows, D, N, 0, 1, scaleWeightOutput, scaleWeightTargets, ws, wsBytes, stream)) return rc;

@@ -48,8 +48,9 @@ def sum_err(k):
 
 
 def need(name, *a):
+    """A workspace full of NaNs: nothing may be read from it that was not written."""
     b = ws_bytes(name, *a)
-    return capi.DeviceBuffer(nbytes=max(b, 16)), b
+    return capi.DeviceBuffer(array=np.full(max(b, 16), 0xFF, np.uint8)), b
 
 
 # ------------------------------------------------------------------------------------------------------------- layer norm
@@ -352,7 +353,9 @@ def check_forward(ref, stats, logp, correct, what=''):
 # inputs, outputs, cases
 FCL_SHAPES = [(1, 1, 1), (1, 2, 3), (3, 1, 5), (16, 2, 1), (160, 4213, 1), (160, 4213, 2), (33, 65, 7), (64, 64, 64), (32, 128, 128),
               (160, 1000, 128), (512, 1999, 128), (100, 333, 129), (17, 4097, 33), (513, 130, 260), (1000, 257, 31), (2049, 96, 40),
-              (128, 640, 512), (96, 10575, 100), (256, 300, 1025)]
+              (128, 640, 512), (96, 10575, 100), (256, 300, 1025), (48, 20000, 17), (200, 70, 48), (96, 600, 63), (96, 600, 64),
+              (96, 600, 65), (1031, 8200, 20), (2050, 4200, 3), (40, 4400, 100),
+              (300, 5600, 130), (20, 70000, 70)]
 
 
 def fcl_run(w, x, b, lab, coeff=1.0, scales=(0.0, 0.0, 1.0, 0.0, 1.0), start=(None, None, None), stream=None):
