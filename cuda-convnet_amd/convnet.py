@@ -218,6 +218,7 @@ PRESETS = {  # name: (layer def, layer params, provider kind, image geometry)
     'deepid2': ('deepid2_10575.cfg', 'deepid_params.cfg', 'deepid2', (55, 55, 3)),
     'deepidn': ('deepidn_10575.cfg', 'deepidn_params.cfg', 'deepid2', (55, 55, 3)),  # DeepID2 + cost.fisher2 (deepidn/*.cfg)
     'deepid2plus': ('deepid2plus_10575.cfg', 'deepid_params.cfg', 'deepid2', (55, 55, 3)),
+    'deepid-head': ('deepid_4213_head.cfg', 'deepid_head_params.cfg', 'deepid', (55, 55, 3)),  # layer norm, dropout, classifier without logits
     'deepid-attr': ('deepid_attr_4131.cfg', 'deepid_attr_params.cfg', 'deepid_attr', (55, 55, 3)),
     'cifar10': ('cifar10.cfg', 'cifar10_params.cfg', 'cifar', (32, 32, 3)),
     'cifar10-cnorm': ('cifar10_cnorm.cfg', 'cifar10_params.cfg', 'cifar', (32, 32, 3)),

@@ -639,6 +639,143 @@ void FCLayer::bpropWeights(float* v, int i, PassType pt) {
                  _net->workspaceBytes(), _net->stream()), "fc bprop weights");
 }
 
+// ============================================================================ LayerNormLayer
+LayerNormLayer::LayerNormLayer(ConvNet* net, const Params& p) : WeightLayer(net, p, true, false) {
+    _eps = (float)pfloat(p, "eps");
+    if (_weights.size() != 1 || (long)_weights[0]->size() != _outputs || (long)_biases->size() != _outputs)
+        throw NetError("layer '" + _name + "': gains and biases must have one entry per input feature");
+    if (_actsTarget >= 0 || _actsGradTarget >= 0) throw NetError("layer '" + _name + "': a layer norm needs matrices of its own");
+}
+
+size_t LayerNormLayer::workspaceBytes(int maxCases) {
+    size_t b = mcn_add_sum_workspace_bytes(_outputs, maxCases, 1);
+    for (int n = 1; n <= maxCases; n++)  // (a short minibatch may take another form)
+        b = std::max({b, mcn_layer_norm_workspace_bytes(_outputs, n), mcn_layer_norm_undo_workspace_bytes(_outputs, n)});
+    return b;
+}
+
+void LayerNormLayer::allocate(int maxCases) {
+    Layer::allocate(maxCases);
+    _stats.ensure((size_t)2 * maxCases);
+}
+
+void LayerNormLayer::fpropActs(int, float, PassType) {
+    const int n = _net->numCases();
+    chk(mcn_layer_norm(_inputs[0], _weights[0]->W(), _biases->W(), _acts, _stats.p, _outputs, n, _eps, _net->workspace(), _net->workspaceBytes(),
+                       _net->stream()), "layer norm");
+    if (fusedNeuron)  // planned like behind any weight layer; this one applies it in place
+        chk(mcn_neuron_fwd(_acts, _acts, (size_t)_outputs * n, fusedNeuron->spec.type, fusedNeuron->spec.a, fusedNeuron->spec.b, _net->stream()),
+            "layer norm neuron");
+}
+
+void LayerNormLayer::bpropActs(float* v, int, float scaleTargets, PassType) {
+    chk(mcn_layer_norm_undo(v, _prev[0]->getActs(), _weights[0]->W(), _stats.p, _prev[0]->getActsGrad(), nullptr, nullptr, _outputs, _net->numCases(),
+                            scaleTargets, 1.f, 0.f, 0.f, 0.f, 0.f, _net->workspace(), _net->workspaceBytes(), _net->stream()), "layer norm undo");
+}
+
+void LayerNormLayer::bpropBiases(float* v, PassType pt) {
+    chk(mcn_add_sum(_biases->gradBuf(), v, _outputs, _net->numCases(), 1, 0.f, gradScale(_biases->eps(), pt), _net->workspace(),
+                    _net->workspaceBytes(), _net->stream()), "layer norm biases");
+}
+
+void LayerNormLayer::bpropWeights(float* v, int, PassType pt) {
+    Weights& w = *_weights[0];
+    chk(mcn_layer_norm_undo(v, _prev[0]->getActs(), w.W(), _stats.p, nullptr, w.getGrad(_net->dataParallel()), nullptr, _outputs, _net->numCases(),
+                            0.f, 0.f, w.numUpdates() > 0 ? 1.f : 0.f, gradScale(w.eps(), pt), 0.f, 0.f, _net->workspace(),
+                            _net->workspaceBytes(), _net->stream()), "layer norm gains");
+}
+
+// ============================================================================ DropoutLayer
+DropoutLayer::DropoutLayer(ConvNet* net, const Params& p) : Layer(net, p) {
+    _prob = (float)pfloat(p, "dropout");
+    _seed = (uint64_t)pint(p, "seed");
+    if (!(_prob >= 0.f && _prob < 1.f)) throw NetError("layer '" + _name + "': dropout must be in [0, 1)");
+}
+
+DropoutLayer::~DropoutLayer() {
+    if (_step) mcn_free(_step);
+}
+
+void DropoutLayer::allocate(int maxCases) {
+    Layer::allocate(maxCases);
+    if (_step) return;  // (a later, larger allocation goes on where the masks are)
+    void* q = nullptr;
+    chk(mcn_alloc(&q, sizeof(uint64_t)), "alloc");
+    _step = (uint64_t*)q;
+    chk(mcn_memset(_step, 0, sizeof(uint64_t), _net->mainStream()), "dropout step");
+}
+
+// every rank masks its own share of a minibatch by its own numbers
+uint64_t DropoutLayer::rankSeed() const { return _seed + 0x9E3779B97F4A7C15ull * (uint64_t)_net->rank(); }
+
+void DropoutLayer::fpropActs(int, float, PassType pt) {
+    const size_t n = (size_t)_outputs * _net->numCases();
+    if (pt == PASS_TEST) {
+        if (_acts != _inputs[0]) chk(mcn_scale(_inputs[0], _acts, n, 1.f, _net->stream()), "dropout (test)");
+        return;
+    }
+    if (pt == PASS_TRAIN) chk(mcn_counter_add(_step, 1, _net->stream()), "dropout step");  // (a gradient check keeps one mask)
+    chk(mcn_dropout(_inputs[0], _acts, n, _prob, rankSeed(), 0, _step, 0.f, 1.f, _net->stream()), "dropout");
+}
+
+void DropoutLayer::bpropActs(float* v, int, float scaleTargets, PassType) {
+    chk(mcn_dropout(v, _prev[0]->getActsGrad(), (size_t)_outputs * _net->numCases(), _prob, rankSeed(), 0, _step, scaleTargets, 1.f,
+                    _net->stream()), "dropout undo");
+}
+
+// ============================================================================ ClassifierLayer
+ClassifierLayer::ClassifierLayer(ConvNet* net, const Params& p) : WeightLayer(net, p, false, true) {
+    _wStep = 0.1f;  // as the fully connected layers, layer.cu:351-352
+    _bStep = 0.01f;
+    if (_weights.size() != 1 || _weights[0]->cols() != _outputs || (long)_biases->size() != _outputs)
+        throw NetError("layer '" + _name + "': a classifier layer has one (inputs, outputs) weight matrix and a bias per output");
+    if (_actsTarget >= 0 || _actsGradTarget >= 0) throw NetError("layer '" + _name + "': a classifier layer has no activities to share");
+}
+
+size_t ClassifierLayer::workspaceBytes(int maxCases) {
+    size_t b = 0;
+    for (int n = 1; n <= maxCases; n++)  // (a short minibatch may take another form)
+        b = std::max(b, mcn_fc_logreg_workspace_bytes(_prev[0]->outputs(), _outputs, n, 1));
+    return b;
+}
+
+void ClassifierLayer::allocate(int maxCases) { _ownActs.ensure(std::max<size_t>(actsElems(maxCases), 4)); }
+
+bool ClassifierLayer::planFusedTail(int) {  // the bias gradient arrives whole
+    _biases->partials = Weights::Partials();
+    return true;
+}
+
+void ClassifierLayer::fpropCost(float* labels, float* logProbs, float* correct, double* cost) {
+    chk(mcn_fc_logreg_cost(_weights[0]->W(), _inputs[0], _biases->W(), labels, _acts, logProbs, correct, _prev[0]->outputs(), _outputs,
+                           _net->numCases(), cost, _net->workspace(), _net->workspaceBytes(), _net->stream()), "classifier cost");
+}
+
+void ClassifierLayer::bpropCommon(float*, PassType pt) {
+    const bool last = _net->lastWeightLayerOfPass(this);
+    auto* cost = static_cast<CostLayer*>(_next[0]);
+    Weights& w = *_weights[0];
+    const bool dp = _net->dataParallel(), wantW = w.eps() > 0, wantB = _biases->eps() > 0, wantX = _prev[0]->isGradConsumer();
+    if (wantX) _prev[0]->awaitSeed();
+    // momentum as in FCLayer::bpropWeights
+    const float scaleW = dp ? (w.numUpdates() > 0 ? 1.f : 0.f) : ((w.numUpdates() == 0 && pt != PASS_GC) ? w.mom() : 0.f);
+    if (wantX || wantW || wantB) {
+        ProfScope ps(_net, _name, "bprop");
+        chk(mcn_fc_logreg_grad(w.W(), _prev[0]->getActs(), _biases->W(), cost->prev()[0]->getActs(), _acts, wantX ? _prev[0]->getActsGrad() : nullptr,
+                               wantW ? w.getGrad(dp) : nullptr, wantB ? _biases->gradBuf() : nullptr, _prev[0]->outputs(), _outputs, _net->numCases(),
+                               cost->coeff(), _prev[0]->rcvdB() > 0 ? 1.f : 0.f, scaleW, gradScale(w.eps(), pt), 0.f,
+                               gradScale(_biases->eps(), pt), _net->workspace(), _net->workspaceBytes(), _net->stream()), "classifier gradients");
+        if (wantW) w.incNumUpdates();
+    }
+    // what the other weight layers' pieces do beside their gradients (WeightLayer::bpropCommon)
+    const bool flushHere = _net->biasBatching() && _net->flushesBiasBatch(this, last);
+    if (last && pt == PASS_TRAIN && !flushHere) _net->earlyUpdate();
+    _net->deferSideWork([this, pt, flushHere] {
+        if (flushHere) _net->flushBiasSums();
+        if (_net->dataParallel() && pt == PASS_TRAIN) _net->gradReady(this);
+    }, last ? 1 : 2, last);
+}
+
 // ============================================================================ LocalLayer / ConvLayer / LocalUnsharedLayer
 LocalLayer::LocalLayer(ConvNet* net, const Params& p, bool useGrad, bool conv) : WeightLayer(net, p, useGrad, false), _conv(conv) {
     _padding = pintv(p, "padding");  // layer.cu:393-407
@@ -1197,10 +1334,16 @@ void CostLayer::allocate(int maxCases) {
     _aux.ensure(std::max<size_t>(maxCases, 4));
 }
 
-size_t LogregCostLayer::workspaceBytes(int maxCases) { return mcn_logreg_cost_workspace_bytes(_prev[1]->outputs(), maxCases); }
+size_t LogregCostLayer::workspaceBytes(int maxCases) {
+    return _prev[1]->type() == "classifier" ? 0 : mcn_logreg_cost_workspace_bytes(_prev[1]->outputs(), maxCases);
+}
 
 void LogregCostLayer::fpropActs(int i, float, PassType) {  // layer.cu:969-981
     if (i != 0) return;
+    if (_prev[1]->type() == "classifier") {  // no probabilities: the layer below finishes this cost from its own operands
+        static_cast<ClassifierLayer*>(_prev[1])->fpropCost(_inputs[0], _acts, _aux.p, dCost);
+        return;
+    }
     if (costDoneBySoftmax) {  // the softmax below left log p[label], hit flags and tie counts (this pass): one small block finishes
         costDoneBySoftmax = false;
         const int nc = _net->numCases();
@@ -1220,7 +1363,7 @@ void LogregCostLayer::fpropActs(int i, float, PassType) {  // layer.cu:969-981
 
 void LogregCostLayer::bpropActs(float*, int i, float scaleTargets, PassType) {  // layer.cu:983-994
     if (i != 1) throw NetError("logreg cost: gradient requested for the labels");
-    const bool doWork = _prev[1]->next().size() > 1 || _prev[1]->type() != "softmax";
+    const bool doWork = (_prev[1]->next().size() > 1 || _prev[1]->type() != "softmax") && _prev[1]->type() != "classifier";
     if (doWork)
         chk(mcn_logreg_grad(_prev[0]->getActs(), _prev[1]->getActs(), _prev[1]->getActsGrad(), _prev[1]->outputs(), _net->numCases(),
                             scaleTargets == 1 ? 1 : 0, _coeff, _net->stream()), "logreg grad");
@@ -1695,6 +1838,9 @@ ConvNet::ConvNet(const std::vector<Params>& layers, int minibatchSize, int devic
         else if (t == "cmrnorm") l = new ResponseNormLayer(this, p, true);
         else if (t == "cnorm") l = new ContrastNormLayer(this, p);
         else if (t == "softmax") l = new SoftmaxLayer(this, p);
+        else if (t == "layernorm") l = new LayerNormLayer(this, p);
+        else if (t == "dropout") l = new DropoutLayer(this, p);
+        else if (t == "classifier") l = new ClassifierLayer(this, p);
         else if (t == "eltsum") l = new EltwiseSumLayer(this, p);
         else if (t == "eltmax") l = new EltwiseMaxLayer(this, p);
         else if (t == "neuron") l = new NeuronLayer(this, p);
@@ -1720,6 +1866,10 @@ ConvNet::ConvNet(const std::vector<Params>& layers, int minibatchSize, int devic
     }
     for (auto& l : _layers)
         for (Layer* p : l->prev()) p->addNext(l.get());
+    for (auto& l : _layers)
+        if (l->type() == "classifier" && (l->prev().size() != 1 || l->next().size() != 1 || l->next()[0]->type() != "cost.logreg" ||
+                                          l->next()[0]->prev().size() != 2 || l->next()[0]->prev()[1] != l.get()))
+            throw NetError("layer '" + l->name() + "': a classifier layer has one input and feeds one cost.logreg, as its second input");
     _dp.reset(new DataProvider(this, minibatchSize));
 }
 

@@ -197,7 +197,7 @@ class WeightLayer : public Layer {
     void weightsUpdated() override;
     void resetUpdateCounters() override;
     bool sharesWeights() const;  // holds a matrix that another Weights object owns
-    bool queuesBiasSum(bool fusedTail) const { return _biases->eps() > 0 && !(_biasInWgrad && fusedTail); }
+    virtual bool queuesBiasSum(bool fusedTail) const { return _biases->eps() > 0 && !(_biasInWgrad && fusedTail); }
     void copyToCPU() override;
     void copyToGPU() override;
     void checkGradients(std::vector<GradCheckResult>& out, long maxElems, bool central) override;
@@ -238,6 +238,56 @@ class FCLayer : public WeightLayer {
     void bpropWeights(float* v, int, PassType) override;
     bool _fwdAllDone = false, _wgradAllDone = false;
     std::vector<char> _bwdDone;
+};
+
+// Layer norm over all features of a case (mcn_layer_norm): the gains are the layer's one weight matrix, numInputs x 1.
+class LayerNormLayer : public WeightLayer {
+   public:
+    LayerNormLayer(ConvNet* net, const Params& p);
+    size_t workspaceBytes(int maxCases) override;
+    void allocate(int maxCases) override;
+   protected:
+    void fpropActs(int, float, PassType) override;
+    void bpropActs(float* v, int, float, PassType) override;
+    void bpropBiases(float* v, PassType) override;
+    void biasSumShape(int numCases, int& rows, int& cols) const override { rows = _outputs; cols = numCases; }
+    void bpropWeights(float* v, int, PassType) override;
+    float _eps;
+    DBuf _stats;
+};
+
+// Dropout (mcn_dropout): training draws a new mask every minibatch from (seed, step), the backward pass draws it again; a test
+// pass copies.  The step lives in device memory, so that a replayed step graph draws new masks too.
+class DropoutLayer : public Layer {
+   public:
+    DropoutLayer(ConvNet* net, const Params& p);
+    ~DropoutLayer() override;
+    void allocate(int maxCases) override;
+   protected:
+    void fpropActs(int, float, PassType) override;
+    void bpropActs(float* v, int, float, PassType) override;
+    uint64_t rankSeed() const;
+    float _prob;
+    uint64_t _seed;
+    uint64_t* _step = nullptr;
+};
+
+// The classifier layer of many classes: fully connected + softmax under a cost.logreg, without the matrix of logits
+// (mcn_fc_logreg_cost / _grad).  It has no activities to read; the cost layer on top calls it.
+class ClassifierLayer : public WeightLayer {
+   public:
+    ClassifierLayer(ConvNet* net, const Params& p);
+    size_t workspaceBytes(int maxCases) override;
+    void allocate(int maxCases) override;
+    bool planFusedTail(int numCases) override;
+    bool queuesBiasSum(bool) const override { return false; }
+    size_t actsElems(int n) const override { return (size_t)2 * n; }  // the case statistics stand where activities would
+    void fpropCost(float* labels, float* logProbs, float* correct, double* cost);
+   protected:
+    void bpropCommon(float* v, PassType pt) override;  // all three gradients, on the main stream (they share the pieces of dz)
+    void bpropBiases(float*, PassType) override {}
+    void biasSumShape(int numCases, int& rows, int& cols) const override { rows = _outputs; cols = numCases; }
+    void bpropWeights(float*, int, PassType) override {}
 };
 
 class LocalLayer : public WeightLayer {

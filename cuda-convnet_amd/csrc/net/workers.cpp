@@ -196,6 +196,7 @@ void ConvNet::runLoad(const CPUData& data) {
 // FeatureWorker::run (worker.cu:191-214): ftrs is (numCases, numFeatures) row-major on the host
 void ConvNet::runFeatures(const CPUData& data, HostMat ftrs, int layerIdx) {
     if (layerIdx < 0 || layerIdx >= numLayers()) throw NetError("feature writer: bad layer index");
+    if (layer(layerIdx).type() == "classifier") throw NetError("feature writer: a classifier layer keeps no outputs (use fc and softmax layers)");
     _dp->setData(data);
     Layer& fl = layer(layerIdx);
     const long F = fl.outputs();
@@ -222,6 +223,8 @@ void ConvNet::runMultiview(const CPUData& data, int numViews, int logregIdx) {
     if (numViews <= 0 || data.numCases() % numViews != 0) throw NetError("multiview test: numCases not divisible by numViews");
     if (logregIdx < 0 || logregIdx >= numLayers() || layer(logregIdx).type() != "cost.logreg")
         throw NetError("multiview test: logregIdx does not name a cost.logreg layer");
+    if (layer(logregIdx).prev()[1]->type() == "classifier")
+        throw NetError("multiview test: a classifier layer keeps no probabilities to average (use fc and softmax layers)");
     _dp->setData(data);
     Layer& logreg = layer(logregIdx);
     const long real = _dp->numCases() / numViews;

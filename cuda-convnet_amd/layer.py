@@ -302,6 +302,57 @@ def _parse_softmax(name, cfg, prev, ctx):
     return dic
 
 
+def _parse_layernorm(name, cfg, prev, ctx):
+    """type=layernorm: each case normalised over all its features, then gains and biases per feature (no counterpart in the
+    reference).  eps is added to the variance; initW / initB are the gains' and biases' first values (1 and 0)."""
+    dic = _with_inputs(name, cfg, prev, 1)
+    _parse_weight_common(dic, name, cfg, prev)
+    dic['usesActs'] = False
+    n = dic['outputs'] = dic['numInputs'][0]
+    dic['eps'] = cfg.get_float(name, 'eps', default=1e-5)
+    _check(dic['eps'] > 0, "Layer '%s': parameter 'eps' must be positive" % name)
+    _check(dic['weightSource'] == [''], "Layer '%s': layers of type 'layernorm' do not share weights" % name)
+    gain = cfg.get_float(name, 'initW', default=1.0)
+    dic['initW'] = [gain]
+    dic['weights'] = [np.full((n, 1), gain, dtype=np.float32)]
+    dic['weightsInc'] = [np.zeros_like(dic['weights'][0])]
+    _make_biases(dic, n, 1, 'C')
+    if prev[dic['inputs'][0]].get('geom'):
+        dic['geom'] = prev[dic['inputs'][0]]['geom']
+    return dic
+
+
+def _parse_dropout(name, cfg, prev, ctx):
+    """type=dropout: dropout=p, and optionally seed=k (else drawn with the net's other random numbers).  The `dropout` key that the
+    DeepID definitions carry on an fc layer stays without effect, as in the reference; this layer is what acts on it."""
+    dic = _with_inputs(name, cfg, prev, 1)
+    dic['outputs'] = dic['numInputs'][0]
+    dic['dropout'] = cfg.get_float(name, 'dropout')
+    _check(0 <= dic['dropout'] < 1, "Layer '%s': parameter 'dropout' must be in [0, 1)" % name)
+    seed = cfg.get_int(name, 'seed', default=-1)
+    dic['seed'] = int(ctx.rng.integers(1 << 62)) if seed < 0 else seed
+    dic['usesActs'] = dic['usesInputs'] = False
+    dic['forceOwnActs'] = prev[dic['inputs'][0]]['type'] == 'data'  # never in the data batch itself
+    if prev[dic['inputs'][0]].get('geom'):
+        dic['geom'] = prev[dic['inputs'][0]]['geom']
+    return dic
+
+
+def _parse_classifier(name, cfg, prev, ctx):
+    """type=classifier: a fully connected layer and the softmax above it for many classes, without the matrix of logits.  Its only
+    consumer is a cost.logreg; parameters as for type=fc."""
+    dic = _with_inputs(name, cfg, prev, 1)
+    _parse_weight_common(dic, name, cfg, prev)
+    dic['outputs'] = cfg.get_int(name, 'outputs')
+    _check(1 <= dic['outputs'] <= 1 << 24, "Layer '%s': parameter 'outputs' out of range" % name)
+    _check(dic['neuron'] in ('', 'ident'), "Layer '%s': layers of type 'classifier' take no neuron" % name)
+    _check(dic['weightSource'] == [''], "Layer '%s': layers of type 'classifier' do not share weights" % name)
+    dic['neuron'] = ''
+    _make_weights(dic, prev, ctx, dic['numInputs'], [dic['outputs']], 'F')
+    _make_biases(dic, 1, dic['outputs'], 'F')
+    return dic
+
+
 def _parse_neuron_layer(name, cfg, prev, ctx, neuron_str=None):
     dic = _with_inputs(name, cfg, prev, 1)
     dic['outputs'] = dic['numInputs'][0]
@@ -500,7 +551,7 @@ def _parse_cost(name, cfg, prev, ctx, num_inputs):
     if t in ('cost.logreg', 'cost.l2-sn', 'cost.fisher2'):
         _check(dic['numInputs'][0] == 1, "Layer '%s': dimensionality of first input must be 1" % name)
     if t == 'cost.logreg':
-        _check(prev[dic['inputs'][1]]['type'] == 'softmax', "Layer '%s': second input must be softmax layer" % name)
+        _check(prev[dic['inputs'][1]]['type'] in ('softmax', 'classifier'), "Layer '%s': second input must be softmax layer" % name)
         if ctx.num_classes:
             _check(dic['numInputs'][1] == ctx.num_classes,
                    "Layer '%s': softmax input '%s' must produce %d outputs, because that is the number of classes in the dataset"
@@ -518,6 +569,9 @@ PARSERS = {
     'conv': lambda n, c, p, x: _parse_local(n, c, p, x, True),
     'local': lambda n, c, p, x: _parse_local(n, c, p, x, False),
     'softmax': _parse_softmax,
+    'layernorm': _parse_layernorm,
+    'dropout': _parse_dropout,
+    'classifier': _parse_classifier,
     'eltsum': _parse_eltsum,
     'eltmax': _parse_eltmax,
     'neuron': _parse_neuron_layer,
@@ -595,7 +649,7 @@ def _add_params(dic, pcfg):
     """Hyper-parameters from the layer-params file (WeightLayerParser.add_params
     layer.py:641-651, NormLayerParser.add_params :1033-1037, CostParser.add_params :1079-1081)."""
     name, t = dic['name'], dic['type']
-    if t in ('fc', 'conv', 'local'):
+    if t in ('fc', 'conv', 'local', 'layernorm', 'classifier'):
         dic['epsW'] = pcfg.get_list(name, 'epsW', float, 'floats')
         dic['epsB'] = pcfg.get_float(name, 'epsB')
         dic['momW'] = pcfg.get_list(name, 'momW', float, 'floats')
@@ -637,6 +691,10 @@ def parse_layers(layer_cfg_path, param_cfg_path, data_dims, num_classes=0, seed=
             if not l['type'].startswith('cost.'):
                 used = any(i in l2['inputs'] for l2 in layers if 'inputs' in l2)
                 _check(used, "Layer '%s' of type '%s' is unused" % (l['name'], l['type']))
+            if l['type'] == 'classifier':
+                users = [l2 for l2 in layers if i in l2.get('inputs', [])]
+                _check([u['type'] for u in users] == ['cost.logreg'] and users[0]['inputs'][1] == i and users[0]['inputs'][0] != i,
+                       "Layer '%s': a layer of type 'classifier' feeds one cost.logreg and nothing else" % l['name'])
     pcfg = Cfg(param_cfg_path)
     for l in layers:
         _check(pcfg.has(l['name']) or not l['requiresParams'],
