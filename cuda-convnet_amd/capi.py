@@ -61,15 +61,16 @@ class Lib:
             fn = getattr(self.dll, name)  # AttributeError if the symbol is not exported
             fn.restype = {'int': C.c_int, 'size_t': C.c_size_t, 'uint64_t': C.c_uint64, 'const char*': C.c_char_p}[ret]
             fn.argtypes = [_CTYPES[t] for t, _ in args]
+        self._entries = {name: (getattr(self.dll, name), ret == 'int') for name, (ret, _) in self.protos.items()}
 
     def raw(self, name):
         return getattr(self.dll, name)
 
     def call(self, name, *args):
         """Call an int-returning entry point; raise McnError on a non-zero status."""
-        conv = [a.ptr if isinstance(a, DeviceBuffer) else a for a in args]
-        rc = getattr(self.dll, name)(*conv)
-        if self.protos[name][0] == 'int' and rc != 0:
+        fn, status = self._entries[name]  # (looked up once: a small launch takes no longer than this function did)
+        rc = fn(*args)
+        if rc != 0 and status:
             raise McnError('%s failed (%d): %s' % (name, rc, self.dll.mcn_last_error().decode()))
         return rc
 
@@ -121,6 +122,10 @@ class DeviceBuffer:
 
     def zero(self):
         lib().call('mcn_memset', self.ptr, 0, self.nbytes, None)
+
+    @property
+    def _as_parameter_(self):  # what ctypes passes for a buffer
+        return self.ptr
 
     def offset(self, nbytes):
         return self.ptr + nbytes
