@@ -154,21 +154,62 @@ __global__ __launch_bounds__(T_WHOLE) void k_ln_whole(const float* x, const floa
     }
 }
 
+// ---- gains' and biases' gradients of a small matrix, by blocks of their own in the same launch: groups of 1 << logLanes lanes take a
+// row each and read it from the caches the other blocks fill.  (Partial sums per tile of columns, and a launch that joins them, for the
+// larger ones: reading those twice would cost more.)
+struct RowSums {
+    float *gainGrad, *biasGrad;
+    float gainTargets, gainOutput, biasTargets, biasOutput;
+    int first;     // first block of this kind
+    int logLanes;
+};
+__device__ __forceinline__ void row_sums_block(const float* g, const float* x, const float* __restrict__ caseStats, int F, int N, const RowSums& q) {
+    const int lanes = 1 << q.logLanes, l = threadIdx.x & (lanes - 1);
+    const int r = (blockIdx.x - q.first) * (T_WHOLE >> q.logLanes) + (threadIdx.x >> q.logLanes);
+    float sg = 0.f, sb = 0.f;
+    if (r < F) {
+        const float *gp = g + (size_t)r * N, *xp = x + (size_t)r * N;
+#pragma unroll 4
+        for (int c = l * 4; c < N; c += lanes * 4) {
+            const int cnt = min(4, N - c);
+            const Cols<4> gv = load_cols<4>(gp + c, cnt), xv = load_cols<4>(xp + c, cnt), mu = load_cols<4>(caseStats + c, cnt),
+                          rs = load_cols<4>(caseStats + N + c, cnt);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                sg += gv.v[j] * ((xv.v[j] - mu.v[j]) * rs.v[j]);
+                sb += gv.v[j];
+            }
+        }
+    }
+    for (int o = lanes >> 1; o > 0; o >>= 1) {
+        sg += __shfl_xor(sg, o, 64);
+        sb += __shfl_xor(sb, o, 64);
+    }
+    if (l == 0 && r < F) {
+        if (q.gainGrad) q.gainGrad[r] = (q.gainTargets != 0.f ? q.gainTargets * q.gainGrad[r] : 0.f) + q.gainOutput * sg;
+        if (q.biasGrad) q.biasGrad[r] = (q.biasTargets != 0.f ? q.biasTargets * q.biasGrad[r] : 0.f) + q.biasOutput * sb;
+    }
+}
+
 // ---- backward, the same way: both matrices in registers.  A block goes through its tiles one after the other with its rows fixed, so
 // the row sums for gains and biases stay in registers too and leave once per block: rowPart[block][2][F].
 template <int VW, int R>
 __global__ __launch_bounds__(T_WHOLE) void k_ln_undo_whole(const float* g, const float* x, const float* __restrict__ gain,
                                                      const float* __restrict__ caseStats, float* target, float* __restrict__ rowPart,
-                                                     float scaleTargets, float scaleOutput, int F, int N, int logLanes, int tiles) {
+                                                     float scaleTargets, float scaleOutput, int F, int N, int logLanes, int tiles, RowSums q) {
+    if ((int)blockIdx.x >= q.first) {
+        row_sums_block(g, x, caseStats, F, N, q);
+        return;
+    }
     constexpr int T = T_WHOLE;
     __shared__ float sh[T / 64][64][2 * VW];
     int grp, sub;
-    mcn_xcd_group(blockIdx.x, 8, gridDim.x / 8, grp, sub);  // (the grid is a multiple of eight)
+    mcn_xcd_group(blockIdx.x, 8, q.first / 8, grp, sub);  // (the blocks of this kind are a multiple of eight)
     const int block = grp * 8 + sub, rowLanes = T >> logLanes, rl = threadIdx.x >> logLanes;
     float sg[R] = {}, sb[R] = {};
     const float invF = 1.f / (float)F;
     const size_t step = (size_t)rowLanes * N;
-    for (int tile = block; tile < tiles; tile += gridDim.x) {
+    for (int tile = block; tile < tiles; tile += q.first) {
         const Place<VW, T> p(tile, logLanes, N);
         const size_t first = (size_t)rl * N + p.col;
         Cols<VW> gv[R], xv[R];
@@ -366,10 +407,15 @@ __global__ __launch_bounds__(T_SPLIT) void k_ln_split_apply(const float* x, cons
 template <int VW>
 __global__ __launch_bounds__(T_SPLIT) void k_ln_undo_split_sums(const float* __restrict__ g, const float* __restrict__ x,
                                                                 const float* __restrict__ gain, const float* __restrict__ caseStats,
-                                                                float* __restrict__ colPart, float* __restrict__ rowPart, Split s) {
+                                                                float* __restrict__ colPart, float* __restrict__ rowPart, Split s, RowSums q) {
+    if ((int)blockIdx.x >= q.first) {
+        row_sums_block(g, x, caseStats, s.F, s.N, q);
+        return;
+    }
     __shared__ float sh[T_SPLIT / 64][64][2 * VW];
-    const Place<VW, T_SPLIT> p(blockIdx.x, s.logLanes, s.N);
-    const int r0 = blockIdx.y * s.rowsPerSplit, r1 = min(s.F, r0 + s.rowsPerSplit);
+    const int tile = blockIdx.x % s.colTiles, split = blockIdx.x / s.colTiles;
+    const Place<VW, T_SPLIT> p(tile, s.logLanes, s.N);
+    const int r0 = split * s.rowsPerSplit, r1 = min(s.F, r0 + s.rowsPerSplit);
     const Cols<VW> mu = load_cols<VW>(caseStats + p.col, p.cnt), rs = load_cols<VW>(caseStats + s.N + p.col, p.cnt);
     float v[2 * VW] = {};
     const int steps = (max(r1 - r0, 0) + p.rowLanes - 1) / p.rowLanes;  // the same for every lane: the shuffles below need whole groups
@@ -395,7 +441,7 @@ __global__ __launch_bounds__(T_SPLIT) void k_ln_undo_split_sums(const float* __r
                 sb += __shfl_xor(sb, o, 64);
             }
             if (p.cl == 0 && r < r1) {
-                float* out = rowPart + (size_t)blockIdx.x * 2 * s.F + r;
+                float* out = rowPart + (size_t)tile * 2 * s.F + r;
                 out[0] = sg;
                 out[s.F] = sb;
             }
@@ -406,7 +452,7 @@ __global__ __launch_bounds__(T_SPLIT) void k_ln_undo_split_sums(const float* __r
         Cols<VW> a, b;
 #pragma unroll
         for (int j = 0; j < VW; j++) { a.v[j] = v[j]; b.v[j] = v[VW + j]; }
-        float* out = colPart + (size_t)blockIdx.y * 2 * s.N + p.col;
+        float* out = colPart + (size_t)split * 2 * s.N + p.col;
         store_cols<VW>(out, a, p.cnt);
         store_cols<VW>(out + s.N, b, p.cnt);
     }
@@ -505,6 +551,7 @@ struct Plan {
     int blocks;               // backward, whole
     Split split;
 };
+constexpr size_t SMALL_BYTES = (size_t)32 << 20;  // both matrices of a backward pass: the rows are summed by blocks of their own
 constexpr int FWD_ROWS = 16, BWD_ROWS = 8;       // rows a thread of the whole kernels holds
 // rows: FWD_ROWS or BWD_ROWS
 Plan ln_plan(int F, int N, int rows) {
@@ -588,7 +635,7 @@ MCN_API int mcn_layer_norm(const float* inputs, const float* gains, const float*
 MCN_API size_t mcn_layer_norm_undo_workspace_bytes(int numFeatures, int numCases) {
     if (!ln_sizes_ok(numFeatures, numCases)) return 0;
     const Plan p = ln_plan(numFeatures, numCases, BWD_ROWS);
-    const size_t parts = p.whole ? p.blocks : p.split.colTiles;
+    const size_t parts = p.whole ? p.blocks : p.split.colTiles;  // (of a small matrix the row sums need none: kept simple)
     return (parts * 2 * numFeatures + (p.whole ? 0 : (size_t)p.split.splits * 2 * numCases)) * sizeof(float);
 }
 
@@ -603,13 +650,19 @@ MCN_API int mcn_layer_norm_undo(const float* outGrads, const float* inputs, cons
     hipStream_t st = (hipStream_t)stream;
     const int F = numFeatures, N = numCases;
     const Plan p = ln_plan(F, N, BWD_ROWS);
-    const bool rows = gainGrads || biasGrads;
-    float* rowPart = rows ? (float*)workspace : nullptr;
+    const bool rows = gainGrads || biasGrads, small = (size_t)F * N * 8 <= SMALL_BYTES;
+    float* rowPart = rows && !small ? (float*)workspace : nullptr;
+    const Split& sp = p.split;
+    RowSums q = {gainGrads, biasGrads, scaleGainTargets, scaleGainOutput, scaleBiasTargets, scaleBiasOutput, 0, 0};
+    while (q.logLanes < 6 && (4 << q.logLanes) < N) q.logLanes++;
+    const int rowBlocks = rows && small ? divup(F, T_WHOLE >> q.logLanes) : 0;
     int parts;
     if (p.whole) {
         parts = p.blocks;
-#define WHOLE(VW, R) MCN_LAUNCH((k_ln_undo_whole<VW, R>), dim3(p.blocks), dim3(T_WHOLE), 0, st, outGrads, inputs, gains, caseStats, target, \
-                                rowPart, scaleTargets, scaleOutput, F, N, p.logLanes, p.tiles)
+        q.first = target || rowPart ? p.blocks : 0;
+        const dim3 grid(q.first + rowBlocks);
+#define WHOLE(VW, R) MCN_LAUNCH((k_ln_undo_whole<VW, R>), grid, dim3(T_WHOLE), 0, st, outGrads, inputs, gains, caseStats, target, \
+                                rowPart, scaleTargets, scaleOutput, F, N, p.logLanes, p.tiles, q)
         const bool few = ((size_t)F << p.logLanes) <= T_WHOLE * 2;
         if (p.vw == 4 && few) WHOLE(4, 2);
         else if (p.vw == 4) WHOLE(4, BWD_ROWS);
@@ -617,19 +670,19 @@ MCN_API int mcn_layer_norm_undo(const float* outGrads, const float* inputs, cons
         else WHOLE(1, BWD_ROWS);
 #undef WHOLE
     } else {
-        const Split& s = p.split;
-        const dim3 grid(s.colTiles, s.splits);
-        parts = s.colTiles;
+        parts = sp.colTiles;
+        q.first = target || rowPart ? sp.colTiles * sp.splits : 0;
+        const dim3 sums(q.first + rowBlocks), grid(sp.colTiles, sp.splits);
         float* colPart = (float*)workspace + (size_t)parts * 2 * F;
         if (p.vw == 4) {
-            MCN_LAUNCH(k_ln_undo_split_sums<4>, grid, dim3(T_SPLIT), 0, st, outGrads, inputs, gains, caseStats, colPart, rowPart, s);
-            if (target) MCN_LAUNCH(k_ln_undo_split_apply<4>, grid, dim3(T_SPLIT), 0, st, outGrads, inputs, gains, caseStats, colPart, target, scaleTargets, scaleOutput, s);
+            MCN_LAUNCH(k_ln_undo_split_sums<4>, sums, dim3(T_SPLIT), 0, st, outGrads, inputs, gains, caseStats, colPart, rowPart, sp, q);
+            if (target) MCN_LAUNCH(k_ln_undo_split_apply<4>, grid, dim3(T_SPLIT), 0, st, outGrads, inputs, gains, caseStats, colPart, target, scaleTargets, scaleOutput, sp);
         } else {
-            MCN_LAUNCH(k_ln_undo_split_sums<1>, grid, dim3(T_SPLIT), 0, st, outGrads, inputs, gains, caseStats, colPart, rowPart, s);
-            if (target) MCN_LAUNCH(k_ln_undo_split_apply<1>, grid, dim3(T_SPLIT), 0, st, outGrads, inputs, gains, caseStats, colPart, target, scaleTargets, scaleOutput, s);
+            MCN_LAUNCH(k_ln_undo_split_sums<1>, sums, dim3(T_SPLIT), 0, st, outGrads, inputs, gains, caseStats, colPart, rowPart, sp, q);
+            if (target) MCN_LAUNCH(k_ln_undo_split_apply<1>, grid, dim3(T_SPLIT), 0, st, outGrads, inputs, gains, caseStats, colPart, target, scaleTargets, scaleOutput, sp);
         }
     }
-    if (rows)
+    if (rowPart)
         MCN_LAUNCH(k_ln_undo_rows, dim3((unsigned)divup_sz((size_t)2 * F, 32)), dim3(512), 0, st, rowPart, gainGrads, biasGrads, scaleGainTargets,
                    scaleGainOutput, scaleBiasTargets, scaleBiasOutput, F, parts);
     return MCN_LAUNCH_CHECK("layerNormUndo");
