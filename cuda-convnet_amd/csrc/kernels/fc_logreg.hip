@@ -532,85 +532,91 @@ __device__ __forceinline__ void product_tile_shared(const char* A, size_t aRow, 
 }
 
 // ---- packing
-// Fragments of x (D, N).  The first caseBlocks blocks take 16 cases each: (rows = cases, k = features) for the logits; the others 16
-// features each: (rows = features, k = cases) for the weight gradient, in which a case without a label is zero, whatever it holds.
+// What a pack launch makes, 512 threads a block: blocks below caseBlocks, 16 cases of x each (rows = cases, k = features) for the logits;
+// the next featBlocks, 16 features of x each (rows = features, k = cases) for the weight gradient, in which a case without a label is
+// zero, whatever it holds; the others, 32 classes of the piece each (rows = classes, k = features).
+struct PackArgs {
+    const float *X, *labels;
+    int *caseExp, *featExp;
+    char *xByCase, *xByFeat;
+    int D, V, N, Kd, Kn, caseBlocks, featBlocks;
+    const float *W, *bias;  // of the piece
+    int* classExp;
+    char* wByClass;
+    int rows;
+};
+
 // Each block finds its rows' largest magnitudes first; what it reads then comes from its caches.
-__global__ __launch_bounds__(512) void k_fcl_pack_x(const float* __restrict__ X, const float* __restrict__ labels, int* __restrict__ caseExp,
-                                                    int* __restrict__ featExp, char* __restrict__ byCase, char* __restrict__ byFeat, int D,
-                                                    int V, int N, int Kd, int Kn, int caseBlocks) {
-    __shared__ float sh[8][16];
-    __shared__ int exps[16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+__device__ __forceinline__ void pack_cases(const PackArgs& p, int block, float* sh, int* exps) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4, n = block * 16 + c;
     float m = 0.f;
-    if ((int)blockIdx.x < caseBlocks) {
-        const int n = blockIdx.x * 16 + c;
-        if (n < N) {
+    if (n < p.N) {
 #pragma unroll 8
-            for (int d = threadIdx.x >> 4; d < D; d += 32) m = max_or_nan(m, fabsf(X[(size_t)d * N + n]));
-        }
-        m = max_or_nan(m, __shfl_xor(m, 16, 64));
-        m = max_or_nan(m, __shfl_xor(m, 32, 64));
-        sh[wave][c] = m;
-        __syncthreads();
-        if (threadIdx.x < 16) {
-            for (int w = 1; w < 8; w++) m = max_or_nan(m, sh[w][c]);
-            caseExp[n] = exps[c] = scale_exp(m);
-        }
-        __syncthreads();
-        const int e = exps[c];
-        for (int kb = wave; kb < Kd; kb += 8) {
-            float y[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int d = kb * 32 + (j >> 2) * 16 + g * 4 + (j & 3);
-                y[j] = n < N && d < D ? ldexpf(X[(size_t)d * N + n], e) : 0.f;
-            }
-            store_pair(byCase + ((size_t)blockIdx.x * Kd + kb) * PAIR, lane, y);
-        }
-        return;
+        for (int d = threadIdx.x >> 4; d < p.D; d += 32) m = max_or_nan(m, fabsf(p.X[(size_t)d * p.N + n]));
     }
-    const int d0 = (blockIdx.x - caseBlocks) * 16, r = threadIdx.x >> 5;
-    if (d0 + r < D) {
+    m = max_or_nan(m, __shfl_xor(m, 16, 64));
+    m = max_or_nan(m, __shfl_xor(m, 32, 64));
+    sh[wave * 16 + c] = m;
+    __syncthreads();
+    if (threadIdx.x < 16) {
+        for (int w = 1; w < 8; w++) m = max_or_nan(m, sh[w * 16 + c]);
+        p.caseExp[n] = exps[c] = scale_exp(m);
+    }
+    __syncthreads();
+    const int e = exps[c];
+    for (int kb = wave; kb < p.Kd; kb += 8) {
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int d = kb * 32 + (j >> 2) * 16 + g * 4 + (j & 3);
+            y[j] = n < p.N && d < p.D ? ldexpf(p.X[(size_t)d * p.N + n], e) : 0.f;
+        }
+        store_pair(p.xByCase + ((size_t)block * p.Kd + kb) * PAIR, lane, y);
+    }
+}
+
+__device__ __forceinline__ void pack_feats(const PackArgs& p, int block, int* exps) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4, d0 = block * 16, r = threadIdx.x >> 5;
+    float m = 0.f;
+    if (d0 + r < p.D) {
 #pragma unroll 4
-        for (int n = threadIdx.x & 31; n < N; n += 32) {
+        for (int n = threadIdx.x & 31; n < p.N; n += 32) {
             int label;
-            const bool counts = label_of(labels[n], V, label);
-            const float v = fabsf(X[(size_t)(d0 + r) * N + n]);
+            const bool counts = label_of(p.labels[n], p.V, label);
+            const float v = fabsf(p.X[(size_t)(d0 + r) * p.N + n]);
             m = counts ? max_or_nan(m, v) : m;
         }
     }
     for (int o = 1; o < 32; o <<= 1) m = max_or_nan(m, __shfl_xor(m, o, 64));
-    if ((threadIdx.x & 31) == 0) featExp[d0 + r] = exps[r] = scale_exp(m);
+    if ((threadIdx.x & 31) == 0) p.featExp[d0 + r] = exps[r] = scale_exp(m);
     __syncthreads();
     const int d = d0 + c, e = exps[c];
-    for (int kb = wave; kb < Kn; kb += 8) {
+    for (int kb = wave; kb < p.Kn; kb += 8) {
         float y[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int n = kb * 32 + (j >> 2) * 16 + g * 4 + (j & 3);
             int label;
-            y[j] = d < D && n < N && label_of(labels[n], V, label) ? ldexpf(X[(size_t)d * N + n], e) : 0.f;
+            y[j] = d < p.D && n < p.N && label_of(p.labels[n], p.V, label) ? ldexpf(p.X[(size_t)d * p.N + n], e) : 0.f;
         }
-        store_pair(byFeat + ((size_t)(d0 / 16) * Kn + kb) * PAIR, lane, y);
+        store_pair(p.xByFeat + ((size_t)block * p.Kn + kb) * PAIR, lane, y);
     }
 }
 
-// Fragments of a piece of W (rows = classes, k = features), 32 classes per block with one scale, a power of 2^8: its largest magnitude
-// comes to [2^7, 2^15), and neighbouring groups mostly share it (k_fcl_igrad).  A class that a bias of -inf takes out is zero, whatever
-// its weights hold.  512 features at a time go through registers (all of a thread's loads in flight at once) and LDS; rows of at most
-// 512 features are read once, longer ones a second time for their max.
+// 32 classes with one scale, a power of 2^8: their largest magnitude comes to [2^7, 2^15), and neighbouring groups mostly share it
+// (CarryScale).  A class that a bias of -inf takes out is zero, whatever its weights hold.  512 features at a time go through registers
+// (all of a thread's loads in flight at once) and LDS; rows of at most 512 features are read once, longer ones a second time for their
+// max.
 constexpr int CW = 512, CW_LD = CW + 4;
 constexpr int PACK_LDS = (32 * CW_LD + 8) * 4;
-__global__ __launch_bounds__(512) void k_fcl_pack_w(const float* __restrict__ W, const float* __restrict__ bias, int* __restrict__ classExp,
-                                                    char* __restrict__ byClass, int D, int rows, int Kd) {
-    extern __shared__ __attribute__((aligned(16))) float tile[];  // [32][CW_LD], then the waves' maxima
+__device__ __forceinline__ void pack_classes(const PackArgs& p, int block, float* tile) {
     float* maxima = tile + 32 * CW_LD;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, v0 = blockIdx.x * 32, c = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, v0 = block * 32, c = lane & 15, g = lane >> 4, D = p.D;
     bool live[4];
 #pragma unroll
     for (int r = 0; r < 4; r++) {
         const int v = v0 + wave * 4 + r;
-        live[r] = v < rows && (!bias || bias[v] != -INFINITY);
+        live[r] = v < p.rows && (!p.bias || p.bias[v] != -INFINITY);
     }
     f32x4 t[4][2];
     auto load = [&](int d0) {  // a wave: rows 4 wave .. + 3, a lane: features d0 + 4 lane .. and 256 further on
@@ -619,7 +625,7 @@ __global__ __launch_bounds__(512) void k_fcl_pack_w(const float* __restrict__ W,
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const int d = d0 + h * 256 + lane * 4;
-                const float* src = W + (size_t)(v0 + wave * 4 + r) * D + d;
+                const float* src = p.W + (size_t)(v0 + wave * 4 + r) * D + d;
                 f32x4 x = {0.f, 0.f, 0.f, 0.f};
                 if (live[r]) {
                     if (d + 4 <= D) {
@@ -647,7 +653,7 @@ __global__ __launch_bounds__(512) void k_fcl_pack_w(const float* __restrict__ W,
     for (int o = 1; o < 64; o <<= 1) m = max_or_nan(m, __shfl_xor(m, o, 64));
     if (lane == 0) maxima[wave] = m;
     int e = 0;
-    for (int d0 = 0; d0 < Kd * 32; d0 += CW) {
+    for (int d0 = 0; d0 < p.Kd * 32; d0 += CW) {
         if (D > CW) load(d0);
         __syncthreads();
 #pragma unroll
@@ -657,12 +663,12 @@ __global__ __launch_bounds__(512) void k_fcl_pack_w(const float* __restrict__ W,
         if (d0 == 0) {
             for (int w = 0; w < 8; w++) m = max_or_nan(m, maxima[w]);  // (every wave: the barrier above covers the maxima)
             e = scale_exp(m) & ~7;
-            if (threadIdx.x == 0) classExp[blockIdx.x] = m == 0.f ? EXP_ZERO : e;
+            if (threadIdx.x == 0) p.classExp[block] = m == 0.f ? EXP_ZERO : e;
         }
         __syncthreads();
         for (int f = wave; f < 2 * CW / 32; f += 8) {
             const int rb = f & 1, kb = d0 / 32 + (f >> 1), r = rb * 16 + c;
-            if (kb >= Kd) break;
+            if (kb >= p.Kd) break;
             float y[8];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
@@ -670,9 +676,18 @@ __global__ __launch_bounds__(512) void k_fcl_pack_w(const float* __restrict__ W,
 #pragma unroll
                 for (int j = 0; j < 4; j++) y[4 * h + j] = ldexpf(x[j], e);
             }
-            store_pair(byClass + (((size_t)blockIdx.x * 2 + rb) * Kd + kb) * PAIR, lane, y);
+            store_pair(p.wByClass + (((size_t)block * 2 + rb) * p.Kd + kb) * PAIR, lane, y);
         }
     }
+}
+
+__global__ __launch_bounds__(512) void k_fcl_pack(PackArgs p) {
+    extern __shared__ __attribute__((aligned(16))) float tile[];  // [32][CW_LD], then the waves' maxima
+    __shared__ int exps[16];
+    const int b = blockIdx.x;
+    if (b < p.caseBlocks) pack_cases(p, b, tile, exps);
+    else if (b < p.caseBlocks + p.featBlocks) pack_feats(p, b - p.caseBlocks, exps);
+    else pack_classes(p, b - p.caseBlocks - p.featBlocks, tile);
 }
 
 // ---- logits of a piece
@@ -848,45 +863,58 @@ __global__ __launch_bounds__(256, SHARED ? 2 : 1) void k_fcl_logits(WideArgs p) 
     }
 }
 
-// ---- weight gradient of a piece: (features x classes) tiles, so that a lane's four rows are four neighbours of one row of W
-template <int MB, bool SHARED>
-__global__ __launch_bounds__(256, SHARED ? 2 : 1) void k_fcl_wgrad(const char* xByFeat, const char* dz, const int* __restrict__ featExp, float* __restrict__ dW,
-                                                      int D, int rows, int Kn, int Kv, int dTiles, int vTiles, float scaleTargets, float scaleOutput) {
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+struct GradArgs {
+    const char *xByFeat, *dz, *wByClass;
+    const int *featExp, *classExp;
+    float *dW, *slabs;
+    int D, rows, Kn, Kv, Kd, Np, Dp, nTiles, dTiles, kPerSplit, first;
+    int inputBlocks;  // blocks of the input gradient, then those of the weight gradient
+    float scaleTargets, scaleOutput;
+};
+
+template <bool SHARED, class Scale>
+__device__ __forceinline__ void turned_tile(const char* A, size_t aRow, const char* B, size_t bRow, int k0, int k1, char* lds, Acc<4>& acc,
+                                            const Scale& scale) {
+    if constexpr (SHARED) product_tile_shared<true>(A, aRow, B, bRow, k0, k1, lds, acc, scale);
+    else product_tile<4, true>(A, aRow, B, bRow, k0, k1, lds, acc, scale);
+}
+
+// weight gradient: (features x classes) tiles, so that a lane's four rows are four neighbours of one row of W
+template <bool SHARED>
+__device__ __forceinline__ void weight_tile(const GradArgs& p, int L, char* lds) {
     int tv, td;
-    mcn_xcd_group(blockIdx.x, dTiles, vTiles, tv, td);
+    mcn_xcd_group(L, p.dTiles, p.Kv / 4, tv, td);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
     const int c = lane & 15, g = lane >> 4;
-    const size_t row = (size_t)Kn * PAIR;
-    Acc<MB> acc;
-    if constexpr (SHARED) product_tile_shared<true>(xByFeat + (size_t)td * 2 * MB * row, row, dz + (size_t)tv * 4 * PAIR, (size_t)Kv * PAIR, 0, Kn, lds, acc, NoScale());
-    else product_tile<MB, true>(xByFeat + (size_t)td * 2 * MB * row, row, dz + (size_t)tv * 4 * PAIR, (size_t)Kv * PAIR, 0, Kn, lds, acc, NoScale());
+    const size_t row = (size_t)p.Kn * PAIR;
+    Acc<4> acc;
+    turned_tile<SHARED>(p.xByFeat + (size_t)td * 8 * row, row, p.dz + (size_t)tv * 4 * PAIR, (size_t)p.Kv * PAIR, 0, p.Kn, lds, acc, NoScale());
 #pragma unroll
-    for (int i = 0; i < MB; i++) {
-        const int d = td * 32 * MB + wm * 16 * MB + i * 16 + g * 4;
+    for (int i = 0; i < 4; i++) {
+        const int d = td * TILE + wm * 64 + i * 16 + g * 4;
         int e[4];
 #pragma unroll
-        for (int r = 0; r < 4; r++) e[r] = -(featExp[d + r] + DZ_EXP);
+        for (int r = 0; r < 4; r++) e[r] = -(p.featExp[d + r] + DZ_EXP);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int v = tv * TILE + wn * 64 + j * 16 + c;
-            if (v >= rows) continue;
-            float* out = dW + (size_t)v * D + d;
+            if (v >= p.rows) continue;
+            float* out = p.dW + (size_t)v * p.D + d;
             float y[4];
 #pragma unroll
-            for (int r = 0; r < 4; r++) y[r] = scaleOutput * ldexpf(acc.value(i, j, r), e[r]);
-            if (d + 4 <= D) {
+            for (int r = 0; r < 4; r++) y[r] = p.scaleOutput * ldexpf(acc.value(i, j, r), e[r]);
+            if (d + 4 <= p.D) {
                 f32x4u t = {y[0], y[1], y[2], y[3]};
-                if (scaleTargets != 0.f) {
+                if (p.scaleTargets != 0.f) {
                     const f32x4u old = *reinterpret_cast<const f32x4u*>(out);
 #pragma unroll
-                    for (int r = 0; r < 4; r++) t[r] += scaleTargets * old[r];
+                    for (int r = 0; r < 4; r++) t[r] += p.scaleTargets * old[r];
                 }
                 *reinterpret_cast<f32x4u*>(out) = t;
             } else {
 #pragma unroll
                 for (int r = 0; r < 4; r++)
-                    if (d + r < D) out[r] = (scaleTargets != 0.f ? scaleTargets * out[r] : 0.f) + y[r];
+                    if (d + r < p.D) out[r] = (p.scaleTargets != 0.f ? p.scaleTargets * out[r] : 0.f) + y[r];
             }
         }
     }
@@ -922,35 +950,40 @@ struct CarryScale {
     }
 };
 
-// ---- input gradient: the sum over the classes is split; slab s of (Dp, Np) adds up its share of every piece, in order
-template <int MB, bool SHARED>
-__global__ __launch_bounds__(256, SHARED ? 2 : 1) void k_fcl_igrad(const char* dz, const char* wByClass, const int* __restrict__ classExp, float* __restrict__ slabs,
-                                                      int Np, int Dp, int Kv, int Kd, int kPerSplit, int nTiles, int dTiles, int first) {
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+// input gradient: the sum over the classes is split; slab s of (Dp, Np) adds up its share of every piece, in order
+template <bool SHARED>
+__device__ __forceinline__ void input_tile(const GradArgs& p, int L, char* lds) {
     // the tiles of one split on one XCD: they read the same classes of dz and W
     int s, t;
-    mcn_xcd_group(blockIdx.x, nTiles * dTiles, gridDim.x / (nTiles * dTiles), s, t);
-    const int td = t / nTiles, tn = t % nTiles;
+    mcn_xcd_group(L, p.nTiles * p.dTiles, p.inputBlocks / (p.nTiles * p.dTiles), s, t);
+    const int td = t / p.nTiles, tn = t % p.nTiles;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
     const int c = lane & 15, g = lane >> 4;
-    const size_t row = (size_t)Kv * PAIR;
-    const int k0 = s * kPerSplit, k1 = min(Kv, k0 + kPerSplit);
-    Acc<MB> acc;
-    const CarryScale carry(classExp + k0, k1 - k0);
-    if constexpr (SHARED) product_tile_shared<true>(dz + (size_t)tn * 2 * MB * row, row, wByClass + (size_t)td * 4 * PAIR, (size_t)Kd * PAIR, k0, k1, lds, acc, carry);
-    else product_tile<MB, true>(dz + (size_t)tn * 2 * MB * row, row, wByClass + (size_t)td * 4 * PAIR, (size_t)Kd * PAIR, k0, k1, lds, acc, carry);
+    const size_t row = (size_t)p.Kv * PAIR;
+    const int k0 = s * p.kPerSplit, k1 = min(p.Kv, k0 + p.kPerSplit);
+    Acc<4> acc;
+    const CarryScale carry(p.classExp + k0, k1 - k0);
+    turned_tile<SHARED>(p.dz + (size_t)tn * 8 * row, row, p.wByClass + (size_t)td * 4 * PAIR, (size_t)p.Kd * PAIR, k0, k1, lds, acc, carry);
     const int e = carry.cur == EXP_ZERO ? 0 : -(carry.cur + DZ_EXP);
 #pragma unroll
-    for (int i = 0; i < MB; i++)
+    for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const int d = td * TILE + wn * 64 + j * 16 + c, n = tn * 32 * MB + wm * 16 * MB + i * 16 + g * 4;
-            f32x4* out = reinterpret_cast<f32x4*>(slabs + ((size_t)s * Dp + d) * Np + n);
+            const int d = td * TILE + wn * 64 + j * 16 + c, n = tn * TILE + wm * 64 + i * 16 + g * 4;
+            f32x4* out = reinterpret_cast<f32x4*>(p.slabs + ((size_t)s * p.Dp + d) * p.Np + n);
             f32x4 y;
 #pragma unroll
             for (int r = 0; r < 4; r++) y[r] = ldexpf(acc.value(i, j, r), e);
-            *out = first ? y : *out + y;
+            *out = p.first ? y : *out + y;
         }
+}
+
+// ---- both gradients of a piece in one launch: they wait for the same logits and not for each other
+template <bool SHARED>
+__global__ __launch_bounds__(256, SHARED ? 2 : 1) void k_fcl_grads(GradArgs p) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    if ((int)blockIdx.x < p.inputBlocks) input_tile<SHARED>(p, blockIdx.x, lds);
+    else weight_tile<SHARED>(p, blockIdx.x - p.inputBlocks, lds);
 }
 
 // ---- the end: input gradients from the slabs (blocks below dxBlocks), bias gradients from the tiles' row sums
@@ -1064,17 +1097,29 @@ WideArgs wide_args(const WidePlan& q, const float* bias, const float* labels, in
     a.kSteps = q.kSteps;
     return a;
 }
-// one piece: its packed rows, tiles and k blocks
-TileKind wide_piece(const WidePlan& q, WideArgs& a, const float* W, int D, int v0, char* ws, hipStream_t s) {
+// one piece: its packed rows, tiles and k blocks; with the first one, x
+TileKind wide_piece(const WidePlan& q, WideArgs& a, PackArgs& k, const float* W, int D, int v0, hipStream_t s) {
     a.v0 = v0;
-    a.rows = std::min(q.rows, a.V - v0);
+    a.rows = k.rows = std::min(q.rows, a.V - v0);
     a.nTiles = q.nTiles;
     a.Kv = divup(a.rows, TILE) * 4;
     const TileKind kind = tile_choice(a.Kv, q.nTiles);
     a.vTiles = a.Kv / tile_rows32(kind);
-    MCN_LAUNCH(k_fcl_pack_w, dim3(a.Kv), dim3(512), PACK_LDS, s, W + (size_t)v0 * D, a.bias ? a.bias + v0 : nullptr, (int*)(ws + q.classExp),
-               ws + q.wByClass, D, a.rows, q.Kd);
+    k.W = W + (size_t)v0 * D;
+    k.bias = a.bias ? a.bias + v0 : nullptr;
+    MCN_LAUNCH(k_fcl_pack, dim3(k.caseBlocks + k.featBlocks + a.Kv), dim3(512), PACK_LDS, s, k);
+    k.caseBlocks = k.featBlocks = 0;
     return kind;
+}
+PackArgs pack_args(const WidePlan& q, const float* X, const float* labels, int D, int V, int N, bool feats, char* ws) {
+    PackArgs k = {};
+    k.X = X; k.labels = labels;
+    k.caseExp = (int*)(ws + q.caseExp); k.featExp = (int*)(ws + q.featExp);
+    k.xByCase = ws + q.xByCase; k.xByFeat = ws + q.xByFeat;
+    k.D = D; k.V = V; k.N = N; k.Kd = q.Kd; k.Kn = q.Kn;
+    k.caseBlocks = q.Np / 16; k.featBlocks = feats ? q.Dp / 16 : 0;
+    k.classExp = (int*)(ws + q.classExp); k.wByClass = ws + q.wByClass;
+    return k;
 }
 
 int wide_cost(const float* W, const float* X, const float* bias, const float* labels, float* stats, float* logp, float* correct, int D, int V,
@@ -1082,11 +1127,10 @@ int wide_cost(const float* W, const float* X, const float* bias, const float* la
     const WidePlan q = wide_plan(D, V, N, false);
     WideArgs a = wide_args(q, bias, labels, V, N, ws);
     a.labelLogits = (float*)(ws + q.labelLogits);
-    MCN_LAUNCH(k_fcl_pack_x, dim3(q.Np / 16), dim3(512), 0, s, X, labels, (int*)(ws + q.caseExp), (int*)nullptr, ws + q.xByCase, (char*)nullptr,
-               D, V, N, q.Kd, q.Kn, q.Np / 16);
+    PackArgs pack = pack_args(q, X, labels, D, V, N, false, ws);
     int tiles = 0;
     for (int v0 = 0; v0 < V; v0 += q.rows) {
-        const TileKind kind = wide_piece(q, a, W, D, v0, ws, s);
+        const TileKind kind = wide_piece(q, a, pack, W, D, v0, s);
         a.part = (float*)(ws + q.part) + (size_t)tiles * 3 * N;
         launch_logits<false>(kind, a, s);
         tiles += a.vTiles;
@@ -1104,35 +1148,28 @@ int wide_grad(const float* W, const float* X, const float* bias, const float* la
     a.stats = stats;
     a.dz = ws + q.dz;
     a.dbPart = dB ? (float*)(ws + q.dbPart) : nullptr;
-    const int* featExp = (const int*)(ws + q.featExp);
     float* slabs = (float*)(ws + q.slabs);
-    MCN_LAUNCH(k_fcl_pack_x, dim3(q.Np / 16 + (dW ? q.Dp / 16 : 0)), dim3(512), 0, s, X, labels, (int*)(ws + q.caseExp), (int*)(ws + q.featExp),
-               ws + q.xByCase, ws + q.xByFeat, D, V, N, q.Kd, q.Kn, q.Np / 16);
+    PackArgs pack = pack_args(q, X, labels, D, V, N, dW != nullptr, ws);
+    GradArgs t = {};
+    t.xByFeat = ws + q.xByFeat; t.dz = ws + q.dz; t.wByClass = ws + q.wByClass;
+    t.featExp = (const int*)(ws + q.featExp); t.classExp = (const int*)(ws + q.classExp);
+    t.slabs = slabs;
+    t.D = D; t.Kn = q.Kn; t.Kd = q.Kd; t.Np = q.Np; t.Dp = q.Dp; t.nTiles = q.nTiles; t.dTiles = q.dTiles;
+    t.scaleTargets = scaleWeightTargets;
+    t.scaleOutput = scaleWeightOutput * coeff;
     for (int v0 = 0; v0 < V; v0 += q.rows) {
-        const TileKind kind = wide_piece(q, a, W, D, v0, ws, s);
+        const TileKind kind = wide_piece(q, a, pack, W, D, v0, s);
         launch_logits<true>(kind, a, s);
-        if (dW) {
-            const int vTiles = a.Kv / 4;
-            const TileKind k = tile_choice(q.dTiles * 4, vTiles);
-            const int dTiles = q.dTiles * 4 / tile_rows32(k);
-            const dim3 grid(vTiles * dTiles), block(256);
-            const float sO = scaleWeightOutput * coeff;
-            float* out = dW + (size_t)v0 * D;
-#define WGRAD(MB, SH) MCN_LAUNCH((k_fcl_wgrad<MB, SH>), grid, block, tile_bytes(k), s, ws + q.xByFeat, a.dz, featExp, out, D, a.rows, q.Kn, a.Kv, dTiles, vTiles, scaleWeightTargets, sO)
-            if (k == SHARED) WGRAD(4, true);
-            else if (k == WHOLE) WGRAD(4, false);
-            else WGRAD(2, false);
-#undef WGRAD
-        }
-        if (dX) {
-            // (a short last piece has fewer, not shorter, shares: each adds to its slab)
-            const int tiles = q.nTiles * q.dTiles, kPer = a.Kv == q.Kv ? q.kPerSplit : std::max(8, divup(a.Kv, q.splits)), splits = divup(a.Kv, kPer);
-            const dim3 grid(splits * tiles), block(256);
-#define IGRAD(SH, KIND) MCN_LAUNCH((k_fcl_igrad<4, SH>), grid, block, tile_bytes(KIND), s, a.dz, a.wByClass, a.classExp, slabs, q.Np, q.Dp, a.Kv, q.Kd, kPer, q.nTiles, q.dTiles, v0 == 0)
-            if (splits * tiles > 256) IGRAD(true, SHARED);
-            else IGRAD(false, WHOLE);
-#undef IGRAD
-        }
+        // (a short last piece has fewer, not shorter, shares of the input gradient: each adds to its slab)
+        t.kPerSplit = a.Kv == q.Kv ? q.kPerSplit : std::max(8, divup(a.Kv, q.splits));
+        t.inputBlocks = dX ? divup(a.Kv, t.kPerSplit) * q.nTiles * q.dTiles : 0;
+        t.dW = dW ? dW + (size_t)v0 * D : nullptr;
+        t.rows = a.rows;
+        t.Kv = a.Kv;
+        t.first = v0 == 0;
+        const int blocks = t.inputBlocks + (dW ? a.Kv / 4 * q.dTiles : 0);
+        if (blocks > 256) MCN_LAUNCH(k_fcl_grads<true>, dim3(blocks), dim3(256), tile_bytes(SHARED), s, t);
+        else if (blocks > 0) MCN_LAUNCH(k_fcl_grads<false>, dim3(blocks), dim3(256), tile_bytes(WHOLE), s, t);
         if (int rc = MCN_LAUNCH_CHECK("fcLogregGrad")) return rc;
     }
     if (dX || dB) {
