@@ -502,31 +502,41 @@ __device__ __forceinline__ void product_tile_shared(const char* A, size_t aRow, 
     copy();
     for (int t = 0; t < n; t++) {
         wait_copies_and_meet<0>();  // stage t has landed, and everyone has read the other buffer
+        if (t + 1 < n) copy();
         Frags<4> f;
         const char* s = lds + take;
         take ^= STAGE;
+        auto readB = [&](int j, int q) {
+            if constexpr (TURNED) {
+                const char* p = s + offB + (j >> 1) * PAIR + q * FRAG + (j & 1) * 512;
+                f.b[j][q] = read_frag_turned(p, p + 4 * PAIR);
+            } else {
+                f.b[j][q] = read_frag(s + offB + j * PAIR + q * FRAG);
+            }
+        };
+        auto readA = [&](int i, int q) { f.a[i][q] = read_frag(s + offA + i * PAIR + q * FRAG); };
+        readA(0, 0);
 #pragma unroll
-        for (int q = 0; q < 2; q++)
+        for (int j = 0; j < 4; j++) readB(j, 0);
+        readA(0, 1);
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if constexpr (TURNED) {
-                    const char* p = s + offB + (j >> 1) * PAIR + q * FRAG + (j & 1) * 512;
-                    f.b[j][q] = read_frag_turned(p, p + 4 * PAIR);
-                } else {
-                    f.b[j][q] = read_frag(s + offB + j * PAIR + q * FRAG);
-                }
+        for (int j = 0; j < 4; j++) readB(j, 1);
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int q = 0; q < 2; q++) f.a[i][q] = read_frag(s + offA + i * PAIR + q * FRAG);
-        if (t + 1 < n) copy();
+        for (int i = 1; i < 4; i++) {
+            readA(i, 0);
+            readA(i, 1);
+        }
         scale(t, acc);
+        // The wave that has its fragments goes before the other block's, which then reads under these products (512 x 100000 x 1024, both
+        // calls, with the copies asked for before the reads and the reads in the products' order: 1.56 -> 1.50 ms).
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int m = 0; m < 48; m++) {
             const int i = m / 12, k = m % 12 / 4, j = m % 4;
             f32x4& to = acc.c[k ? 1 : 0][i][j];
             to = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.a[i][k == 2], f.b[j][k == 1], to, 0, 0, 0);
         }
+        __builtin_amdgcn_s_setprio(0);
     }
     wait_copies_and_meet<0>();
 }
