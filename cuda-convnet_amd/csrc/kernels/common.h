@@ -77,6 +77,10 @@ __device__ __forceinline__ void mcn_xcd_group(int L, int T, int nG, int& group, 
 
 static inline int divup(int a, int b) { return (a + b - 1) / b; }
 static inline size_t divup_sz(size_t a, size_t b) { return (a + b - 1) / b; }
+// whether na floats at a and nb at b share any (a null pointer shares nothing)
+static inline bool mcn_overlap(const float* a, size_t na, const float* b, size_t nb) {
+    return a && b && (uintptr_t)a < (uintptr_t)b + nb * sizeof(float) && (uintptr_t)b < (uintptr_t)a + na * sizeof(float);
+}
 
 // v_mfma_f32_16x16x4_f32: lane l holds A[row=l&15][k=l>>4], B[k=l>>4][col=l&15];
 // acc[r] = D[row=(l>>4)*4+r][col=l&15].  Exact fp32 (k-ordered fma chain).

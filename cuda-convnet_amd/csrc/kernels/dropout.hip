@@ -60,7 +60,8 @@ MCN_API int mcn_dropout(const float* inputs, float* target, size_t numElements, 
                         const uint64_t* deviceStep, float scaleTargets, float scaleOutput, void* stream) {
     MCN_REQUIRE(inputs && target, "dropout: null pointer");
     MCN_REQUIRE(dropProb >= 0.f && dropProb < 1.f, "dropout: probability %g is not in [0, 1)", (double)dropProb);  // (refuses a NaN too)
-    MCN_REQUIRE(target == inputs || target + numElements <= inputs || inputs + numElements <= target, "dropout: target overlaps inputs in part");
+    MCN_REQUIRE(numElements <= (size_t)1 << 40, "dropout: %zu elements", numElements);
+    MCN_REQUIRE(target == inputs || !mcn_overlap(target, numElements, inputs, numElements), "dropout: target overlaps inputs in part");
     if (numElements == 0) return MCN_OK;
     const uint32_t threshold = (uint32_t)((double)dropProb * 4294967296.0);  // (a float below 1 is at most 1 - 2^-24: fits)
     const float keepScale = (float)((double)scaleOutput / (1.0 - (double)dropProb));

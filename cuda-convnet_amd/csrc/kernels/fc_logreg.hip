@@ -13,19 +13,13 @@ namespace {
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // (16-byte accesses at any multiple of four bytes)
 
 constexpr int NARROW = 64;  // k_fcl_narrow: most cases
-constexpr size_t NARROW_GRAD = (size_t)1 << 23;  // ... and weights, for the gradients
-constexpr size_t PIECE_ELEMS = (size_t)1 << 24;
 constexpr int PIECE_MB = 128;  // fragments of a piece; 512 x 100000 x 1024, both calls: 64 MB 1.77 ms, 128 MB 1.65 ms, 224 MB 1.62 ms
 
 struct NarrowArgs {
     const float *W, *X, *bias, *labels;
     int D, V, N;
-    int v0, vRows;        // the piece: classes [v0, v0 + vRows)
-    float* part;          // forward: [tiles][3][N]
-    float* labelLogits;   // forward: [N]
-    const float* stats;   // backward: [2][N]
-    float* dz;            // backward: [vRows][N]
-    float coeff;
+    float* part;         // [tiles][3][N]
+    float* labelLogits;  // [N]
 };
 
 // Statistics of a set of logits: the max, the entries at the max, and the sum of exp(z - max) over the OTHER entries.  The three are
@@ -66,17 +60,16 @@ __device__ __forceinline__ float exp_neg(float x) {
 // takes 16 RG classes, its four waves a quarter of the features each (16 at a time: a lane reads 16 bytes of its class's row, and the
 // four matrix instructions that follow take one feature of every lane's four); their sums are joined in LDS.  RG = 1 while the classes
 // do not fill the chip, 4 beyond, where it keeps the number of tiles to join down.
-template <bool BWD, int NB, int RG>
+template <int NB, int RG>
 __global__ __launch_bounds__(256) void k_fcl_narrow(NarrowArgs p) {
     __shared__ f32x4 red[4][RG][NB][64];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int vBase = blockIdx.x * 16 * RG;
     const float* rowPtr[RG];
 #pragma unroll
-    for (int q = 0; q < RG; q++) rowPtr[q] = p.W + (size_t)(p.v0 + min(vBase + q * 16 + c, p.vRows - 1)) * p.D;  // (a class behind the last one: read and not used)
+    for (int q = 0; q < RG; q++) rowPtr[q] = p.W + (size_t)min(vBase + q * 16 + c, p.V - 1) * p.D;  // (a class behind the last one: read and not used)
     f32x4 acc[RG][NB] = {};
     const int steps = (p.D + 15) / 16;
-#pragma unroll 4
     for (int t = wave; t < steps; t += 4) {
         const int k = t * 16 + g * 4;
         f32x4 a[RG];
@@ -111,11 +104,7 @@ __global__ __launch_bounds__(256) void k_fcl_narrow(NarrowArgs p) {
     if (wave >= NB) return;  // a wave: 16 cases
     const int n = wave * 16 + c;
     int label = -1;
-    float M = 0.f, S = 0.f;
-    if (n < p.N && label_of(p.labels[n], p.V, label) && BWD) {
-        M = p.stats[n];
-        S = p.stats[p.N + n];
-    }
+    if (n < p.N) label_of(p.labels[n], p.V, label);
     float z[RG][4], m = -INFINITY;
 #pragma unroll
     for (int q = 0; q < RG; q++) {
@@ -123,25 +112,10 @@ __global__ __launch_bounds__(256) void k_fcl_narrow(NarrowArgs p) {
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const int v = vBase + q * 16 + g * 4 + r;
-            const float bv = v < p.vRows ? (p.bias ? p.bias[p.v0 + v] : 0.f) : -INFINITY;
+            const float bv = v < p.V ? (p.bias ? p.bias[v] : 0.f) : -INFINITY;
             z[q][r] = bv == -INFINITY ? -INFINITY : s[r] + bv;  // (a class that is taken out, whatever its weights hold)
             m = fmaxf(z[q][r], m);
         }
-    }
-    if (BWD) {
-        const bool counts = S != 0.f;  // (no label, or no class left: nothing; a NaN goes on)
-        const float inv = counts ? 1.f / S : 0.f;
-#pragma unroll
-        for (int q = 0; q < RG; q++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int v = vBase + q * 16 + g * 4 + r;
-                if (v < p.vRows && n < p.N) {
-                    const float hot = label == p.v0 + v ? 1.f : 0.f;
-                    p.dz[(size_t)v * p.N + n] = counts ? p.coeff * (hot - exp_neg(z[q][r] - M) * inv) : 0.f;
-                }
-            }
-        return;
     }
     for (int o = 16; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
     const float from = m == -INFINITY ? 0.f : m;
@@ -154,7 +128,7 @@ __global__ __launch_bounds__(256) void k_fcl_narrow(NarrowArgs p) {
             const bool top = x == 0.f && m != -INFINITY;
             rest += top ? 0.f : exp_neg(x);
             cnt += top ? 1.f : 0.f;
-            if (label >= 0 && label == p.v0 + vBase + q * 16 + g * 4 + r) p.labelLogits[n] = z[q][r];
+            if (label >= 0 && label == vBase + q * 16 + g * 4 + r) p.labelLogits[n] = z[q][r];
         }
     for (int o = 16; o < 64; o <<= 1) {
         rest += __shfl_xor(rest, o, 64);
@@ -270,7 +244,7 @@ __global__ __launch_bounds__(256) void k_fcl_cost(const float* __restrict__ labe
 // bits.  With the largest magnitude of a scaled group below 2^15 the relative error of a product is about 2^-22 for entries down to
 // 2^-21 of the group's largest, and an entry further down is off by at most 2^-43 of it.  The groups: a case's features for the
 // logits, a feature's cases for the weight gradient, 32 classes' weights, and +-1 for dz / coeff.  Along the summed dimension a group
-// is either whole or, for the classes of the input gradient, its scale is carried along (k_fcl_igrad), so a row of large weights
+// is either whole or, for the classes of the input gradient, its scale is carried along (CarryScale), so a row of large weights
 // takes no bits from the other groups.
 //
 // Operands are split ONCE by a pack launch into fragments of 16 rows x 32 k entries and two pieces, 1 KB each:
@@ -618,6 +592,10 @@ __device__ __forceinline__ void pack_feats(const PackArgs& p, int block, int* ex
 // (all of a thread's loads in flight at once) and LDS; rows of at most 512 features are read once, longer ones a second time for their
 // max.
 constexpr int CW = 512, CW_LD = CW + 4;
+// A sum that has groups of large weights in it is multiplied up where a group of tiny ones follows: |sum| <= 2 max|w| (of dz / coeff, the
+// magnitudes of a case add up to 2 at most), so with this bound on the exponents no weights below 2^48 take it out of range.  It
+// leaves a group whose largest weight is below 2^-50 with less than 22 bits below 2^-78.
+constexpr int CLASS_EXP_MAX = 64;
 constexpr int PACK_LDS = (32 * CW_LD + 8) * 4;
 __device__ __forceinline__ void pack_classes(const PackArgs& p, int block, float* tile) {
     float* maxima = tile + 32 * CW_LD;
@@ -672,7 +650,7 @@ __device__ __forceinline__ void pack_classes(const PackArgs& p, int block, float
             for (int h = 0; h < 2; h++) *reinterpret_cast<f32x4*>(tile + (wave * 4 + r) * CW_LD + h * 256 + lane * 4) = t[r][h];
         if (d0 == 0) {
             for (int w = 0; w < 8; w++) m = max_or_nan(m, maxima[w]);  // (every wave: the barrier above covers the maxima)
-            e = scale_exp(m) & ~7;
+            e = min(scale_exp(m) & ~7, CLASS_EXP_MAX);
             if (threadIdx.x == 0) p.classExp[block] = m == 0.f ? EXP_ZERO : e;
         }
         __syncthreads();
@@ -996,26 +974,34 @@ __global__ __launch_bounds__(256, SHARED ? 2 : 1) void k_fcl_grads(GradArgs p) {
     else weight_tile<SHARED>(p, blockIdx.x - p.inputBlocks, lds);
 }
 
-// ---- the end: input gradients from the slabs (blocks below dxBlocks), bias gradients from the tiles' row sums
-__global__ __launch_bounds__(256) void k_fcl_finish(const float* __restrict__ slabs, const float* __restrict__ dbPart, float* dX, float* dB,
-                                                    int D, int V, int N, int Np, int Dp, int splits, int nTiles, int dxBlocks, float coeff,
-                                                    float scaleInputTargets, float scaleBiasTargets, float scaleBiasOutput) {
-    if ((int)blockIdx.x < dxBlocks) {
-        const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-        if (i >= (size_t)D * N) return;
-        const size_t d = i / N, n = i % N;
-        float v = 0.f;
+// ---- the end: input gradients from the slabs (blocks below dxBlocks), bias gradients from the tiles' row sums.  The packed weights of a
+// class that its bias takes out are zero; a case that has such a class for its label, and others left, still has the formula's
+// weights[label] * 1, and gets it here.
+struct FinishArgs {
+    const float *slabs, *dbPart, *W, *bias, *labels, *stats;
+    float *dX, *dB;
+    int D, V, N, Np, Dp, splits, nTiles, dxBlocks;
+    float coeff, scaleInputTargets, scaleBiasTargets, scaleBiasOutput;
+};
+__global__ __launch_bounds__(256) void k_fcl_finish(FinishArgs p) {
+    if ((int)blockIdx.x < p.dxBlocks) {
+        for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < (size_t)p.D * p.N; i += (size_t)p.dxBlocks * 256) {
+            const size_t d = i / p.N, n = i % p.N;
+            float v = 0.f;
 #pragma unroll 8
-        for (int s = 0; s < splits; s++) v += slabs[((size_t)s * Dp + d) * Np + n];
-        dX[i] = (scaleInputTargets != 0.f ? scaleInputTargets * dX[i] : 0.f) + coeff * v;
+            for (int s = 0; s < p.splits; s++) v += p.slabs[((size_t)s * p.Dp + d) * p.Np + n];
+            int label;
+            if (p.bias && label_of(p.labels[n], p.V, label) && p.bias[label] == -INFINITY && p.stats[p.N + n] != 0.f) v += p.W[(size_t)label * p.D + d];
+            p.dX[i] = (p.scaleInputTargets != 0.f ? p.scaleInputTargets * p.dX[i] : 0.f) + p.coeff * v;
+        }
         return;
     }
-    const int v = (blockIdx.x - dxBlocks) * 256 + threadIdx.x;
-    if (v >= V) return;
+    const int v = (blockIdx.x - p.dxBlocks) * 256 + threadIdx.x;
+    if (v >= p.V) return;
     float s = 0.f;
 #pragma unroll 8
-    for (int t = 0; t < nTiles; t++) s += dbPart[(size_t)t * V + v];
-    dB[v] = (scaleBiasTargets != 0.f ? scaleBiasTargets * dB[v] : 0.f) + scaleBiasOutput * coeff * s;
+    for (int t = 0; t < p.nTiles; t++) s += p.dbPart[(size_t)t * p.V + v];
+    p.dB[v] = (p.scaleBiasTargets != 0.f ? p.scaleBiasTargets * p.dB[v] : 0.f) + p.scaleBiasOutput * p.coeff * s;
 }
 
 // Which tile a product takes: SHARED 128 x 128, two blocks per CU; WHOLE 128 x 128 or HALF 64 x 128, one block per CU with its stages
@@ -1039,11 +1025,10 @@ struct WidePlan {
                                                  // writes every slab
     size_t classExp, caseExp, featExp, xByCase, xByFeat, wByClass, dz, dbPart, slabs, part, labelLogits, total;
 };
-// When the packed operands pay (us, narrow / wide).  Cost, 512 x 10575: 16 cases 16 / 34, 64 cases 26 / 35; 512 x 100000: 56 / 145, 121 / 147.
-// Gradients, whose narrow form takes dz through mcn_gemm: 512 x 10575 16 cases 51 / 59, 64 cases 60 / 60; 2048 x 10575 179 / 152;
-// 512 x 100000 404 / 314: by the number of weights.
+// When the packed operands pay for the cost alone (us, narrow / wide).  512 x 10575: 16 cases 16 / 34, 64 cases 26 / 35; 512 x 100000:
+// 56 / 145, 121 / 147.  The gradients always take them: 512 x 10575, one case 52 us, 64 cases 47 us (fp32 products of a dz of their own
+// layout: 50 and 60 us).
 bool wide_cost_usable(int N) { return N > NARROW; }
-bool wide_grad_usable(int D, int V, int N) { return N > NARROW || (size_t)D * V > NARROW_GRAD; }
 
 size_t al256(size_t b) { return (b + 255) / 256 * 256; }
 
@@ -1183,44 +1168,33 @@ int wide_grad(const float* W, const float* X, const float* bias, const float* la
         if (int rc = MCN_LAUNCH_CHECK("fcLogregGrad")) return rc;
     }
     if (dX || dB) {
-        const int dxBlocks = dX ? (int)divup_sz((size_t)D * N, 256) : 0;
-        MCN_LAUNCH(k_fcl_finish, dim3(dxBlocks + (dB ? divup(V, 256) : 0)), dim3(256), 0, s, slabs, (const float*)(ws + q.dbPart), dX, dB, D, V, N, q.Np,
-                   q.Dp, q.splits, q.nTiles, dxBlocks, coeff, scaleInputTargets, scaleBiasTargets, scaleBiasOutput);
+        const int dxBlocks = dX ? (int)std::min<size_t>(divup_sz((size_t)D * N, 256), 1 << 16) : 0;
+        const FinishArgs f = {slabs, (const float*)(ws + q.dbPart), W, bias, labels, stats, dX, dB, D, V, N, q.Np, q.Dp, q.splits, q.nTiles,
+                              dxBlocks, coeff, scaleInputTargets, scaleBiasTargets, scaleBiasOutput};
+        MCN_LAUNCH(k_fcl_finish, dim3(dxBlocks + (dB ? divup(V, 256) : 0)), dim3(256), 0, s, f);
     }
     return MCN_LAUNCH_CHECK("fcLogregGrad");
 }
 
-bool fcl_sizes_ok(int D, int V, int N) { return D > 0 && V > 0 && N > 0 && V <= (1 << 24) && D <= (1 << 20) && N <= (1 << 20); }
+bool fcl_sizes_ok(int D, int V, int N) {
+    return D > 0 && V > 0 && N > 0 && V <= (1 << 24) && D <= (1 << 20) && N <= (1 << 20) && (size_t)D * N <= (size_t)1 << 34;
+}
 
 size_t al16b(size_t b) { return (b + 15) / 16 * 16; }
-
-// The narrow path: tiles of the forward pass, and the pieces whose dz (and the products that take it) fit the workspace.
 int narrow_groups(int V) { return V > 16 * 1024 ? 4 : 1; }
 int narrow_tiles(int V) { return divup(V, 16 * narrow_groups(V)); }
-int narrow_piece(int V, int D, int N) {
-    const size_t rows = std::min<size_t>(PIECE_ELEMS / (size_t)std::max(N, D), (size_t)1 << 19) / 64 * 64;
-    return (int)std::min<size_t>((size_t)V, std::max<size_t>(rows, 64));
-}
-size_t narrow_inner_bytes(int rows, int D, int N) {
-    return al16b(std::max({mcn_gemm_workspace_bytes(rows, D, N, 0, 1), mcn_gemm_workspace_bytes(D, N, rows, 1, 0), mcn_add_sum_workspace_bytes(rows, N, 1)}));
-}
 size_t fcl_cost_bytes(int D, int V, int N) {
     if (wide_cost_usable(N)) return wide_plan(D, V, N, false).total;
     return al16b((size_t)narrow_tiles(V) * 3 * N * sizeof(float)) + al16b((size_t)N * sizeof(float));
 }
-size_t fcl_grad_bytes(int D, int V, int N) {
-    if (wide_grad_usable(D, V, N)) return wide_plan(D, V, N, true).total;
-    const int rows = narrow_piece(V, D, N), rest = V % rows;
-    return al16b((size_t)rows * N * sizeof(float)) + std::max(narrow_inner_bytes(rows, D, N), rest ? narrow_inner_bytes(rest, D, N) : 0);
-}
+size_t fcl_grad_bytes(int D, int V, int N) { return wide_plan(D, V, N, true).total; }
 
-template <bool BWD>
 void launch_narrow(const NarrowArgs& p, hipStream_t s) {
-    const int groups = narrow_groups(p.vRows);
-    const dim3 grid(divup(p.vRows, 16 * groups)), block(256);
-#define NARROW_LAUNCH(NB)                                                                       \
-    if (groups == 1) MCN_LAUNCH((k_fcl_narrow<BWD, NB, 1>), grid, block, 0, s, p); \
-    else MCN_LAUNCH((k_fcl_narrow<BWD, NB, 4>), grid, block, 0, s, p)
+    const int groups = narrow_groups(p.V);
+    const dim3 grid(narrow_tiles(p.V)), block(256);
+#define NARROW_LAUNCH(NB)                                                                 \
+    if (groups == 1) MCN_LAUNCH((k_fcl_narrow<NB, 1>), grid, block, 0, s, p); \
+    else MCN_LAUNCH((k_fcl_narrow<NB, 4>), grid, block, 0, s, p)
     switch (divup(p.N, 16)) {
         case 1: NARROW_LAUNCH(1); break;
         case 2: NARROW_LAUNCH(2); break;
@@ -1258,10 +1232,10 @@ MCN_API int mcn_fc_logreg_cost(const float* weights, const float* inputs, const 
         if (int rc = wide_cost(weights, inputs, biases, labels, caseStats, labelLogProbs, correctProbs, numInputs, numOutputs, numCases, (char*)workspace, s)) return rc;
     } else {
         const int tiles = narrow_tiles(numOutputs);
-        NarrowArgs p = {weights, inputs, biases, labels, numInputs, numOutputs, numCases, 0, numOutputs};
+        NarrowArgs p = {weights, inputs, biases, labels, numInputs, numOutputs, numCases};
         p.part = (float*)workspace;
         p.labelLogits = (float*)((char*)workspace + al16b((size_t)tiles * 3 * numCases * sizeof(float)));
-        launch_narrow<false>(p, s);
+        launch_narrow(p, s);
         MCN_LAUNCH(k_fcl_join, dim3(divup(numCases, 16)), dim3(1024), 0, s, p.part, p.labelLogits, labels, caseStats, labelLogProbs, correctProbs,
                    numOutputs, numCases, tiles);
     }
@@ -1275,31 +1249,14 @@ MCN_API int mcn_fc_logreg_grad(const float* weights, const float* inputs, const 
                                float scaleBiasTargets, float scaleBiasOutput, void* workspace, size_t workspaceBytes, void* stream) {
     MCN_REQUIRE(weights && inputs && labels && caseStats, "fcLogregGrad: null pointer");
     MCN_REQUIRE(inputGrads || weightGrads || biasGrads, "fcLogregGrad: nothing to compute");
-    MCN_REQUIRE(inputGrads != inputs && weightGrads != weights, "fcLogregGrad: a gradient is written over its operand");
     MCN_REQUIRE(fcl_sizes_ok(numInputs, numOutputs, numCases), "fcLogregGrad: %d inputs, %d outputs, %d cases", numInputs, numOutputs, numCases);
+    const size_t nX = (size_t)numInputs * numCases, nW = (size_t)numOutputs * numInputs, nB = (size_t)numOutputs;
+    const struct { const float* p; size_t n; } ins[] = {{weights, nW}, {inputs, nX}, {biases, nB}, {labels, (size_t)numCases}, {caseStats, (size_t)numCases * 2}},
+                                               outs[] = {{inputGrads, nX}, {weightGrads, nW}, {biasGrads, nB}};
+    for (const auto& o : outs)
+        for (const auto& i : ins) MCN_REQUIRE(!mcn_overlap(o.p, o.n, i.p, i.n), "fcLogregGrad: a gradient is written over an operand");
     if (int rc = fcl_check("fcLogregGrad", workspace, workspaceBytes, fcl_grad_bytes(numInputs, numOutputs, numCases))) return rc;
-    hipStream_t s = (hipStream_t)stream;
-    if (wide_grad_usable(numInputs, numOutputs, numCases))
-        return wide_grad(weights, inputs, biases, labels, caseStats, inputGrads, weightGrads, biasGrads, numInputs, numOutputs, numCases, coeff,
-                         scaleInputTargets, scaleWeightTargets, scaleWeightOutput, scaleBiasTargets, scaleBiasOutput, (char*)workspace, s);
-    const int D = numInputs, N = numCases, piece = narrow_piece(numOutputs, D, N);
-    float* dz = (float*)workspace;
-    void* ws = (char*)workspace + al16b((size_t)piece * N * sizeof(float));
-    const size_t wsBytes = workspaceBytes - al16b((size_t)piece * N * sizeof(float));
-    for (int v0 = 0; v0 < numOutputs; v0 += piece) {
-        const int rows = std::min(piece, numOutputs - v0);
-        NarrowArgs p = {weights, inputs, biases, labels, D, numOutputs, N, v0, rows};
-        p.stats = caseStats;
-        p.dz = dz;
-        p.coeff = coeff;
-        launch_narrow<true>(p, s);
-        if (int rc = MCN_LAUNCH_CHECK("fcLogregGrad")) return rc;
-        if (weightGrads)
-            if (int rc = mcn_gemm(dz, inputs, weightGrads + (size_t)v0 * D, rows, D, N, 0, 1, scaleWeightOutput, scaleWeightTargets, ws, wsBytes, stream)) return rc;
-        if (biasGrads)
-            if (int rc = mcn_add_sum(biasGrads + v0, dz, rows, N, 1, scaleBiasTargets, scaleBiasOutput, ws, wsBytes, stream)) return rc;
-        if (inputGrads)
-            if (int rc = mcn_gemm(weights + (size_t)v0 * D, dz, inputGrads, D, N, rows, 1, 0, 1.f, v0 ? 1.f : scaleInputTargets, ws, wsBytes, stream)) return rc;
-    }
-    return MCN_OK;
+    return wide_grad(weights, inputs, biases, labels, caseStats, inputGrads, weightGrads, biasGrads, numInputs, numOutputs, numCases, coeff,
+                     scaleInputTargets, scaleWeightTargets, scaleWeightOutput, scaleBiasTargets, scaleBiasOutput, (char*)workspace,
+                     (hipStream_t)stream);
 }

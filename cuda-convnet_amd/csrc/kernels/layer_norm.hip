@@ -581,7 +581,7 @@ Plan ln_plan(int F, int N, int rows) {
 
 inline bool al16(const void* p) { return ((uintptr_t)p % 16) == 0; }
 
-bool ln_sizes_ok(int F, int N) { return F > 0 && N > 0 && F <= (1 << 28) && N <= (1 << 28); }
+bool ln_sizes_ok(int F, int N) { return F > 0 && N > 0 && F <= (1 << 26) && N <= (1 << 26); }  // (every grid: below 2^32 threads)
 
 int ln_require_workspace(const void* ws, size_t have, size_t need, const char* what) {
     if (need > 0 && (!ws || have < need)) {
@@ -603,6 +603,8 @@ MCN_API size_t mcn_layer_norm_workspace_bytes(int numFeatures, int numCases) {
 MCN_API int mcn_layer_norm(const float* inputs, const float* gains, const float* biases, float* target, float* caseStats, int numFeatures,
                            int numCases, float eps, void* workspace, size_t workspaceBytes, void* stream) {
     MCN_REQUIRE(inputs && target && ln_sizes_ok(numFeatures, numCases), "layerNorm: bad argument");
+    const size_t n = (size_t)numFeatures * numCases;
+    MCN_REQUIRE(target == inputs || !mcn_overlap(target, n, inputs, n), "layerNorm: target overlaps inputs in part");
     MCN_REQUIRE(eps > 0.f, "layerNorm: eps %g is not positive", (double)eps);
     if (int rc = ln_require_workspace(workspace, workspaceBytes, mcn_layer_norm_workspace_bytes(numFeatures, numCases), "layerNorm")) return rc;
     hipStream_t st = (hipStream_t)stream;
@@ -645,7 +647,8 @@ MCN_API int mcn_layer_norm_undo(const float* outGrads, const float* inputs, cons
                                 void* workspace, size_t workspaceBytes, void* stream) {
     MCN_REQUIRE(outGrads && inputs && caseStats && ln_sizes_ok(numFeatures, numCases), "layerNormUndo: bad argument");
     MCN_REQUIRE(target || gainGrads || biasGrads, "layerNormUndo: nothing to compute");
-    MCN_REQUIRE(target != outGrads && target != inputs, "layerNormUndo: the target is one of the operands");
+    const size_t n = (size_t)numFeatures * numCases;
+    MCN_REQUIRE(!mcn_overlap(target, n, outGrads, n) && !mcn_overlap(target, n, inputs, n), "layerNormUndo: the target overlaps an operand");
     if (int rc = ln_require_workspace(workspace, workspaceBytes, mcn_layer_norm_undo_workspace_bytes(numFeatures, numCases), "layerNormUndo")) return rc;
     hipStream_t st = (hipStream_t)stream;
     const int F = numFeatures, N = numCases;

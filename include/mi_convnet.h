@@ -574,8 +574,9 @@ int mcn_l2reg_grad(const float* ground, const float* data, float* target, int nu
  * its DeepID definitions carry a dropout key that no parser reads -- and keeps the logits of every class) ------------------- */
 /* Layer norm over the features of each case: inputs, target (numFeatures, numCases); gains, biases (numFeatures, may be NULL: 1 / 0);
  *   target[f,n] = gains[f] * (inputs[f,n] - mean[n]) * r[n] + biases[f],  r = 1 / sqrt(var + eps), var over numFeatures, eps > 0.
- * caseStats (2, numCases): the means, then r, for mcn_layer_norm_undo (may be NULL).  target may be inputs itself.  Sizes up to
- * 2^28 each.  Calls that run at the same time need a workspace each; so do graphs that are replayed at the same time. */
+ * caseStats (2, numCases): the means, then r, for mcn_layer_norm_undo (may be NULL).  target may be inputs itself; otherwise the two do
+ * not overlap.  Sizes from 1 to 2^26 each.  Calls that run at the same time need a workspace each; so do graphs that are replayed at
+ * the same time. */
 size_t mcn_layer_norm_workspace_bytes(int numFeatures, int numCases);
 int mcn_layer_norm(const float* inputs, const float* gains, const float* biases, float* target, float* caseStats, int numFeatures,
                    int numCases, float eps, void* workspace, size_t workspaceBytes, void* stream);
@@ -583,7 +584,7 @@ int mcn_layer_norm(const float* inputs, const float* gains, const float* biases,
  * be NULL (not wanted), but not all of them:
  *   target (numFeatures, numCases) = scaleTargets*target + scaleOutput * d/d inputs,
  *   gainGrads, biasGrads (numFeatures) = scale{Gain,Bias}Targets * old + scale{Gain,Bias}Output * d/d gains, biases.
- * The target is neither outGrads nor inputs. */
+ * The target overlaps neither outGrads nor inputs. */
 size_t mcn_layer_norm_undo_workspace_bytes(int numFeatures, int numCases);
 int mcn_layer_norm_undo(const float* outGrads, const float* inputs, const float* gains, const float* caseStats, float* target,
                         float* gainGrads, float* biasGrads, int numFeatures, int numCases, float scaleTargets, float scaleOutput,
@@ -594,7 +595,7 @@ int mcn_layer_norm_undo(const float* outGrads, const float* inputs, const float*
  * (e / 4, step), key seed, word e % 4, kept when that is at least floor(dropProb * 2^32)), so the gradient is the same call with
  * the same seed and step on the output's gradient.  Every call of a run takes a step of its own; layers and ranks differ in their
  * seed.  deviceStep (device memory, may be NULL) is added to step when the kernel runs, so that replays of a captured graph draw new
- * masks: advance it with mcn_counter_add.  target may be inputs itself; otherwise the two do not overlap. */
+ * masks: advance it with mcn_counter_add.  target may be inputs itself; otherwise the two do not overlap.  Up to 2^40 elements. */
 int mcn_dropout(const float* inputs, float* target, size_t numElements, float dropProb, uint64_t seed, uint64_t step,
                 const uint64_t* deviceStep, float scaleTargets, float scaleOutput, void* stream);
 /* *counter += by, on the stream (counter: 8 bytes of device memory) */
@@ -607,14 +608,17 @@ int mcn_counter_add(uint64_t* counter, uint64_t by, void* stream);
  *   caseStats (2, numCases) = max_v z, then sum_v exp(z - max);  labelLogProbs = log p[label];
  *   correctProbs = (z[label] is the max) / (number of entries at the max);
  *   costOut (device doubles, may be NULL): [0] += -sum(labelLogProbs), [1] += cases that count - sum(correctProbs).
- * A case all of whose classes are -inf has statistics (-inf, 0), log probability -inf and no gradient.  numOutputs up to 2^24 (labels
- * are fp32), numInputs and numCases up to 2^20.  Workspaces as for mcn_layer_norm; backward != 0: for both calls, 0: the cost alone. */
+ * A case all of whose classes are -inf has statistics (-inf, 0), log probability -inf and no gradient.  What the weights of a class
+ * that is taken out hold, or the inputs of a case that does not count, comes through nowhere, except for such a case's own statistics.
+ * numOutputs from 1 to 2^24 (labels are fp32), numInputs and numCases to 2^20, numInputs * numCases to 2^34.  Workspaces as for
+ * mcn_layer_norm; backward != 0: for both calls, 0: the cost alone. */
 size_t mcn_fc_logreg_workspace_bytes(int numInputs, int numOutputs, int numCases, int backward);
 int mcn_fc_logreg_cost(const float* weights, const float* inputs, const float* biases, const float* labels, float* caseStats,
                        float* labelLogProbs, float* correctProbs, int numInputs, int numOutputs, int numCases, double* costOut,
                        void* workspace, size_t workspaceBytes, void* stream);
 /* The gradients, given the caseStats that mcn_fc_logreg_cost left for the same operands.  With dz = coeff * ((v == label) - p)
- * (the sign of computeLogregSoftmaxGrad, layer_kernels.cu:287-308), computed again in pieces of the classes, each output may be NULL:
+ * (the sign of computeLogregSoftmaxGrad, layer_kernels.cu:287-308), computed again in pieces of the classes, each output may be NULL
+ * and none may overlap an operand:
  *   inputGrads (numInputs, numCases) = scaleInputTargets*inputGrads + weights^T dz,
  *   weightGrads (as weights) = scaleWeightTargets*weightGrads + scaleWeightOutput * dz inputs^T,
  *   biasGrads (numOutputs) = scaleBiasTargets*biasGrads + scaleBiasOutput * (row sums of dz). */

@@ -453,6 +453,63 @@ def test_fc_logreg_ties_and_masks(n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('bad', [np.nan, np.inf, 1e38])
+@pytest.mark.parametrize('n', [1, 6, 40, 140])
+def test_fc_logreg_masked_places_do_not_come_through(n, bad):
+    """Weights of classes that are taken out and inputs of cases that do not count: whatever they hold."""
+    d, v = 36, 500
+    w, x, b, lab = fcl_data(d, v, n, 31, masked=0.2, padded=n // 3)
+    out, off = np.isneginf(b), lab < 0
+    assert out.any()
+    w0, x0 = w.copy(), x.copy()
+    w0[out], x0[:, off] = 0, 0
+    w[out], x[:, off] = bad, bad
+    ref = fcl_ref(w0, x0, b, lab, 0.5)
+    st, lp, ok, dx, dw, db, _ = fcl_run(w, x, b, lab, 0.5)
+    keep = ~off
+    within(st[:, keep], np.stack([ref['top'], ref['tot']])[:, keep], np.stack([ref['ez'] + 2 * U * np.abs(ref['top']), ref['tot'] * ref['er']])[:, keep], 'stats')
+    within(lp, ref['logp'], 2 * ref['er'] + 4 * U * np.abs(ref['logp']), 'logp')
+    for got, k in ((dx, 'dx'), (dw, 'dw'), (db, 'db')):
+        within(got, ref[k], ref['e' + k], k)
+    assert not dx[:, off].any() and not dw[out].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n', [1, 6, 140])
+def test_fc_logreg_label_of_a_masked_class(n):
+    """log p = -inf, and the gradients of the formula: the label's one stays, and takes that class's weights with it."""
+    d, v = 36, 500
+    w, x, b, lab = fcl_data(d, v, n, 32)
+    b[100:140] = -np.inf
+    lab[::2] = 100 + np.arange(n)[::2] % 40
+    with np.errstate(invalid='ignore'):
+        ref = fcl_ref(w, x, b, lab, 0.5)
+    st, lp, ok, dx, dw, db, cost = fcl_run(w, x, b, lab, 0.5)
+    assert np.all(np.isneginf(lp[::2])) and not ok[::2].any() and np.isposinf(cost[0])
+    check_forward(ref, st, lp, ok)
+    for got, k in ((dx, 'dx'), (dw, 'dw'), (db, 'db')):
+        within(got, ref[k], ref['e' + k], k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n', [6, 140])
+@pytest.mark.parametrize('large,tiny', [(1e4, 1e-30), (1e6, 1e-20), (1.0, 1e-12)])
+def test_fc_logreg_weights_of_very_different_sizes(n, large, tiny):
+    """Groups of classes with large and tiny weights beside each other, in either order: every sum stays in range."""
+    d, v = 40, 400
+    w, x, b, lab = fcl_data(d, v, n, 33, lean=0)
+    w[:100] *= tiny
+    w[100:200] *= large
+    w[200:300] *= tiny
+    x /= large
+    ref = fcl_ref(w, x, b, lab, 0.5)
+    st, lp, ok, dx, dw, db, _ = fcl_run(w, x, b, lab, 0.5)
+    check_forward(ref, st, lp, ok)
+    for got, k in ((dx, 'dx'), (dw, 'dw'), (db, 'db')):
+        within(got, ref[k], ref['e' + k], k)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('d,v,n', [(12, 30, 9), (40, 150, 66)])
 def test_fc_logreg_gradient_against_differences(d, v, n):
     """d sum(log p) along random directions (central differences of the float64 formula, step 1e-4: 1e-6 of the magnitudes)."""
@@ -539,3 +596,164 @@ def test_head_together(captured):
     if captured:
         call('mcn_graph_destroy', exe)
     call('mcn_stream_destroy', stream)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('d,v,n', [(160, 4213, 1), (160, 1000, 128), (5000, 300, 130)])
+def test_head_two_at_once(d, v, n):
+    """The same calls on two streams at once, each with workspaces of its own: the bits of one alone."""
+    w, x, b, lab = fcl_data(d, v, n, 41)
+    g, gain, bias, _ = norm_data(d, n, 42)
+    kw, kx, kb, kl, kg, kgain, kbias = (dev(a) for a in (w, x, b, lab, g, gain, bias))
+
+    class Side:
+        def __init__(self):
+            self.stream = C.c_void_p()
+            call('mcn_stream_create', C.byref(self.stream))
+            self.ws = [need('mcn_fc_logreg_workspace_bytes', d, v, n, 1), need('mcn_layer_norm_workspace_bytes', d, n),
+                       need('mcn_layer_norm_undo_workspace_bytes', d, n)]
+            self.o = [Out(s) for s in ((d, n), (2, n), (2, n), (n,), (n,), (d, n), (v, d), (v,), (d, n), (d,), (d,))]
+
+        def run(self):
+            (cw, cs), (fw, fs), (uw, us) = self.ws
+            y, st, cst, lp, ok, dx, dw, db, dn, dg, dbi = self.o
+            s = self.stream
+            call('mcn_layer_norm', kx, kgain, kbias, y, st, d, n, EPS, fw, fs, s)
+            call('mcn_fc_logreg_cost', kw, y, kb, kl, cst, lp, ok, d, v, n, None, cw, cs, s)
+            call('mcn_fc_logreg_grad', kw, y, kb, kl, cst, dx, dw, db, d, v, n, 0.5, 0.0, 0.0, 1.0, 0.0, 1.0, cw, cs, s)
+            call('mcn_layer_norm_undo', kg, kx, kgain, st, dn, dg, dbi, d, n, 0.0, 1.0, 0.0, 1.0, 0.0, 1.0, uw, us, s)
+
+    one, two = Side(), Side()
+    one.run()
+    call('mcn_device_sync')
+    want = [o.get() for o in one.o]
+    assert all(np.isfinite(a).all() for a in want)
+    for _ in range(3):
+        for _ in range(4):
+            one.run()
+            two.run()
+        call('mcn_device_sync')
+        for side in (one, two):
+            for o, a in zip(side.o, want):
+                assert np.array_equal(o.get(), a)
+    for side in (one, two):
+        call('mcn_stream_destroy', side.stream)
+
+
+# ------------------------------------------------------------------------------------------------------------- beyond 32 bits
+class Huge(capi.DeviceBuffer):
+    """`count` zeros, of which single stretches are set and read."""
+
+    def __init__(self, count):
+        super().__init__(nbytes=count * 4)
+        self.zero()
+
+    def put(self, at, a):
+        a = np.ascontiguousarray(a, np.float32)
+        call('mcn_h2d', self.ptr + at * 4, a.ctypes.data, a.nbytes, None)
+        call('mcn_device_sync')
+
+    def take(self, at, count):
+        out = np.empty(count, np.float32)
+        call('mcn_device_sync')
+        call('mcn_d2h', out.ctypes.data, self.ptr + at * 4, out.nbytes, None)
+        call('mcn_device_sync')
+        return out
+
+
+@pytest.mark.gpu
+def test_dropout_beyond_32_bits():
+    n, tail = (1 << 32) + 1003, 4096
+    at = n - tail - (n - tail) % 4
+    count = n - at
+    big = Huge(n)
+    x = np.random.default_rng(51).standard_normal(count).astype(np.float32)
+    big.put(at, x)
+    call('mcn_dropout', big, big, n, 0.4, 5, 6, None, 0.0, 1.0, None)
+    keep = philox_words(count, 5, 6, first_quad=at // 4) >= np.uint32(int(float(np.float32(0.4)) * 2 ** 32))
+    want = np.where(keep, x / (1 - float(np.float32(0.4))), 0)
+    within(big.take(at, count), want, 2 * U * np.abs(want), 'tail')
+    assert not big.take(0, 1 << 20).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('f,n', [(300, 14500001), (66000, 65541)])  # whole columns in registers, ranges of rows
+def test_layer_norm_beyond_32_bits(f, n):
+    """Two columns at the very end and one at the start hold something (the last row, and the first, of all columns too)."""
+    assert f * n > 1 << 32
+    rng = np.random.default_rng(52)
+    rows = {r: rng.standard_normal(n).astype(np.float32) for r in (0, f - 1)}
+    gain, bias = (rng.standard_normal(f).astype(np.float32) for _ in range(2))
+    big, dx = Huge(f * n), Huge(f * n)
+    for r, a in rows.items():
+        big.put(r * n, a)
+    st = Out((2, n))
+    ws, size = need('mcn_layer_norm_workspace_bytes', f, n)
+    kg, kb = dev(gain), dev(bias)
+    call('mcn_layer_norm', big, kg, kb, dx, st, f, n, EPS, ws, size, None)
+    a = np.stack([rows[0], rows[f - 1]]).astype(np.float64)
+    mean = a.sum(0) / f
+    r = 1 / np.sqrt((((a - mean) ** 2).sum(0) + (f - 2) * mean ** 2) / f + EPS)
+    got = st.get()
+    within(got[0], mean, (sum_err(f) + 4 * U) * np.abs(a).sum(0) / f + 1e-12, 'means')
+    within(got[1], r, (sum_err(f) + 16 * U) * r, 'r')
+    bound = lambda k, v: np.abs(gain[k]) * (sum_err(f) + 32 * U) * (np.abs(v) * r) + 4 * U * np.abs(bias[k]) + 1e-12  # noqa: E731
+    for k, v in ((0, a[0] - mean), (f - 2, -mean), (f - 1, a[1] - mean)):
+        within(dx.take(k * n, n), gain[k] * (v * r) + bias[k], bound(k, np.abs(v) + np.abs(a).sum(0) / f), 'row %d' % k)
+    # backward: the outputs' gradient is the input itself, its target the matrix of outputs
+    dg, db = Out((f,)), Out((f,))
+    ws, size = need('mcn_layer_norm_undo_workspace_bytes', f, n)
+    grad = Huge(f * n)
+    for k, v in rows.items():
+        grad.put(k * n, v)
+    call('mcn_layer_norm_undo', grad, big, kg, st, dx, dg, db, f, n, 0.0, 1.0, 0.0, 1.0, 0.0, 1.0, ws, size, None)
+    mu, rs = got.astype(np.float64)
+    xh = (a - mu) * rs
+    h = np.stack([gain[0] * a[0], gain[f - 1] * a[1]]).astype(np.float64)
+    s1, s2 = h.sum(0) / f, (h * xh).sum(0) / f
+    for i, k in enumerate((0, f - 1)):
+        want = rs * (h[i] - s1 - xh[i] * s2)
+        within(dx.take(k * n, n), want, (sum_err(f) + 64 * U) * rs * (np.abs(h[i]) + np.abs(h).sum(0) / f + np.abs(xh[i]) * np.abs(h * xh).sum(0) / f) + 1e-12, 'dx of row %d' % k)
+        assert abs(dg.get()[k] - (a[i] * xh[i]).sum()) <= (sum_err(n) + 16 * U) * (np.abs(a[i]) * (np.abs(a[i]) + np.abs(mu)) * rs).sum()
+        assert abs(db.get()[k] - a[i].sum()) <= (sum_err(n) + 4 * U) * np.abs(a[i]).sum()
+    assert not dg.get()[1:f - 1].any() and not db.get()[1:f - 1].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n', [3, 70])
+def test_fc_logreg_beyond_32_bits(n):
+    """The most classes there can be; the weights of the first and the last two are not zero."""
+    d, v, coeff = 260, 1 << 24, 0.5
+    assert d * v > 1 << 32
+    rng = np.random.default_rng(53)
+    some = np.array([0, v - 2, v - 1])
+    ws_rows = rng.standard_normal((3, d)).astype(np.float32)
+    x = rng.standard_normal((d, n)).astype(np.float32)
+    lab = some[np.arange(n) % 3].astype(np.float32)
+    w, dw = Huge(d * v), Huge(d * v)
+    for r, a in zip(some, ws_rows):
+        w.put(int(r) * d, a)
+    st, lp, ok, dx, db = Out((2, n)), Out((n,)), Out((n,)), Out((d, n)), Out((v,))
+    ws, size = need('mcn_fc_logreg_workspace_bytes', d, v, n, 1)
+    kx, kl = dev(x), dev(lab)
+    call('mcn_fc_logreg_cost', w, kx, None, kl, st, lp, ok, d, v, n, None, ws, size, None)
+    call('mcn_fc_logreg_grad', w, kx, None, kl, st, dx, dw, db, d, v, n, coeff, 0.0, 0.0, 1.0, 0.0, 1.0, ws, size, None)
+    w64, x64 = ws_rows.astype(np.float64), x.astype(np.float64)
+    z = w64 @ x64
+    top = np.maximum(z.max(0), 0)
+    e = np.exp(z - top)
+    tot = (v - 3) * np.exp(-top) + e.sum(0)
+    ez = (sum_err(d) + 4 * U) * (np.abs(w64) @ np.abs(x64)).max(0)
+    er = 2 * ez + sum_err(v) + 16 * U
+    zl = z[np.arange(n) % 3, np.arange(n)]
+    within(lp.get(), zl - top - np.log(tot), 2 * er + 4 * U * np.abs(zl - top - np.log(tot)), 'logp')
+    dz = -e / tot
+    dz[np.arange(n) % 3, np.arange(n)] += 1
+    dz *= coeff
+    edz = e / tot * er + 4 * U * np.abs(dz) + 2.0 ** -43
+    within(dx.get(), w64.T @ dz, np.abs(w64).T @ edz + 16 * U * np.abs(w64).T @ np.abs(dz), 'dx')
+    rest = -coeff * np.exp(-top) / tot  # dz of every other class
+    for i, r in enumerate(some):
+        within(dw.take(int(r) * d, d), x64 @ dz[i], np.abs(x64) @ edz[i] + (sum_err(n) + 2 * U) * np.abs(x64) @ np.abs(dz[i]), 'dw of class %d' % r)
+        assert abs(db.get()[r] - dz[i].sum()) <= edz[i].sum() + sum_err(n) * np.abs(dz[i]).sum()
+    within(dw.take((v - 3) * d, d), x64 @ rest, np.abs(x64) @ (np.abs(rest) * er + 2.0 ** -43) + (sum_err(n) + 2 * U) * np.abs(x64) @ np.abs(rest), 'dw before them')

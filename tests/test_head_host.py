@@ -12,7 +12,7 @@ ccn_loader.load()
 from cuda_convnet_amd import capi  # noqa: E402
 
 EINVAL, EWORKSPACE = -1, -3
-P = [0x10000 * (i + 1) for i in range(10)]
+P = [(i + 1) << 32 for i in range(10)]
 BIG = 1 << 40
 
 
@@ -28,7 +28,7 @@ def norm(**k):
     return rc('mcn_layer_norm', a['x'], a['gain'], a['bias'], a['y'], a['stats'], a['f'], a['n'], a['eps'], a['ws'], a['size'], None)
 
 
-@pytest.mark.parametrize('k', [dict(x=None), dict(y=None), dict(f=0), dict(n=0), dict(f=-3), dict(n=-1), dict(f=(1 << 28) + 1),
+@pytest.mark.parametrize('k', [dict(x=None), dict(y=None), dict(f=0), dict(n=0), dict(f=-3), dict(n=-1), dict(f=(1 << 26) + 1), dict(n=(1 << 26) + 1), dict(y=P[0] + 4),
                                dict(eps=0.0), dict(eps=-1.0), dict(eps=math.nan), dict(ws=P[5] + 4)])
 def test_layer_norm_refuses(k):
     code, msg = norm(**k)
@@ -51,7 +51,7 @@ def undo(**k):
 
 
 @pytest.mark.parametrize('k', [dict(g=None), dict(x=None), dict(stats=None), dict(dx=None, dg=None, db=None), dict(f=0), dict(n=0),
-                               dict(dx=P[0]), dict(dx=P[1]), dict(ws=P[7] + 8)])
+                               dict(dx=P[0]), dict(dx=P[1]), dict(dx=P[0] - 8), dict(dx=P[1] + 124), dict(ws=P[7] + 8)])
 def test_layer_norm_undo_refuses(k):
     code, msg = undo(**k)
     assert code == EINVAL and 'layerNormUndo' in msg
@@ -73,6 +73,7 @@ def test_dropout_refuses_pointers():
     assert rc('mcn_dropout', None, P[1], 16, 0.5, 1, 2, None, 0.0, 1.0, None)[0] == EINVAL
     assert rc('mcn_dropout', P[0], None, 16, 0.5, 1, 2, None, 0.0, 1.0, None)[0] == EINVAL
     assert rc('mcn_dropout', P[0], P[0] + 16, 16, 0.5, 1, 2, None, 0.0, 1.0, None)[0] == EINVAL  # overlaps in part
+    assert rc('mcn_dropout', P[0], P[1], (1 << 62) + 5, 0.5, 1, 2, None, 0.0, 1.0, None)[0] == EINVAL  # more than there is memory for
     assert rc('mcn_dropout', P[0], P[1], 0, 0.5, 1, 2, None, 0.0, 1.0, None)[0] == 0  # nothing to do
     assert rc('mcn_counter_add', None, 1, None)[0] == EINVAL
 
@@ -90,7 +91,8 @@ def grad(**k):
               1.0, 0.0, 0.0, 1.0, 0.0, 1.0, a['ws'], a['size'], None)
 
 
-SIZES = [dict(d=0), dict(v=0), dict(n=0), dict(n=-5), dict(v=(1 << 24) + 1), dict(d=(1 << 20) + 1), dict(n=(1 << 20) + 1), dict(ws=P[7] + 4)]
+SIZES = [dict(d=0), dict(v=0), dict(n=0), dict(n=-5), dict(v=(1 << 24) + 1), dict(d=(1 << 20) + 1), dict(n=(1 << 20) + 1),
+         dict(d=1 << 18, n=(1 << 16) + 1), dict(ws=P[7] + 4)]
 
 
 @pytest.mark.parametrize('k', SIZES + [dict(w=None), dict(x=None), dict(l=None), dict(st=None), dict(lp=None), dict(ok=None)])
@@ -100,7 +102,8 @@ def test_fc_logreg_cost_refuses(k):
 
 
 @pytest.mark.parametrize('k', SIZES + [dict(w=None), dict(x=None), dict(l=None), dict(st=None), dict(dx=None, dw=None, db=None),
-                                       dict(dx=P[1]), dict(dw=P[0])])
+                                       dict(dx=P[1]), dict(dx=P[1] + 8), dict(dx=P[4] - 4), dict(dw=P[0]), dict(dw=P[0] - 64), dict(dw=P[3] - 4),
+                                       dict(db=P[2]), dict(db=P[2] + 396), dict(db=P[4] + 60)])
 def test_fc_logreg_grad_refuses(k):
     code, msg = grad(**k)
     assert code == EINVAL and 'fcLogregGrad' in msg
