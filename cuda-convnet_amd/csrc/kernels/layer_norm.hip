@@ -419,7 +419,6 @@ __global__ __launch_bounds__(T_SPLIT) void k_ln_undo_split_sums(const float* __r
     const Cols<VW> mu = load_cols<VW>(caseStats + p.col, p.cnt), rs = load_cols<VW>(caseStats + s.N + p.col, p.cnt);
     float v[2 * VW] = {};
     const int steps = (max(r1 - r0, 0) + p.rowLanes - 1) / p.rowLanes;  // the same for every lane: the shuffles below need whole groups
-#pragma unroll 4
     for (int i = 0; i < steps; i++) {
         const int r = r0 + p.rl + i * p.rowLanes;
         float sg = 0.f, sb = 0.f;
@@ -551,6 +550,7 @@ struct Plan {
     int blocks;               // backward, whole
     Split split;
 };
+constexpr size_t CACHED_BYTES = (size_t)128 << 20;  // a matrix that stays in the last-level cache
 constexpr size_t SMALL_BYTES = (size_t)32 << 20;  // both matrices of a backward pass: the rows are summed by blocks of their own
 constexpr int FWD_ROWS = 16, BWD_ROWS = 8;       // rows a thread of the whole kernels holds
 // rows: FWD_ROWS or BWD_ROWS
@@ -563,17 +563,23 @@ Plan ln_plan(int F, int N, int rows) {
     while (p.vw == 4 && lg > 0 && (divup(lanes, 1 << lg) < CUS || ((size_t)F << lg) > (size_t)most)) lg--;
     p.logLanes = lg;
     p.tiles = divup(lanes, 1 << lg);
-    // one lane a row (16 bytes) only pays where the matrix is small
-    p.whole = ((size_t)F << lg) <= (size_t)most && (lg > 0 || p.tiles <= CUS);
+    // Two lanes a row (32 bytes) read every cache line from several tiles, which pays while the cache holds the matrix (forward, whole /
+    // split: 2048 x 8192, 67 MB, 27 / 37 us; 2048 x 32768, 268 MB, 223 / 164 us), one lane only where it is small.
+    p.whole = ((size_t)F << lg) <= (size_t)most && (lg > 1 || (lg == 1 ? (size_t)F * N * 4 <= CACHED_BYTES : p.tiles <= CUS));
     p.blocks = std::min(divup(p.tiles, 8) * 8, 4 * CUS);
     Split& s = p.split;
     s.F = F;
     s.N = N;
     s.logLanes = 0;
     while ((1 << s.logLanes) < lanes && s.logLanes < 4) s.logLanes++;
-    s.colTiles = divup(lanes, 1 << s.logLanes);
-    const int rowLanes = T_SPLIT >> s.logLanes;
-    s.splits = std::max(1, std::min({64, JOIN * rowLanes, divup(4 * CUS, s.colTiles), divup(F, 4 * rowLanes)}));
+    // split: 256 bytes of a row (16 lanes), fewer while that leaves CUs without a block (9075 x 128 forward: 11.6 -> 9.7 us; 100000 x 64:
+    // 75 -> 28 us), and up to 16 blocks a CU (4096 x 16384, both passes: 4 a CU 457 us, 16 438 us)
+    for (;; s.logLanes--) {
+        s.colTiles = divup(lanes, 1 << s.logLanes);
+        const int rowLanes = T_SPLIT >> s.logLanes;
+        s.splits = std::max(1, std::min({JOIN * rowLanes, divup(16 * CUS, s.colTiles), divup(F, 4 * rowLanes)}));
+        if (s.logLanes <= 2 || s.colTiles * s.splits >= CUS) break;
+    }
     s.rowsPerSplit = divup(F, s.splits);
     s.splits = divup(F, s.rowsPerSplit);
     return p;

@@ -85,7 +85,7 @@ def norm_data(f, n, seed, offset=2.0):
 NORM_SHAPES = [(1, 1), (1, 5), (2, 1), (3, 64), (5, 3), (16, 16), (63, 65), (64, 4), (160, 128), (160, 37), (257, 12), (512, 1),
                (512, 128), (1000, 31), (1025, 8), (2048, 20), (2049, 64), (4096, 36), (4097, 16), (9075, 5), (9075, 128), (40000, 1),
                (20000, 4), (33, 5000), (128, 3010), (7, 20001),
-               (512, 8260), (513, 8263), (4100, 1030)]
+               (512, 8260), (513, 8263), (4100, 1030), (30000, 20), (30001, 100), (70000, 3)]
 
 
 @pytest.mark.gpu
