@@ -689,6 +689,10 @@ void LayerNormLayer::bpropWeights(float* v, int, PassType pt) {
 DropoutLayer::DropoutLayer(ConvNet* net, const Params& p) : Layer(net, p) {
     _prob = (float)pfloat(p, "dropout");
     _seed = (uint64_t)pint(p, "seed");
+    _hSteps = pmat(p, "steps");
+    if (_hSteps.size() != 3) throw NetError("layer '" + _name + "': steps must have three entries");
+    for (int i = 0; i < 3; i++)
+        if (!(_hSteps.data[i] >= 0.f && _hSteps.data[i] < 1048576.f)) throw NetError("layer '" + _name + "': steps must lie in [0, 2^20)");
     if (!(_prob >= 0.f && _prob < 1.f)) throw NetError("layer '" + _name + "': dropout must be in [0, 1)");
 }
 
@@ -702,7 +706,22 @@ void DropoutLayer::allocate(int maxCases) {
     void* q = nullptr;
     chk(mcn_alloc(&q, sizeof(uint64_t)), "alloc");
     _step = (uint64_t*)q;
-    chk(mcn_memset(_step, 0, sizeof(uint64_t), _net->mainStream()), "dropout step");
+    copyToGPU();
+}
+
+void DropoutLayer::copyToGPU() {
+    if (!_step) return;
+    uint64_t step = 0;
+    for (int i = 2; i >= 0; i--) step = (step << 20) + (uint64_t)_hSteps.data[i];
+    chk(mcn_h2d(_step, &step, sizeof(step), _net->stream()), "dropout step");
+    chk(mcn_stream_sync(_net->stream()), "sync");
+}
+
+void DropoutLayer::copyToCPU() {
+    uint64_t step = 0;
+    chk(mcn_d2h(&step, _step, sizeof(step), _net->stream()), "dropout step");
+    chk(mcn_stream_sync(_net->stream()), "sync");
+    for (int i = 0; i < 3; i++) _hSteps.data[i] = (float)(step >> 20 * i & 0xFFFFF);
 }
 
 // every rank masks its own share of a minibatch by its own numbers

@@ -263,10 +263,13 @@ class DropoutLayer : public Layer {
     DropoutLayer(ConvNet* net, const Params& p);
     ~DropoutLayer() override;
     void allocate(int maxCases) override;
+    void copyToCPU() override;
+    void copyToGPU() override;
    protected:
     void fpropActs(int, float, PassType) override;
     void bpropActs(float* v, int, float, PassType) override;
     uint64_t rankSeed() const;
+    HostMat _hSteps;  // the step, three digits in base 2^20
     float _prob;
     uint64_t _seed;
     uint64_t* _step = nullptr;

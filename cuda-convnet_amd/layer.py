@@ -331,6 +331,7 @@ def _parse_dropout(name, cfg, prev, ctx):
     _check(0 <= dic['dropout'] < 1, "Layer '%s': parameter 'dropout' must be in [0, 1)" % name)
     seed = cfg.get_int(name, 'seed', default=-1)
     dic['seed'] = int(ctx.rng.integers(1 << 62)) if seed < 0 else seed
+    dic['steps'] = np.zeros((1, 3), dtype=np.float32)  # minibatches drawn for so far, in base 2^20: a checkpoint goes on with new masks
     dic['usesActs'] = dic['usesInputs'] = False
     dic['forceOwnActs'] = prev[dic['inputs'][0]]['type'] == 'data'  # never in the data batch itself
     if prev[dic['inputs'][0]].get('geom'):

@@ -186,6 +186,42 @@ def test_masks_change_from_step_to_step_and_test_passes_have_none():
         assert np.array_equal(out['norm1'], out['drop1']) and np.isfinite(out['norm1']).all()
 
 
+def test_a_resumed_run_goes_on_with_the_masks():
+    """Four minibatches at once, or two, a checkpoint's layers, and two: the same bits."""
+    dp, L = net(32)
+    randomise(L)
+    data = dp.get_next_batch()[2]
+
+    def train(layers, batches):
+        with Native(layers, 32) as lib:
+            for _ in range(batches):
+                lib.startBatch(data, 0)
+                lib.finishBatch()
+            lib.syncWithHost()
+
+    whole, parts = copy.deepcopy(L), copy.deepcopy(L)
+    train(whole, 4)
+    train(parts, 2)
+    drop = [l for l in parts if l['type'] == 'dropout'][0]
+    assert drop['steps'].tolist() == [[2, 0, 0]]
+    drop['steps'][:] = 1048575, 7, 1  # (digits carry)
+    train(parts, 0)
+    assert drop['steps'].tolist() == [[1048575, 7, 1]]
+    more = copy.deepcopy(parts)
+    train(more, 1)
+    assert [l['steps'].tolist() for l in more if l['type'] == 'dropout'] == [[[0, 8, 1]]]
+    drop['steps'][:] = 2, 0, 0
+    parts = copy.deepcopy(parts)
+    train(parts, 2)
+    for a, b in zip(whole, parts):
+        for k in ('weights', 'weightsInc'):
+            for p, q in zip(a.get(k, []), b.get(k, [])):
+                assert np.array_equal(p, q), (a['name'], k)
+        for k in ('biases', 'biasesInc', 'steps'):
+            if k in a:
+                assert np.array_equal(a[k], b[k]), (a['name'], k)
+
+
 def cost64(q, x, labels, scale, eps):
     """-sum(log p[label]) of the net, float64; q: the six weight and bias matrices."""
     h = np.maximum(q[0].T @ x + q[1], 0)
