@@ -264,6 +264,45 @@ def test_gradient_check_reports_what_its_steps_allow():
         assert abs(r[3] - want) <= 0.01 + noise, (r, want, noise)
 
 
+def test_norm_with_a_neuron_in_a_residual_sum(tmp_path):
+    """fc1 + dropout(relu(norm(fc1))): every layer's gradient arrives added onto another's; norms of the gradients against differences of
+    the float64 formula (steps of 1e-6; a kink that lies within them is met by a negligible share of the entries)."""
+    text = open(CFG).read().replace('eps=0.001', 'eps=0.001\nneuron=relu').replace('[id]', '[sum]\ntype=eltsum\ninputs=drop1,fc1\ncoeffs=1,1\n\n[id]')
+    text = text.replace('type=classifier\noutputs=10\ninputs=drop1', 'type=classifier\noutputs=10\ninputs=sum')
+    path = tmp_path / 'sum.cfg'
+    path.write_text(text)
+    dp, L = net(32, str(path))
+    randomise(L)
+    data = dp.get_next_batch()[2]
+    x, labels = data[0].astype(np.float64), data[1].ravel().astype(int)
+    by = {l['name']: l for l in L}
+    col = lambda a: a.astype(np.float64).reshape(-1, 1)  # noqa: E731
+    q = [by['fc1']['weights'][0].astype(np.float64), col(by['fc1']['biases']), col(by['norm1']['weights'][0]), col(by['norm1']['biases']),
+         by['id']['weights'][0].astype(np.float64), col(by['id']['biases'])]
+    scale = kept(40 * 32, 0.4, 77, 0).reshape(40, 32) / (1 - float(np.float32(0.4)))
+
+    def cost():
+        h = np.maximum(q[0].T @ x + q[1], 0)
+        d = np.maximum(q[2] * (h - h.mean(0)) / np.sqrt(h.var(0) + 0.001) + q[3], 0) * scale + h
+        z = q[4].T @ d + q[5]
+        top = z.max(0)
+        return (top + np.log(np.exp(z - top).sum(0)) - z[labels, np.arange(32)]).sum()
+
+    with Native(L, 32) as lib:
+        res = lib.checkGradients(data, 0, 1)
+    assert [r[0].split()[0] for r in res] == ['fc1', 'fc1', 'norm1', 'norm1', 'id', 'id']
+    for k, r in enumerate(res):
+        grad, h = np.zeros_like(q[k]), 1e-6
+        for i in np.ndindex(*q[k].shape):
+            keep = q[k][i]
+            q[k][i] = keep + h
+            up = cost()
+            q[k][i] = keep - h
+            grad[i] = (up - cost()) / (2 * 32 * h)
+            q[k][i] = keep
+        assert abs(r[1] - np.linalg.norm(grad)) <= 1e-3 * np.linalg.norm(grad), r
+
+
 def test_classifier_refusals():
     dp, L = net(32)
     idx = {l['name']: i for i, l in enumerate(L)}
