@@ -7,6 +7,11 @@
 #include <algorithm>
 #include "common.h"
 
+// Every product is rounded before it is added, as in the formulas written out operation by operation: with two or three features the
+// gradient is a difference of nearly equal numbers, and a product left unrounded on one side of it shows.  (All kernels here wait for
+// memory: no time is lost.)
+#pragma clang fp contract(off)
+
 namespace {
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));

@@ -225,6 +225,32 @@ def test_layer_norm_undo_against_differences(f, n):
         assert abs((got[k] * d[k]).sum() - want) <= (bounds[k] * np.abs(d[k])).sum() + 1e-6 * (np.abs(got[k] * d[k])).sum()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('n', [1, 4, 7, 3755])
+def test_layer_norm_of_two_features_rounds_like_the_formula(n):
+    """With two features h - mean(h) - xh mean(h xh) cancels down to rounding errors: the same ones as of the formula in float32, one
+    operation after the other (two terms have one order), so the same bits."""
+    f = np.float32
+    rng = np.random.default_rng(9)
+    x, g = rng.standard_normal((2, n)).astype(f) * 2 + 1, rng.standard_normal((2, n)).astype(f)
+    gain, bias = (1 + 0.2 * rng.standard_normal(2)).astype(f), rng.standard_normal(2).astype(f)
+    mean = (x[0] + x[1]) / f(2)
+    d = x - mean
+    r = f(1) / np.sqrt((d[0] * d[0] + d[1] * d[1]) / f(2) + f(EPS))
+    xh = d * r
+    h = gain[:, None] * g
+    m1, m2 = (h[0] + h[1]) / f(2), (h[0] * xh[0] + h[1] * xh[1]) / f(2)
+    y, st, dx = Out((2, n)), Out((2, n)), Out((2, n))
+    ws, size = need('mcn_layer_norm_workspace_bytes', 2, n)
+    wu, sizeu = need('mcn_layer_norm_undo_workspace_bytes', 2, n)
+    kx, kg, kgain, kbias = dev(x), dev(g), dev(gain), dev(bias)
+    call('mcn_layer_norm', kx, kgain, kbias, y, st, 2, n, EPS, ws, size, None)
+    call('mcn_layer_norm_undo', kg, kx, kgain, st, dx, None, None, 2, n, 0.0, 1.0, 0.0, 1.0, 0.0, 1.0, wu, sizeu, None)
+    assert np.array_equal(st.get(), np.stack([mean, r]))
+    assert np.array_equal(y.get(), gain[:, None] * xh + bias[:, None])
+    assert np.array_equal(dx.get(), r * ((h - m1) - xh * m2))
+
+
 # ------------------------------------------------------------------------------------------------------------- dropout
 def philox_words(count, seed, step, first_quad=0):
     """Philox-4x32, ten rounds, in Python integers' width by uint64 arithmetic."""
