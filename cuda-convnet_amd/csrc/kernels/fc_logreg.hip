@@ -18,8 +18,13 @@ constexpr int PIECE_MB = 128;  // fragments of a piece; 512 x 100000 x 1024, bot
 struct NarrowArgs {
     const float *W, *X, *bias, *labels;
     int D, V, N;
-    float* part;         // [tiles][3][N]
-    float* labelLogits;  // [N]
+    int v0, rows;        // the piece: classes [v0, v0 + rows)
+    float* part;         // forward: [tiles][3][N]
+    float* labelLogits;  // forward: [N]
+    const float* stats;  // backward
+    char* dz;            // backward: dz / coeff, split into fragments of (rows = cases, k = classes) as the wide path's
+    float* dbPart;       // backward: [V], row sums of dz / coeff
+    int Kv;
 };
 
 // Statistics of a set of logits: the max, the entries at the max, and the sum of exp(z - max) over the OTHER entries.  The three are
@@ -39,6 +44,16 @@ __device__ __forceinline__ void stat_join(Stat& a, float m, float rest, float cn
         a.rest += (rest + cnt) * (m == -INFINITY ? 1.f : expf(m - a.m));
     }
 }
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef __fp16 fp16x4 __attribute__((__vector_size__(4 * sizeof(__fp16))));  // (the type the transposing read is declared with)
+
+constexpr int FRAG = 1024, PAIR = 2 * FRAG;  // bytes of a fragment, of its two pieces
+constexpr int TILE = 128;                    // columns of a product's tile
+constexpr float LO = 2048.f;                 // scale of the low piece
+constexpr int DZ_EXP = 14;                   // |dz / coeff| <= 1
+constexpr int EXP_ZERO = 1 << 20;            // a group of zeros: any scale will do
 
 __device__ __forceinline__ bool label_of(float l, int V, int& label) {
     const bool ok = l >= 0.f && l < (float)V;  // (false for a NaN)
@@ -60,14 +75,17 @@ __device__ __forceinline__ float exp_neg(float x) {
 // takes 16 RG classes, its four waves a quarter of the features each (16 at a time: a lane reads 16 bytes of its class's row, and the
 // four matrix instructions that follow take one feature of every lane's four); their sums are joined in LDS.  RG = 1 while the classes
 // do not fill the chip, 4 beyond, where it keeps the number of tiles to join down.
-template <int NB, int RG>
+// Backward, the logits are computed again in the same way, and so to the same bits: where a case is all but certain, 1 - p of its label
+// is a difference that other roundings of z would drown.
+template <bool BWD, int NB, int RG>
 __global__ __launch_bounds__(256) void k_fcl_narrow(NarrowArgs p) {
     __shared__ f32x4 red[4][RG][NB][64];
+    __shared__ float rowSum[4][16 * RG];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int vBase = blockIdx.x * 16 * RG;
     const float* rowPtr[RG];
 #pragma unroll
-    for (int q = 0; q < RG; q++) rowPtr[q] = p.W + (size_t)min(vBase + q * 16 + c, p.V - 1) * p.D;  // (a class behind the last one: read and not used)
+    for (int q = 0; q < RG; q++) rowPtr[q] = p.W + (size_t)(p.v0 + min(vBase + q * 16 + c, p.rows - 1)) * p.D;  // (a class behind the last one: read and not used)
     f32x4 acc[RG][NB] = {};
     const int steps = (p.D + 15) / 16;
     for (int t = wave; t < steps; t += 4) {
@@ -101,22 +119,58 @@ __global__ __launch_bounds__(256) void k_fcl_narrow(NarrowArgs p) {
 #pragma unroll
         for (int n = 0; n < NB; n++) red[wave][q][n][lane] = acc[q][n];
     __syncthreads();
-    if (wave >= NB) return;  // a wave: 16 cases
-    const int n = wave * 16 + c;
-    int label = -1;
-    if (n < p.N) label_of(p.labels[n], p.V, label);
     float z[RG][4], m = -INFINITY;
+    const int n = wave * 16 + c;  // a wave: 16 cases
+    int label = -1;
+    if (wave < NB) {
+        if (n < p.N) label_of(p.labels[n], p.V, label);
 #pragma unroll
-    for (int q = 0; q < RG; q++) {
-        const f32x4 s = (red[0][q][wave][lane] + red[1][q][wave][lane]) + (red[2][q][wave][lane] + red[3][q][wave][lane]);
+        for (int q = 0; q < RG; q++) {
+            const f32x4 s = (red[0][q][wave][lane] + red[1][q][wave][lane]) + (red[2][q][wave][lane] + red[3][q][wave][lane]);
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int v = vBase + q * 16 + g * 4 + r;
-            const float bv = v < p.V ? (p.bias ? p.bias[v] : 0.f) : -INFINITY;
-            z[q][r] = bv == -INFINITY ? -INFINITY : s[r] + bv;  // (a class that is taken out, whatever its weights hold)
-            m = fmaxf(z[q][r], m);
+            for (int r = 0; r < 4; r++) {
+                const int v = vBase + q * 16 + g * 4 + r;
+                const float bv = v < p.rows ? (p.bias ? p.bias[p.v0 + v] : 0.f) : -INFINITY;
+                z[q][r] = bv == -INFINITY ? -INFINITY : s[r] + bv;  // (a class that is taken out, whatever its weights hold)
+                m = fmaxf(z[q][r], m);
+            }
         }
     }
+    if constexpr (BWD) {
+        float M = 0.f, S = 0.f;
+        if (label >= 0) {
+            M = p.stats[n];
+            S = p.stats[p.N + n];
+        }
+        const bool counts = S != 0.f;  // (no label, or no class left: nothing; a NaN goes on)
+        const float inv = counts ? 1.f / S : 0.f;
+        char* out = p.dz + ((size_t)wave * p.Kv + vBase / 32) * PAIR + lane * 8;
+        char* rest = out + (size_t)4 * p.Kv * PAIR;  // cases 64 .. 127 of the tile: there are none
+#pragma unroll
+        for (int q = 0; q < RG; q++) {
+            f16x4 hi = {}, lo = {};
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                float t = 0.f;
+                if (wave < NB && counts) t = (label == p.v0 + vBase + q * 16 + g * 4 + r ? 1.f : 0.f) - exp_neg(z[q][r] - M) * inv;
+                const float y = t * (float)(1 << DZ_EXP);
+                hi[r] = (_Float16)y;
+                lo[r] = (_Float16)((y - (float)hi[r]) * LO);
+                for (int o = 1; o < 16; o <<= 1) t += __shfl_xor(t, o, 64);
+                if (c == 0) rowSum[wave][q * 16 + g * 4 + r] = t;
+            }
+            const int at = ((vBase / 16 + q) & 1) * 512 + (((vBase & 16) + q * 16) >> 5) * PAIR;
+            *reinterpret_cast<f16x4*>(out + at) = hi;
+            *reinterpret_cast<f16x4*>(out + at + FRAG) = lo;
+            *reinterpret_cast<f16x4*>(rest + at) = (f16x4){};
+            *reinterpret_cast<f16x4*>(rest + at + FRAG) = (f16x4){};
+        }
+        __syncthreads();
+        if (p.dbPart && tid < 16 * RG && vBase + tid < p.rows)
+            p.dbPart[p.v0 + vBase + tid] = (rowSum[0][tid] + rowSum[1][tid]) + (rowSum[2][tid] + rowSum[3][tid]);
+        return;
+    }
+    if (wave >= NB) return;
     for (int o = 16; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
     const float from = m == -INFINITY ? 0.f : m;
     float rest = 0.f, cnt = 0.f;
@@ -254,16 +308,6 @@ __global__ __launch_bounds__(256) void k_fcl_cost(const float* __restrict__ labe
 // is the fragments' ROW, a transposing LDS read (ds_read_b64_tr_b16) gives lane (k = 16 h + c, g) rows 4 g .. 4 g + 3 of two fragments.
 // Both read 512 contiguous bytes a wave, without conflicts, and in both a lane's eight entries are 4 g + j and 16 + 4 g + j of the step's
 // 32, so that every pairing sums the same terms.  So W and dz are each stored once, and serve two products.
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-typedef __fp16 fp16x4 __attribute__((__vector_size__(4 * sizeof(__fp16))));  // (the type the transposing read is declared with)
-
-constexpr int FRAG = 1024, PAIR = 2 * FRAG;  // bytes of a fragment, of its two pieces
-constexpr int TILE = 128;                    // columns of a product's tile
-constexpr float LO = 2048.f;                 // scale of the low piece
-constexpr int DZ_EXP = 14;                   // |dz / coeff| <= 1
-constexpr int EXP_ZERO = 1 << 20;            // a group of zeros: any scale will do
-
 // the power of two that brings a group of largest magnitude m to [2^14, 2^15); infinities and NaNs stay as they are
 __device__ __forceinline__ int scale_exp(float m) { return m > 0.f && m < INFINITY ? 14 - ilogbf(m) : 0; }
 __device__ __forceinline__ float max_or_nan(float m, float v) { return v > m || v != v ? v : m; }
@@ -1025,9 +1069,9 @@ struct WidePlan {
                                                  // writes every slab
     size_t classExp, caseExp, featExp, xByCase, xByFeat, wByClass, dz, dbPart, slabs, part, labelLogits, total;
 };
-// When the packed operands pay for the cost alone (us, narrow / wide).  512 x 10575: 16 cases 16 / 34, 64 cases 26 / 35; 512 x 100000:
-// 56 / 145, 121 / 147.  The gradients always take them: 512 x 10575, one case 52 us, 64 cases 47 us (fp32 products of a dz of their own
-// layout: 50 and 60 us).
+// When the packed operands pay for the logits (us of a whole cost call, narrow / wide).  512 x 10575: 16 cases 16 / 34, 64 cases 26 / 35;
+// 512 x 100000: 56 / 145, 121 / 147.  Both calls go by the number of cases alone: the gradients' logits are the cost's, to the bit.
+// The other products of the gradients always take them (512 x 10575: one case 50 us, 16 cases 43 us, 64 cases 49 us).
 bool wide_cost_usable(int N) { return N > NARROW; }
 
 size_t al256(size_t b) { return (b + 255) / 256 * 256; }
@@ -1068,6 +1112,23 @@ WidePlan wide_plan(int D, int V, int N, bool bwd) {
     }
     p.total = at;
     return p;
+}
+
+int narrow_groups(int rows) { return rows > 16 * 1024 ? 4 : 1; }
+int narrow_tiles(int rows) { return divup(rows, 16 * narrow_groups(rows)); }
+// blocks: narrow_tiles(rows) forward, all of the piece's packed classes backward
+template <bool BWD>
+void launch_narrow(const NarrowArgs& p, int blocks, hipStream_t s) {
+#define NARROW_LAUNCH(NB)                                                                                                    \
+    if (narrow_groups(p.rows) == 1) MCN_LAUNCH((k_fcl_narrow<BWD, NB, 1>), dim3(blocks), dim3(256), 0, s, p); \
+    else MCN_LAUNCH((k_fcl_narrow<BWD, NB, 4>), dim3(blocks), dim3(256), 0, s, p)
+    switch (divup(p.N, 16)) {
+        case 1: NARROW_LAUNCH(1); break;
+        case 2: NARROW_LAUNCH(2); break;
+        case 3: NARROW_LAUNCH(3); break;
+        default: NARROW_LAUNCH(4); break;
+    }
+#undef NARROW_LAUNCH
 }
 
 template <bool BWD>
@@ -1144,7 +1205,11 @@ int wide_grad(const float* W, const float* X, const float* bias, const float* la
     a.dz = ws + q.dz;
     a.dbPart = dB ? (float*)(ws + q.dbPart) : nullptr;
     float* slabs = (float*)(ws + q.slabs);
+    const bool narrow = !wide_cost_usable(N);  // (the forward call's logits, to the bit)
     PackArgs pack = pack_args(q, X, labels, D, V, N, dW != nullptr, ws);
+    if (narrow) pack.caseBlocks = 0;
+    NarrowArgs few = {W, X, bias, labels, D, V, N};
+    few.stats = stats; few.dz = a.dz; few.dbPart = a.dbPart;
     GradArgs t = {};
     t.xByFeat = ws + q.xByFeat; t.dz = ws + q.dz; t.wByClass = ws + q.wByClass;
     t.featExp = (const int*)(ws + q.featExp); t.classExp = (const int*)(ws + q.classExp);
@@ -1154,7 +1219,14 @@ int wide_grad(const float* W, const float* X, const float* bias, const float* la
     t.scaleOutput = scaleWeightOutput * coeff;
     for (int v0 = 0; v0 < V; v0 += q.rows) {
         const TileKind kind = wide_piece(q, a, pack, W, D, v0, s);
-        launch_logits<true>(kind, a, s);
+        if (narrow) {
+            few.v0 = v0;
+            few.rows = a.rows;
+            few.Kv = a.Kv;
+            launch_narrow<true>(few, a.Kv * 2 / narrow_groups(a.rows), s);
+        } else {
+            launch_logits<true>(kind, a, s);
+        }
         // (a short last piece has fewer, not shorter, shares of the input gradient: each adds to its slab)
         t.kPerSplit = a.Kv == q.Kv ? q.kPerSplit : std::max(8, divup(a.Kv, q.splits));
         t.inputBlocks = dX ? divup(a.Kv, t.kPerSplit) * q.nTiles * q.dTiles : 0;
@@ -1181,28 +1253,11 @@ bool fcl_sizes_ok(int D, int V, int N) {
 }
 
 size_t al16b(size_t b) { return (b + 15) / 16 * 16; }
-int narrow_groups(int V) { return V > 16 * 1024 ? 4 : 1; }
-int narrow_tiles(int V) { return divup(V, 16 * narrow_groups(V)); }
 size_t fcl_cost_bytes(int D, int V, int N) {
     if (wide_cost_usable(N)) return wide_plan(D, V, N, false).total;
     return al16b((size_t)narrow_tiles(V) * 3 * N * sizeof(float)) + al16b((size_t)N * sizeof(float));
 }
 size_t fcl_grad_bytes(int D, int V, int N) { return wide_plan(D, V, N, true).total; }
-
-void launch_narrow(const NarrowArgs& p, hipStream_t s) {
-    const int groups = narrow_groups(p.V);
-    const dim3 grid(narrow_tiles(p.V)), block(256);
-#define NARROW_LAUNCH(NB)                                                                 \
-    if (groups == 1) MCN_LAUNCH((k_fcl_narrow<NB, 1>), grid, block, 0, s, p); \
-    else MCN_LAUNCH((k_fcl_narrow<NB, 4>), grid, block, 0, s, p)
-    switch (divup(p.N, 16)) {
-        case 1: NARROW_LAUNCH(1); break;
-        case 2: NARROW_LAUNCH(2); break;
-        case 3: NARROW_LAUNCH(3); break;
-        default: NARROW_LAUNCH(4); break;
-    }
-#undef NARROW_LAUNCH
-}
 
 int fcl_check(const char* what, const void* ws, size_t have, size_t need) {
     if (!ws || have < need) {
@@ -1232,10 +1287,10 @@ MCN_API int mcn_fc_logreg_cost(const float* weights, const float* inputs, const 
         if (int rc = wide_cost(weights, inputs, biases, labels, caseStats, labelLogProbs, correctProbs, numInputs, numOutputs, numCases, (char*)workspace, s)) return rc;
     } else {
         const int tiles = narrow_tiles(numOutputs);
-        NarrowArgs p = {weights, inputs, biases, labels, numInputs, numOutputs, numCases};
+        NarrowArgs p = {weights, inputs, biases, labels, numInputs, numOutputs, numCases, 0, numOutputs};
         p.part = (float*)workspace;
         p.labelLogits = (float*)((char*)workspace + al16b((size_t)tiles * 3 * numCases * sizeof(float)));
-        launch_narrow(p, s);
+        launch_narrow<false>(p, tiles, s);
         MCN_LAUNCH(k_fcl_join, dim3(divup(numCases, 16)), dim3(1024), 0, s, p.part, p.labelLogits, labels, caseStats, labelLogProbs, correctProbs,
                    numOutputs, numCases, tiles);
     }

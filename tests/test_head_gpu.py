@@ -325,11 +325,11 @@ def test_dropout_statistics():
 
 
 # ------------------------------------------------------------------------------------------------------------- classifier cost
-def fcl_data(d, v, n, seed, masked=0.0, padded=0, lean=6.0):
+def fcl_data(d, v, n, seed, masked=0.0, padded=0, lean=6.0, least=0.0):
     rng = np.random.default_rng(seed)
     w = (rng.standard_normal((v, d)) / np.sqrt(d)).astype(np.float32)
     labels = rng.integers(v, size=n)
-    x = (rng.standard_normal((d, n)) + lean * rng.random(n) * w[labels].T).astype(np.float32)
+    x = (rng.standard_normal((d, n)) + (least + lean * rng.random(n)) * w[labels].T).astype(np.float32)
     b = (0.1 * rng.standard_normal(v)).astype(np.float32)
     if masked:
         hide = rng.random(v) < masked
@@ -360,7 +360,10 @@ def fcl_ref(w, x, b, lab, coeff):
     a = np.abs(w) @ np.abs(x) + np.where(np.isfinite(b), np.abs(b), 0)[:, None]
     ez = (sum_err(w.shape[1]) + 4 * U) * a.max(0)
     er = 2 * ez + sum_err(v) + 16 * U
-    edz = (np.abs(coeff) * ok) * (e / tot) * er + 4 * U * np.abs(dz)
+    # p is off by p (sum over the others of p times twice the error of a logit) -- the error of its own logit cancels, the two calls'
+    # logits being the same -- and by the rounding of the sum: of what is not at the maximum, and of the whole
+    p = e / tot
+    edz = (np.abs(coeff) * ok) * p * ((1 - p) * 2 * ez + sum_err(v) * (1 - p.max(0)) + 16 * U) + 4 * U * np.abs(dz)
     return dict(z=z, top=top, tot=tot, logp=logp, correct=correct, dz=dz, dx=w.T @ dz, dw=dz @ x.T, db=dz.sum(1), ez=ez, er=er, ok=ok,
                 edx=np.abs(w).T @ edz + (sum_err(v) + 2 * U) * (np.abs(w).T @ np.abs(dz)),
                 edw=edz @ np.abs(x).T + (sum_err(n) + 2 * U) * (np.abs(dz) @ np.abs(x).T),
@@ -420,6 +423,18 @@ def test_fc_logreg(d, v, n):
     within(got[3], t[0] + ref['dx'], ref['edx'] + 4 * U * (np.abs(t[0]) + np.abs(ref['dx'])), 'dx added')
     within(got[4], 0.9 * t[1] + 0.5 * ref['dw'], 0.5 * ref['edw'] + 4 * U * (np.abs(t[1]) + np.abs(ref['dw'])), 'dw added')
     within(got[5], 0.25 * t[2] - 2 * ref['db'], 2 * ref['edb'] + 4 * U * (np.abs(t[2]) + 2 * np.abs(ref['db'])), 'db added')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('d,v,n', [(580, 23, 52), (512, 5, 3), (160, 4213, 64), (160, 4213, 65), (512, 1000, 128), (96, 33000, 20), (2000, 5000, 16)])
+def test_fc_logreg_of_certain_cases(d, v, n):
+    """Labels whose probability is 1 - 1e-3 to 1 - 1e-8: the gradient is what is left of 1 - p."""
+    w, x, b, lab = fcl_data(d, v, n, 61, lean=10.0, least=14.0)
+    ref = fcl_ref(w, x, b, lab, 1.0)
+    st, lp, ok, dx, dw, db, cost = fcl_run(w, x, b, lab)
+    check_forward(ref, st, lp, ok)
+    for got, k in ((dx, 'dx'), (dw, 'dw'), (db, 'db')):
+        within(got, ref[k], ref['e' + k], k)
 
 
 @pytest.mark.gpu
