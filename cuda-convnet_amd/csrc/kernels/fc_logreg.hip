@@ -13,7 +13,7 @@ namespace {
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // (16-byte accesses at any multiple of four bytes)
 
 constexpr int NARROW = 64;  // k_fcl_narrow: most cases
-constexpr int PIECE_MB = 128;  // fragments of a piece; 512 x 100000 x 1024, both calls: 64 MB 1.77 ms, 128 MB 1.65 ms, 224 MB 1.62 ms
+constexpr int PIECE_MB = 192;  // fragments of a piece; 512 x 100000 x 1024, both calls: 96 MB 1.50 ms, 128 MB 1.49 ms, 192 MB 1.45 ms, 256 MB 1.49 ms
 
 struct NarrowArgs {
     const float *W, *X, *bias, *labels;
