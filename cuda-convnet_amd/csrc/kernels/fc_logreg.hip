@@ -1069,7 +1069,8 @@ int tile_bytes(TileKind k) { return k == SHARED ? SHARED_LDS : tile_lds(tile_row
 // Sizes and workspace of the wide path: a function of the shape alone.
 struct WidePlan {
     int Np, Dp, Kd, kSteps, Kn, nTiles, dTiles;  // Kd: k blocks of W's and x's fragments, padded; kSteps: those that hold anything
-    int rows, Kv;                                // classes per piece; k blocks of a whole piece, padded
+    int rows, last;                              // classes per piece, and of the last one, which takes a short rest with it
+    int Kv;                                      // k blocks of the first piece, padded
     int kPerSplit, splits;                       // input gradient: every split of a whole piece holds something, so that the first piece
                                                  // writes every slab
     size_t classExp, caseExp, featExp, xByCase, xByFeat, wByClass, dz, dbPart, slabs, part, labelLogits, total;
@@ -1091,24 +1092,28 @@ WidePlan wide_plan(int D, int V, int N, bool bwd) {
     p.Dp = p.dTiles * TILE;
     p.Kn = p.Np / 32;
     // a piece's fragments should stay in the 256 MB last-level cache between the launches that write and read them; whole rounds of
-    // shared tiles where the classes fill some
+    // shared tiles where the classes fill some; a rest of at most a quarter goes with the last piece
     const size_t perRow = (size_t)p.Kd * 128 + (bwd ? (size_t)p.Np * 4 : 0);
     const int most = (int)std::max<size_t>(TILE, std::min<size_t>(((size_t)PIECE_MB << 20) / perRow / TILE * TILE, (size_t)1 << 17));
     const int round = std::max(1, 512 / p.nTiles) * TILE;
     p.rows = std::min(V, most > round ? most / round * round : most);
+    const int rest = V % p.rows;
+    p.last = rest == 0 ? p.rows : rest <= p.rows / 4 ? p.rows + rest : rest;
+    p.rows = std::min(V, V <= p.last ? p.last : p.rows);
     p.Kv = divup(p.rows, TILE) * 4;
+    const size_t mostKv = (size_t)divup(std::max(p.rows, p.last), TILE) * 4;
     p.kPerSplit = divup(p.Kv, std::max(1, std::min(p.Kv / 8, 512 / (p.nTiles * p.dTiles))));
     p.splits = divup(p.Kv, p.kPerSplit);
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t o = at; at += al256(bytes); return o; };
-    p.classExp = take((size_t)p.Kv * 4);
+    p.classExp = take(mostKv * 4);
     p.caseExp = take((size_t)p.Np * 4);
     p.xByCase = take((size_t)p.Np / 16 * p.Kd * PAIR);
-    p.wByClass = take((size_t)p.Kv * 2 * p.Kd * PAIR);
+    p.wByClass = take(mostKv * 2 * p.Kd * PAIR);
     if (bwd) {
         p.featExp = take((size_t)p.Dp * 4);
         p.xByFeat = take((size_t)p.Dp / 16 * p.Kn * PAIR);
-        p.dz = take((size_t)p.Np / 16 * p.Kv * PAIR);
+        p.dz = take((size_t)p.Np / 16 * mostKv * PAIR);
         p.dbPart = take((size_t)p.nTiles * V * 4);
         p.slabs = take((size_t)p.splits * p.Dp * p.Np * 4);
     } else {
@@ -1161,7 +1166,7 @@ WideArgs wide_args(const WidePlan& q, const float* bias, const float* labels, in
 // one piece: its packed rows, tiles and k blocks; with the first one, x
 TileKind wide_piece(const WidePlan& q, WideArgs& a, PackArgs& k, const float* W, int D, int v0, hipStream_t s) {
     a.v0 = v0;
-    a.rows = k.rows = std::min(q.rows, a.V - v0);
+    a.rows = k.rows = a.V - v0 <= q.last ? a.V - v0 : q.rows;
     a.nTiles = q.nTiles;
     a.Kv = divup(a.rows, TILE) * 4;
     const TileKind kind = tile_choice(a.Kv, q.nTiles);
@@ -1190,7 +1195,7 @@ int wide_cost(const float* W, const float* X, const float* bias, const float* la
     a.labelLogits = (float*)(ws + q.labelLogits);
     PackArgs pack = pack_args(q, X, labels, D, V, N, false, ws);
     int tiles = 0;
-    for (int v0 = 0; v0 < V; v0 += q.rows) {
+    for (int v0 = 0; v0 < V; v0 += a.rows) {
         const TileKind kind = wide_piece(q, a, pack, W, D, v0, s);
         a.part = (float*)(ws + q.part) + (size_t)tiles * 3 * N;
         launch_logits<false>(kind, a, s);
@@ -1222,7 +1227,7 @@ int wide_grad(const float* W, const float* X, const float* bias, const float* la
     t.D = D; t.Kn = q.Kn; t.Kd = q.Kd; t.Np = q.Np; t.Dp = q.Dp; t.nTiles = q.nTiles; t.dTiles = q.dTiles;
     t.scaleTargets = scaleWeightTargets;
     t.scaleOutput = scaleWeightOutput * coeff;
-    for (int v0 = 0; v0 < V; v0 += q.rows) {
+    for (int v0 = 0; v0 < V; v0 += a.rows) {
         const TileKind kind = wide_piece(q, a, pack, W, D, v0, s);
         if (narrow) {
             few.v0 = v0;
@@ -1232,7 +1237,7 @@ int wide_grad(const float* W, const float* X, const float* bias, const float* la
         } else {
             launch_logits<true>(kind, a, s);
         }
-        // (a short last piece has fewer, not shorter, shares of the input gradient: each adds to its slab)
+        // (the last piece has no more shares of the input gradient than there are slabs, and a short one fewer, not shorter ones)
         t.kPerSplit = a.Kv == q.Kv ? q.kPerSplit : std::max(8, divup(a.Kv, q.splits));
         t.inputBlocks = dX ? divup(a.Kv, t.kPerSplit) * q.nTiles * q.dTiles : 0;
         t.dW = dW ? dW + (size_t)v0 * D : nullptr;

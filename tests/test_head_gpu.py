@@ -426,6 +426,23 @@ def test_fc_logreg(d, v, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('d,v,n', [(20000, 5000, 70), (20000, 5600, 8)])
+def test_fc_logreg_of_more_classes_than_a_piece_takes(d, v, n):
+    """Two pieces, the last one with a short rest; three, the last one short."""
+    rng = np.random.default_rng(71)
+    w = rng.standard_normal((v, d), dtype=np.float32) * np.float32(d ** -0.5)
+    x = rng.standard_normal((d, n), dtype=np.float32)
+    b = (0.1 * rng.standard_normal(v)).astype(np.float32)
+    lab = rng.integers(v, size=n).astype(np.float32)
+    lab[:4] = 0, 2431, 2432, v - 1
+    ref = fcl_ref(w, x, b, lab, 0.5)
+    st, lp, ok, dx, dw, db, cost = fcl_run(w, x, b, lab, 0.5)
+    check_forward(ref, st, lp, ok)
+    for got, k in ((dx, 'dx'), (dw, 'dw'), (db, 'db')):
+        within(got, ref[k], ref['e' + k], k)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('d,v,n', [(580, 23, 52), (512, 5, 3), (160, 4213, 64), (160, 4213, 65), (512, 1000, 128), (96, 33000, 20), (2000, 5000, 16)])
 def test_fc_logreg_of_certain_cases(d, v, n):
     """Labels whose probability is 1 - 1e-3 to 1 - 1e-8: the gradient is what is left of 1 - p."""
