@@ -13,7 +13,7 @@ namespace {
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // (16-byte accesses at any multiple of four bytes)
 
 constexpr int NARROW = 64;  // k_fcl_narrow: most cases
-constexpr int PIECE_MB = 192;  // fragments of a piece; 512 x 100000 x 1024, both calls: 96 MB 1.50 ms, 128 MB 1.49 ms, 192 MB 1.45 ms, 256 MB 1.49 ms
+constexpr int PIECE_MB = 192;  // fragments of a piece; 512 x 100000 x 1024, both calls: 128 MB 1.52 ms, 160 MB 1.50 ms, 192 MB 1.41 ms, 256 MB 1.48 ms
 
 struct NarrowArgs {
     const float *W, *X, *bias, *labels;
@@ -576,8 +576,8 @@ struct PackArgs {
     int rows;
 };
 
-// Bound by memory: W is read once and written once, as two pieces of 16 bits (10575 x 512: 13 us, 3.3 TB/s; 100000 x 512, one call: 88 us,
-// 4.7 TB/s).  Each block finds its rows' largest magnitudes first; what it reads then comes from its caches.
+// Bound by memory: W is read once and written once, as two pieces of 16 bits (10575 x 512: 13 us, 3.3 TB/s; 100000 x 512, one call: 83 us,
+// 5.0 TB/s).  Each block finds its rows' largest magnitudes first; what it reads then comes from its caches.
 __device__ __forceinline__ void pack_cases(const PackArgs& p, int block, float* sh, int* exps) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4, n = block * 16 + c;
     float m = 0.f;
@@ -737,8 +737,8 @@ struct WideArgs {
     int Kv;
 };
 
-// SHARED: two blocks per CU (MB = 4).  512 x 100000 x 1024: forward 349 us, 900 TFLOP/s of fp16 products, backward, which writes dz,
-// 398 us, 790; a large library product of fp16 operands reaches 1126.
+// SHARED: two blocks per CU (MB = 4).  512 x 100000 x 1024: forward 346 us, 909 TFLOP/s of fp16 products, backward, which writes dz,
+// 393 us, 800; a large library product of fp16 operands reaches 1126.
 template <int MB, bool BWD, bool SHARED>
 __global__ __launch_bounds__(256, SHARED ? 2 : 1) void k_fcl_logits(WideArgs p) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -1014,7 +1014,7 @@ __device__ __forceinline__ void input_tile(const GradArgs& p, int L, char* lds) 
         }
 }
 
-// ---- both gradients of a piece in one launch: they wait for the same logits and not for each other.  512 x 100000 x 1024: 588 us, 1070
+// ---- both gradients of a piece in one launch: they wait for the same logits and not for each other.  512 x 100000 x 1024: 579 us, 1087
 // TFLOP/s of fp16 products; 512 x 10575 x 128: 17.5 us.
 template <bool SHARED>
 __global__ __launch_bounds__(256, SHARED ? 2 : 1) void k_fcl_grads(GradArgs p) {
