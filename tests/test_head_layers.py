@@ -39,7 +39,7 @@ def test_dropout_seed_is_drawn_where_none_is_given(tmp_path):
 
 
 def test_dropout_key_of_other_layers_stays_without_effect(tmp_path):
-    """The DeepID definitions carry dropout=0.4 on fc5, which the reference does not read."""
+    """The DeepID definitions carry dropout=0.4 on fc5, which no parser of the reference reads."""
     p = tmp_path / 'a.cfg'
     p.write_text(open(CFG).read().replace('neuron=relu', 'neuron=relu\ndropout=0.4'))
     assert [(l['name'], l['type']) for l in parse(str(p))] == [(l['name'], l['type']) for l in parse()]
