@@ -629,6 +629,7 @@ MCN_API int mcn_layer_norm(const float* inputs, const float* gains, const float*
     if (p.whole) {
         const dim3 grid(divup(p.tiles, 8) * 8);
 #define WHOLE(VW, R) MCN_LAUNCH((k_ln_whole<VW, R>), grid, dim3(T_WHOLE), 0, st, inputs, gains, biases, target, caseStats, eps, F, N, p.logLanes, p.tiles)
+        // (few rows a thread: 160 x 4096 5.3 -> 4.6 us, 512 x 128 5.3 -> 4.8 us)
         const bool few = ((size_t)F << p.logLanes) <= T_WHOLE * 4;
         if (p.vw == 4 && few) WHOLE(4, 4);
         else if (p.vw == 4) WHOLE(4, FWD_ROWS);
@@ -682,10 +683,7 @@ MCN_API int mcn_layer_norm_undo(const float* outGrads, const float* inputs, cons
         const dim3 grid(q.first + rowBlocks);
 #define WHOLE(VW, R) MCN_LAUNCH((k_ln_undo_whole<VW, R>), grid, dim3(T_WHOLE), 0, st, outGrads, inputs, gains, caseStats, target, \
                                 rowPart, scaleTargets, scaleOutput, F, N, p.logLanes, p.tiles, q)
-        const bool few = ((size_t)F << p.logLanes) <= T_WHOLE * 2;
-        if (p.vw == 4 && few) WHOLE(4, 2);
-        else if (p.vw == 4) WHOLE(4, BWD_ROWS);
-        else if (few) WHOLE(1, 2);
+        if (p.vw == 4) WHOLE(4, BWD_ROWS);
         else WHOLE(1, BWD_ROWS);
 #undef WHOLE
     } else {
