@@ -310,6 +310,7 @@ __global__ __launch_bounds__(256) void k_fcl_cost(const float* __restrict__ labe
 // is the fragments' ROW, a transposing LDS read (ds_read_b64_tr_b16) gives lane (k = 16 h + c, g) rows 4 g .. 4 g + 3 of two fragments.
 // Both read 512 contiguous bytes a wave, without conflicts, and in both a lane's eight entries are 4 g + j and 16 + 4 g + j of the step's
 // 32, so that every pairing sums the same terms.  So W and dz are each stored once, and serve two products.
+
 // the power of two that brings a group of largest magnitude m to [2^14, 2^15); infinities and NaNs stay as they are
 __device__ __forceinline__ int scale_exp(float m) { return m > 0.f && m < INFINITY ? 14 - ilogbf(m) : 0; }
 __device__ __forceinline__ float max_or_nan(float m, float v) { return v > m || v != v ? v : m; }

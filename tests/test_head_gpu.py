@@ -602,11 +602,12 @@ def head_ref(x, gain, bias, w, b, lab, keep, p, coeff):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize('captured', [False, True])
-def test_head_together(captured):
+@pytest.mark.parametrize('n', [96, 24])
+def test_head_together(captured, n):
     """norm -> dropout -> classifier cost and back, on a stream of its own: eager, and as a graph that is replayed with new masks
     between the program's own eager work.  Six stages, each with sums of at most 900 terms (sum_err(900) = 1.5e-5 of the magnitudes):
     1e-4 of the largest value."""
-    f, v, n, p, coeff = 160, 900, 96, 0.4, 1.0 / 96
+    f, v, p, coeff = 160, 900, 0.4, 1.0 / n
     x, gain, bias, _ = norm_data(f, n, 21)
     w, _, b, lab = fcl_data(f, v, n, 22)
     stream = C.c_void_p()
