@@ -4,6 +4,7 @@
 #include <stdint.h>
 #include <stdio.h>
 #include <time.h>
+#include <initializer_list>
 #include "../../../include/mi_convnet.h"
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -80,6 +81,19 @@ static inline size_t divup_sz(size_t a, size_t b) { return (a + b - 1) / b; }
 // whether na floats at a and nb at b share any (a null pointer shares nothing)
 static inline bool mcn_overlap(const float* a, size_t na, const float* b, size_t nb) {
     return a && b && (uintptr_t)a < (uintptr_t)b + nb * sizeof(float) && (uintptr_t)b < (uintptr_t)a + na * sizeof(float);
+}
+// MCN_EINVAL where an output shares memory with an operand or another output: blocks of one launch would read what others have written
+struct McnSpan {
+    const char* name;
+    const float* p;
+    size_t n;
+};
+static inline int mcn_refuse_overlaps(const char* what, std::initializer_list<McnSpan> outs, std::initializer_list<McnSpan> ins) {
+    for (const McnSpan* o = outs.begin(); o != outs.end(); o++) {
+        for (const McnSpan& i : ins) MCN_REQUIRE(!mcn_overlap(o->p, o->n, i.p, i.n), "%s: %s overlaps %s", what, o->name, i.name);
+        for (const McnSpan* q = outs.begin(); q != o; q++) MCN_REQUIRE(!mcn_overlap(o->p, o->n, q->p, q->n), "%s: %s overlaps %s", what, o->name, q->name);
+    }
+    return MCN_OK;
 }
 
 // v_mfma_f32_16x16x4_f32: lane l holds A[row=l&15][k=l>>4], B[k=l>>4][col=l&15];

@@ -621,6 +621,10 @@ MCN_API int mcn_layer_norm(const float* inputs, const float* gains, const float*
     MCN_REQUIRE(inputs && target && ln_sizes_ok(numFeatures, numCases), "layerNorm: bad argument");
     const size_t n = (size_t)numFeatures * numCases;
     MCN_REQUIRE(target == inputs || !mcn_overlap(target, n, inputs, n), "layerNorm: target overlaps inputs in part");
+    const size_t f = numFeatures, stats = (size_t)2 * numCases;
+    if (int rc = mcn_refuse_overlaps("layerNorm", {{"target", target, n}}, {{"gains", gains, f}, {"biases", biases, f}})) return rc;
+    if (int rc = mcn_refuse_overlaps("layerNorm", {{"caseStats", caseStats, stats}},
+                                     {{"target", target, n}, {"inputs", inputs, n}, {"gains", gains, f}, {"biases", biases, f}})) return rc;
     MCN_REQUIRE(eps > 0.f, "layerNorm: eps %g is not positive", (double)eps);
     if (int rc = ln_require_workspace(workspace, workspaceBytes, mcn_layer_norm_workspace_bytes(numFeatures, numCases), "layerNorm")) return rc;
     hipStream_t st = (hipStream_t)stream;
@@ -665,7 +669,9 @@ MCN_API int mcn_layer_norm_undo(const float* outGrads, const float* inputs, cons
     MCN_REQUIRE(outGrads && inputs && caseStats && ln_sizes_ok(numFeatures, numCases), "layerNormUndo: bad argument");
     MCN_REQUIRE(target || gainGrads || biasGrads, "layerNormUndo: nothing to compute");
     const size_t n = (size_t)numFeatures * numCases;
-    MCN_REQUIRE(!mcn_overlap(target, n, outGrads, n) && !mcn_overlap(target, n, inputs, n), "layerNormUndo: the target overlaps an operand");
+    const size_t f = numFeatures;
+    if (int rc = mcn_refuse_overlaps("layerNormUndo", {{"target", target, n}, {"gainGrads", gainGrads, f}, {"biasGrads", biasGrads, f}},
+                                     {{"outGrads", outGrads, n}, {"inputs", inputs, n}, {"gains", gains, f}, {"caseStats", caseStats, (size_t)2 * numCases}})) return rc;
     if (int rc = ln_require_workspace(workspace, workspaceBytes, mcn_layer_norm_undo_workspace_bytes(numFeatures, numCases), "layerNormUndo")) return rc;
     hipStream_t st = (hipStream_t)stream;
     const int F = numFeatures, N = numCases;

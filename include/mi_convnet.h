@@ -574,9 +574,9 @@ int mcn_l2reg_grad(const float* ground, const float* data, float* target, int nu
  * its DeepID definitions carry a dropout key that no parser reads -- and keeps the logits of every class) ------------------- */
 /* Layer norm over the features of each case: inputs, target (numFeatures, numCases); gains, biases (numFeatures, may be NULL: 1 / 0);
  *   target[f,n] = gains[f] * (inputs[f,n] - mean[n]) * r[n] + biases[f],  r = 1 / sqrt(var + eps), var over numFeatures, eps > 0.
- * caseStats (2, numCases): the means, then r, for mcn_layer_norm_undo (may be NULL).  target may be inputs itself; otherwise the two do
- * not overlap.  Sizes from 1 to 2^26 each.  Calls that run at the same time need a workspace each; so do graphs that are replayed at
- * the same time. */
+ * caseStats (2, numCases): the means, then r, for mcn_layer_norm_undo (may be NULL).  target may be inputs itself; otherwise no output
+ * overlaps an operand or the other output (MCN_EINVAL).  Sizes from 1 to 2^26 each.  Calls that run at the same time need a workspace
+ * each; so do graphs that are replayed at the same time. */
 size_t mcn_layer_norm_workspace_bytes(int numFeatures, int numCases);
 int mcn_layer_norm(const float* inputs, const float* gains, const float* biases, float* target, float* caseStats, int numFeatures,
                    int numCases, float eps, void* workspace, size_t workspaceBytes, void* stream);
@@ -584,7 +584,7 @@ int mcn_layer_norm(const float* inputs, const float* gains, const float* biases,
  * be NULL (not wanted), but not all of them:
  *   target (numFeatures, numCases) = scaleTargets*target + scaleOutput * d/d inputs,
  *   gainGrads, biasGrads (numFeatures) = scale{Gain,Bias}Targets * old + scale{Gain,Bias}Output * d/d gains, biases.
- * The target overlaps neither outGrads nor inputs. */
+ * No output overlaps an operand or another output (MCN_EINVAL): gains are updated from gainGrads by a launch of its own. */
 size_t mcn_layer_norm_undo_workspace_bytes(int numFeatures, int numCases);
 int mcn_layer_norm_undo(const float* outGrads, const float* inputs, const float* gains, const float* caseStats, float* target,
                         float* gainGrads, float* biasGrads, int numFeatures, int numCases, float scaleTargets, float scaleOutput,

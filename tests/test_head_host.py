@@ -129,3 +129,30 @@ def test_dropout_plain_generator_known_answers():
     ones = (1 << 64) - 1
     got = [int(v) for v in philox_words(4, ones, ones, first_quad=ones)]
     assert got == [0x408f276d, 0x41c83b0e, 0xa20bc7c6, 0x6d5451fd]
+
+
+NORM = dict(x=32, gain=8, bias=8, y=32, stats=8)  # floats of each operand of norm()
+UNDO = dict(g=32, x=32, gain=8, stats=8, dx=32, dg=8, db=8)
+
+
+def overlaps(sizes, outs, ins):
+    """(pointer to move, the one it is moved over): every output against every operand and every other output."""
+    return [(o, i) for o in outs for i in list(ins) + [q for q in outs if q < o]]
+
+
+@pytest.mark.parametrize('end', [False, True])
+@pytest.mark.parametrize('o,i', [p for p in overlaps(NORM, ('y', 'stats'), ('x', 'gain', 'bias')) if p != ('y', 'x')])
+def test_layer_norm_refuses_outputs_over_operands(o, i, end):
+    """A block that is ahead of the others would write what they have still to read."""
+    at = dict(x=P[0], gain=P[1], bias=P[2], y=P[3], stats=P[4])
+    code, msg = norm(**{o: at[i] + (NORM[i] - 1 if end else 1 - NORM[o]) * 4})
+    assert code == EINVAL and 'layerNorm' in msg and 'overlap' in msg
+
+
+@pytest.mark.parametrize('end', [False, True])
+@pytest.mark.parametrize('o,i', overlaps(UNDO, ('dx', 'dg', 'db'), ('g', 'x', 'gain', 'stats')))
+def test_layer_norm_undo_refuses_outputs_over_operands(o, i, end):
+    at = dict(g=P[0], x=P[1], gain=P[2], stats=P[3], dx=P[4], dg=P[5], db=P[6])
+    code, msg = undo(**{o: at[i] + (UNDO[i] - 1 if end else 1 - UNDO[o]) * 4})
+    assert code == EINVAL and 'layerNormUndo' in msg and 'overlap' in msg
+    assert undo(**{o: at[i]})[0] == EINVAL  # in place of one another
