@@ -1296,6 +1296,12 @@ MCN_API int mcn_fc_logreg_cost(const float* weights, const float* inputs, const 
                                void* workspace, size_t workspaceBytes, void* stream) {
     MCN_REQUIRE(weights && inputs && labels && caseStats && labelLogProbs && correctProbs, "fcLogregCost: null pointer");
     MCN_REQUIRE(fcl_sizes_ok(numInputs, numOutputs, numCases), "fcLogregCost: %d inputs, %d outputs, %d cases", numInputs, numOutputs, numCases);
+    const size_t n = (size_t)numCases;
+    if (int rc = mcn_refuse_overlaps("fcLogregCost",
+                                     {{"caseStats", caseStats, 2 * n}, {"labelLogProbs", labelLogProbs, n}, {"correctProbs", correctProbs, n}, {"costOut", (const float*)costOut, 4}},
+                                     {{"weights", weights, (size_t)numOutputs * numInputs}, {"inputs", inputs, (size_t)numInputs * numCases},
+                                      {"biases", biases, (size_t)numOutputs}, {"labels", labels, n}}))
+        return rc;
     if (int rc = fcl_check("fcLogregCost", workspace, workspaceBytes, fcl_cost_bytes(numInputs, numOutputs, numCases))) return rc;
     hipStream_t s = (hipStream_t)stream;
     if (wide_cost_usable(numCases)) {
@@ -1320,11 +1326,10 @@ MCN_API int mcn_fc_logreg_grad(const float* weights, const float* inputs, const 
     MCN_REQUIRE(weights && inputs && labels && caseStats, "fcLogregGrad: null pointer");
     MCN_REQUIRE(inputGrads || weightGrads || biasGrads, "fcLogregGrad: nothing to compute");
     MCN_REQUIRE(fcl_sizes_ok(numInputs, numOutputs, numCases), "fcLogregGrad: %d inputs, %d outputs, %d cases", numInputs, numOutputs, numCases);
-    const size_t nX = (size_t)numInputs * numCases, nW = (size_t)numOutputs * numInputs, nB = (size_t)numOutputs;
-    const struct { const float* p; size_t n; } ins[] = {{weights, nW}, {inputs, nX}, {biases, nB}, {labels, (size_t)numCases}, {caseStats, (size_t)numCases * 2}},
-                                               outs[] = {{inputGrads, nX}, {weightGrads, nW}, {biasGrads, nB}};
-    for (const auto& o : outs)
-        for (const auto& i : ins) MCN_REQUIRE(!mcn_overlap(o.p, o.n, i.p, i.n), "fcLogregGrad: a gradient is written over an operand");
+    const size_t nX = (size_t)numInputs * numCases, nW = (size_t)numOutputs * numInputs, nB = (size_t)numOutputs, n = (size_t)numCases;
+    if (int rc = mcn_refuse_overlaps("fcLogregGrad", {{"inputGrads", inputGrads, nX}, {"weightGrads", weightGrads, nW}, {"biasGrads", biasGrads, nB}},
+                                     {{"weights", weights, nW}, {"inputs", inputs, nX}, {"biases", biases, nB}, {"labels", labels, n}, {"caseStats", caseStats, 2 * n}}))
+        return rc;
     if (int rc = fcl_check("fcLogregGrad", workspace, workspaceBytes, fcl_grad_bytes(numInputs, numOutputs, numCases))) return rc;
     return wide_grad(weights, inputs, biases, labels, caseStats, inputGrads, weightGrads, biasGrads, numInputs, numOutputs, numCases, coeff,
                      scaleInputTargets, scaleWeightTargets, scaleWeightOutput, scaleBiasTargets, scaleBiasOutput, (char*)workspace,

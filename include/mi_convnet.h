@@ -610,15 +610,15 @@ int mcn_counter_add(uint64_t* counter, uint64_t by, void* stream);
  *   costOut (device doubles, may be NULL): [0] += -sum(labelLogProbs), [1] += cases that count - sum(correctProbs).
  * A case all of whose classes are -inf has statistics (-inf, 0), log probability -inf and no gradient.  What the weights of a class
  * that is taken out hold, or the inputs of a case that does not count, comes through nowhere, except for such a case's own statistics.
- * numOutputs from 1 to 2^24 (labels are fp32), numInputs and numCases to 2^20, numInputs * numCases to 2^34.  Workspaces as for
- * mcn_layer_norm; backward != 0: for both calls, 0: the cost alone. */
+ * numOutputs from 1 to 2^24 (labels are fp32), numInputs and numCases to 2^20, numInputs * numCases to 2^34.  No output overlaps an operand
+ * or another output (MCN_EINVAL).  Workspaces as for mcn_layer_norm; backward != 0: for both calls, 0: the cost alone. */
 size_t mcn_fc_logreg_workspace_bytes(int numInputs, int numOutputs, int numCases, int backward);
 int mcn_fc_logreg_cost(const float* weights, const float* inputs, const float* biases, const float* labels, float* caseStats,
                        float* labelLogProbs, float* correctProbs, int numInputs, int numOutputs, int numCases, double* costOut,
                        void* workspace, size_t workspaceBytes, void* stream);
 /* The gradients, given the caseStats that mcn_fc_logreg_cost left for the same operands.  With dz = coeff * ((v == label) - p)
  * (the sign of computeLogregSoftmaxGrad, layer_kernels.cu:287-308), computed again in pieces of the classes, each output may be NULL
- * and none may overlap an operand:
+ * (not all of them) and none may overlap an operand or another output:
  *   inputGrads (numInputs, numCases) = scaleInputTargets*inputGrads + weights^T dz,
  *   weightGrads (as weights) = scaleWeightTargets*weightGrads + scaleWeightOutput * dz inputs^T,
  *   biasGrads (numOutputs) = scaleBiasTargets*biasGrads + scaleBiasOutput * (row sums of dz). */

@@ -156,3 +156,25 @@ def test_layer_norm_undo_refuses_outputs_over_operands(o, i, end):
     code, msg = undo(**{o: at[i] + (UNDO[i] - 1 if end else 1 - UNDO[o]) * 4})
     assert code == EINVAL and 'layerNormUndo' in msg and 'overlap' in msg
     assert undo(**{o: at[i]})[0] == EINVAL  # in place of one another
+
+
+COST = dict(w=1600, x=128, b=100, l=8, st=16, lp=8, ok=8, out=4)
+GRAD = dict(w=1600, x=128, b=100, l=8, st=16, dx=128, dw=1600, db=100)
+
+
+@pytest.mark.parametrize('end', [False, True])
+@pytest.mark.parametrize('o,i', overlaps(COST, ('st', 'lp', 'ok', 'out'), ('w', 'x', 'b', 'l')))
+def test_fc_logreg_cost_refuses_outputs_over_operands(o, i, end):
+    """The labels are read again after the log probabilities are written."""
+    at = dict(w=P[0], x=P[1], b=P[2], l=P[3], st=P[4], lp=P[5], ok=P[6], out=P[8])
+    at[o] = at[i] + (COST[i] - 1 if end else 1 - COST[o]) * 4
+    code, msg = rc('mcn_fc_logreg_cost', at['w'], at['x'], at['b'], at['l'], at['st'], at['lp'], at['ok'], 16, 100, 8, at['out'], P[7], BIG, None)
+    assert code == EINVAL and 'fcLogregCost' in msg and 'overlap' in msg
+
+
+@pytest.mark.parametrize('end', [False, True])
+@pytest.mark.parametrize('o,i', overlaps(GRAD, ('dx', 'dw', 'db'), ('w', 'x', 'b', 'l', 'st')))
+def test_fc_logreg_grad_refuses_outputs_over_operands(o, i, end):
+    at = dict(w=P[0], x=P[1], b=P[2], l=P[3], st=P[4], dx=P[5], dw=P[6], db=P[8])
+    code, msg = grad(**{o: at[i] + (GRAD[i] - 1 if end else 1 - GRAD[o]) * 4})
+    assert code == EINVAL and 'fcLogregGrad' in msg and 'overlap' in msg
