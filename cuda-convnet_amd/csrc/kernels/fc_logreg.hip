@@ -355,10 +355,10 @@ __device__ __forceinline__ void wait_copies_and_meet() {
     asm volatile("" ::: "memory");
 }
 // The two pieces of a pair (2 KB) from global memory to LDS; the instruction's offset counts on both sides.  The compiler would drain
-// every such copy in front of the next LDS read if it knew of it; here the waits are wait_copies_and_meet's.  No register is written.
+// every such copy in front of the next LDS read if it knew of it; here the waits are wait_copies_and_meet's.  No register but m0 is written.
 __device__ __forceinline__ void copy_pair_half(const char* src, unsigned lds, unsigned laneOff, int piece) {
-    if (piece == 0) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(laneOff), "s"(src) : "memory");
-    else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024" ::"s"(lds), "v"(laneOff), "s"(src) : "memory");
+    if (piece == 0) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(laneOff), "s"(src) : "m0", "memory");
+    else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024" ::"s"(lds), "v"(laneOff), "s"(src) : "m0", "memory");
 }
 __device__ __forceinline__ f16x8 read_frag(const char* p) {
     const f16x4 a = *reinterpret_cast<const f16x4*>(p), b = *reinterpret_cast<const f16x4*>(p + 512);

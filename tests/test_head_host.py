@@ -2,7 +2,10 @@
 
 The pointers are numbers that nothing may look at; a call that got past the checks would fail at the launch (no GPU) with another code."""
 import ctypes as C
+import glob
 import math
+import os
+import re
 
 import pytest
 
@@ -178,3 +181,15 @@ def test_fc_logreg_grad_refuses_outputs_over_operands(o, i, end):
     at = dict(w=P[0], x=P[1], b=P[2], l=P[3], st=P[4], dx=P[5], dw=P[6], db=P[8])
     code, msg = grad(**{o: at[i] + (GRAD[i] - 1 if end else 1 - GRAD[o]) * 4})
     assert code == EINVAL and 'fcLogregGrad' in msg and 'overlap' in msg
+
+
+def test_inline_assembly_names_m0_where_it_writes_it():
+    """The compiler keeps values of its own in m0 (LDS copies, indexed moves): a block that writes it has to say so."""
+    kernels = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'cuda-convnet_amd', 'csrc', 'kernels')
+    seen = 0
+    for path in glob.glob(os.path.join(kernels, '*.h*')):
+        for block in re.findall(r'\basm\b[^;]*;', open(path).read()):
+            if re.search(r'\bm0\s*,', block):  # (as a destination)
+                seen += 1
+                assert re.search(r':[^:]*"m0"[^:]*\)\s*;$', block), (os.path.basename(path), block)
+    assert seen
