@@ -559,9 +559,12 @@ struct Plan {
     Split split;
 };
 constexpr size_t CACHED_BYTES = (size_t)128 << 20;  // a matrix that stays in the last-level cache
-// both matrices of a backward pass: the rows are summed by blocks of their own, as their second read comes from the caches (512 x 128,
-// forward and backward: 15.6 us with partial sums and a launch to join them, 11.8 us so)
+// Both matrices of a backward pass, and the cases of a row: up to these the rows are summed by blocks of their own in the same launch, as
+// their second read comes from the caches, with at most 16 steps of a wave along a row (forward and backward, so / with partial sums and a
+// launch that joins them: 16 x 512 13.7 / 16.5 us, 128 x 4096 14.4 / 16.6, 512 x 4096 19.6 / 18.9, 2 x 8192 20.3 / 16.4, 128 x 8192 22.2 /
+// 16.0, 16 x 32768 71 / 27, 16 x 262144 583 / 113, 2 x 2000000 4050 / 770).  Longer rows of one wave would also be one long chain of sums.
 constexpr size_t SMALL_BYTES = (size_t)32 << 20;
+constexpr int SMALL_CASES = 4096;
 constexpr int FWD_ROWS = 16, BWD_ROWS = 8;       // rows a thread of the whole kernels holds
 // rows: FWD_ROWS or BWD_ROWS
 Plan ln_plan(int F, int N, int rows) {
@@ -676,7 +679,7 @@ MCN_API int mcn_layer_norm_undo(const float* outGrads, const float* inputs, cons
     hipStream_t st = (hipStream_t)stream;
     const int F = numFeatures, N = numCases;
     const Plan p = ln_plan(F, N, BWD_ROWS);
-    const bool rows = gainGrads || biasGrads, small = (size_t)F * N * 8 <= SMALL_BYTES;
+    const bool rows = gainGrads || biasGrads, small = N <= SMALL_CASES && (size_t)F * N * 8 <= SMALL_BYTES;
     float* rowPart = rows && !small ? (float*)workspace : nullptr;
     const Split& sp = p.split;
     RowSums q = {gainGrads, biasGrads, scaleGainTargets, scaleGainOutput, scaleBiasTargets, scaleBiasOutput, 0, 0};

@@ -226,6 +226,25 @@ def test_layer_norm_undo_against_differences(f, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('f,n', [(2, 1 << 20), (16, 1 << 18)])
+def test_layer_norm_undo_sums_long_rows_in_short_chains(f, n):
+    """Equal terms, whose rounding errors all go the same way: the error of a row's sum is the number of additions one after the other
+    times u.  n / 1024 by a thread, 2 over the lanes of a row, 64 + 16 over the blocks' partial sums, and 2 u for the product and the output:
+    at most 340 u (one wave along the whole row would add n / 64 terms: 2590 u and 646 u for 0.1)."""
+    x = np.where(np.arange(f) % 2 == 0, 1, -1).astype(np.float32)[:, None] * np.ones((1, n), np.float32)
+    g = np.full((f, n), 0.1, np.float32)
+    r = np.float32(1 / np.sqrt(1 + EPS))
+    st = Out((2, n), np.stack([np.zeros(n), np.full(n, r)]))
+    dg, db = Out((f,)), Out((f,))
+    ws, size = need('mcn_layer_norm_undo_workspace_bytes', f, n)
+    keep = dev(g), dev(x), dev(np.ones(f, np.float32))
+    call('mcn_layer_norm_undo', *keep, st, None, dg, db, f, n, 0.0, 1.0, 0.0, 1.0, 0.0, 1.0, ws, size, None)
+    term = n * float(np.float32(0.1))
+    within(db.get(), np.full(f, term), 340 * U * term, 'dbias')
+    within(dg.get(), term * float(r) * x[:, 0].astype(np.float64), 340 * U * term, 'dgain')
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('n', [1, 4, 7, 3755])
 def test_layer_norm_of_two_features_rounds_like_the_formula(n):
     """With two features h - mean(h) - xh mean(h xh) cancels down to rounding errors: the same ones as of the formula in float32, one
