@@ -1024,8 +1024,9 @@ __global__ __launch_bounds__(256, SHARED ? 2 : 1) void k_fcl_grads(GradArgs p) {
     else weight_tile<SHARED>(p, blockIdx.x - p.inputBlocks, lds);
 }
 
-// ---- the end: input gradients from the slabs (blocks below dxBlocks), bias gradients from the tiles' row sums.  The packed weights of a
-// class that its bias takes out are zero; a case that has such a class for its label, and others left, still has the formula's
+// ---- the end: input gradients from the slabs (blocks below dxBlocks), bias gradients from the tiles' row sums.  A case that does not count,
+// or has no class left, gets zero whatever the weights hold (its dz is zero, but 0 times an infinity or NaN is not).  The packed weights of
+// a class that its bias takes out are zero; a case that has such a class for its label, and others left, still has the formula's
 // weights[label] * 1, and gets it here.
 struct FinishArgs {
     const float *slabs, *dbPart, *W, *bias, *labels, *stats;
@@ -1041,7 +1042,8 @@ __global__ __launch_bounds__(256) void k_fcl_finish(FinishArgs p) {
 #pragma unroll 8
             for (int s = 0; s < p.splits; s++) v += p.slabs[((size_t)s * p.Dp + d) * p.Np + n];
             int label;
-            if (p.bias && label_of(p.labels[n], p.V, label) && p.bias[label] == -INFINITY && p.stats[p.N + n] != 0.f) v += p.W[(size_t)label * p.D + d];
+            if (!label_of(p.labels[n], p.V, label) || p.stats[p.N + n] == 0.f) v = 0.f;
+            else if (p.bias && p.bias[label] == -INFINITY) v += p.W[(size_t)label * p.D + d];
             p.dX[i] = (p.scaleInputTargets != 0.f ? p.scaleInputTargets * p.dX[i] : 0.f) + p.coeff * v;
         }
         return;

@@ -552,6 +552,20 @@ def test_fc_logreg_masked_places_do_not_come_through(n, bad):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('bad', [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize('n', [6, 140])
+def test_fc_logreg_cases_that_do_not_count_have_no_gradient_whatever_the_weights_hold(n, bad):
+    """A class that takes part has a weight that is no number: the padded cases' input gradients are zero all the same, and added as such."""
+    d, v = 36, 500
+    w, x, b, lab = fcl_data(d, v, n, 34, padded=n // 3)
+    off = lab < 0
+    w[77, 5] = bad
+    assert not fcl_run(w, x, b, lab, 0.5)[3][:, off].any()
+    t = np.random.default_rng(3).standard_normal((d, n)).astype(np.float32)
+    assert np.array_equal(fcl_run(w, x, b, lab, 0.5, (0.5, 0.0, 1.0, 0.0, 1.0), (t, None, None))[3][:, off], np.float32(0.5) * t[:, off])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('n', [1, 6, 140])
 def test_fc_logreg_label_of_a_masked_class(n):
     """log p = -inf, and the gradients of the formula: the label's one stays, and takes that class's weights with it."""
