@@ -54,6 +54,10 @@ constexpr int TILE = 128;                    // columns of a product's tile
 constexpr float LO = 2048.f;                 // scale of the low piece
 constexpr int DZ_EXP = 14;                   // |dz / coeff| <= 1
 constexpr int EXP_ZERO = 1 << 20;            // a group of zeros: any scale will do
+// The exponents of the cases and of the groups of 32 classes are kept with a flag: whether the group holds an infinity or NaN.
+__device__ __forceinline__ int exp_odd(int e, bool odd) { return e * 2 + (odd ? 1 : 0); }
+__device__ __forceinline__ int exp_of(int eo) { return eo >> 1; }
+__device__ __forceinline__ bool is_odd(int eo) { return eo & 1; }
 
 __device__ __forceinline__ bool label_of(float l, int V, int& label) {
     const bool ok = l >= 0.f && l < (float)V;  // (false for a NaN)
@@ -311,10 +315,16 @@ __global__ __launch_bounds__(256) void k_fcl_cost(const float* __restrict__ labe
 // Both read 512 contiguous bytes a wave, without conflicts, and in both a lane's eight entries are 4 g + j and 16 + 4 g + j of the step's
 // 32, so that every pairing sums the same terms.  So W and dz are each stored once, and serve two products.
 
-// the power of two that brings a group of largest magnitude m to [2^14, 2^15); infinities and NaNs stay as they are
-__device__ __forceinline__ int scale_exp(float m) { return m > 0.f && m < INFINITY ? 14 - ilogbf(m) : 0; }
-__device__ __forceinline__ float max_or_nan(float m, float v) { return v > m || v != v ? v : m; }
+// the power of two that brings a group of largest finite magnitude m to [2^14, 2^15)
+__device__ __forceinline__ int scale_exp(float m) { return m > 0.f ? 14 - ilogbf(m) : 0; }
+__device__ __forceinline__ void max_finite(float& m, bool& odd, float v) {
+    const bool finite = v < INFINITY;  // (v >= 0; false for a NaN)
+    m = fmaxf(m, finite ? v : 0.f);
+    odd |= !finite;
+}
 
+// An infinity's pieces are infinite and NaN, and so are its products: right for the gradients, where a finite dz (0, or below 1 in size)
+// meets it, but not for the logits (odd_logits).
 // entries k = 16 h + 4 g + j (y[4 h + j]) of row c into a fragment pair, lane = 16 g + c
 __device__ __forceinline__ void store_pair(char* out, int lane, const float (&y)[8]) {
 #pragma unroll
@@ -564,10 +574,10 @@ __device__ __forceinline__ void product_tile_shared(const char* A, size_t aRow, 
 
 // ---- packing
 // What a pack launch makes, 512 threads a block: blocks below caseBlocks, 16 cases of x each (rows = cases, k = features) for the logits;
-// the next featBlocks, 16 features of x each (rows = features, k = cases) for the weight gradient, in which a case without a label is
-// zero, whatever it holds; the others, 32 classes of the piece each (rows = classes, k = features).
+// the next featBlocks, 16 features of x each (rows = features, k = cases) for the weight gradient, in which a case without a label, or
+// without a class left, is zero, whatever it holds; the others, 32 classes of the piece each (rows = classes, k = features).
 struct PackArgs {
-    const float *X, *labels;
+    const float *X, *labels, *stats;  // stats: for the features' blocks
     int *caseExp, *featExp;
     char *xByCase, *xByFeat;
     int D, V, N, Kd, Kn, caseBlocks, featBlocks;
@@ -582,17 +592,26 @@ struct PackArgs {
 __device__ __forceinline__ void pack_cases(const PackArgs& p, int block, float* sh, int* exps) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4, n = block * 16 + c;
     float m = 0.f;
+    bool odd = false;
     if (n < p.N) {
 #pragma unroll 8
-        for (int d = threadIdx.x >> 4; d < p.D; d += 32) m = max_or_nan(m, fabsf(p.X[(size_t)d * p.N + n]));
+        for (int d = threadIdx.x >> 4; d < p.D; d += 32) max_finite(m, odd, fabsf(p.X[(size_t)d * p.N + n]));
     }
-    m = max_or_nan(m, __shfl_xor(m, 16, 64));
-    m = max_or_nan(m, __shfl_xor(m, 32, 64));
+    float any = odd ? 1.f : 0.f;
+    for (int o = 16; o < 64; o <<= 1) {
+        m = fmaxf(m, __shfl_xor(m, o, 64));
+        any = fmaxf(any, __shfl_xor(any, o, 64));
+    }
     sh[wave * 16 + c] = m;
+    sh[128 + wave * 16 + c] = any;
     __syncthreads();
     if (threadIdx.x < 16) {
-        for (int w = 1; w < 8; w++) m = max_or_nan(m, sh[w * 16 + c]);
-        p.caseExp[n] = exps[c] = scale_exp(m);
+        for (int w = 1; w < 8; w++) {
+            m = fmaxf(m, sh[w * 16 + c]);
+            any = fmaxf(any, sh[128 + w * 16 + c]);
+        }
+        exps[c] = scale_exp(m);
+        p.caseExp[n] = exp_odd(exps[c], any != 0.f);
     }
     __syncthreads();
     const int e = exps[c];
@@ -607,19 +626,23 @@ __device__ __forceinline__ void pack_cases(const PackArgs& p, int block, float* 
     }
 }
 
+// (not without a label, and not without a class left)
+__device__ __forceinline__ bool has_gradient(const PackArgs& p, int n) {
+    int label;
+    return label_of(p.labels[n], p.V, label) && p.stats[p.N + n] != 0.f;
+}
 __device__ __forceinline__ void pack_feats(const PackArgs& p, int block, int* exps) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4, d0 = block * 16, r = threadIdx.x >> 5;
     float m = 0.f;
+    bool odd = false;
     if (d0 + r < p.D) {
 #pragma unroll 4
         for (int n = threadIdx.x & 31; n < p.N; n += 32) {
-            int label;
-            const bool counts = label_of(p.labels[n], p.V, label);
             const float v = fabsf(p.X[(size_t)(d0 + r) * p.N + n]);
-            m = counts ? max_or_nan(m, v) : m;
+            if (has_gradient(p, n)) max_finite(m, odd, v);
         }
     }
-    for (int o = 1; o < 32; o <<= 1) m = max_or_nan(m, __shfl_xor(m, o, 64));
+    for (int o = 1; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
     if ((threadIdx.x & 31) == 0) p.featExp[d0 + r] = exps[r] = scale_exp(m);
     __syncthreads();
     const int d = d0 + c, e = exps[c];
@@ -628,8 +651,7 @@ __device__ __forceinline__ void pack_feats(const PackArgs& p, int block, int* ex
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int n = kb * 32 + (j >> 2) * 16 + g * 4 + (j & 3);
-            int label;
-            y[j] = d < p.D && n < p.N && label_of(p.labels[n], p.V, label) ? ldexpf(p.X[(size_t)d * p.N + n], e) : 0.f;
+            y[j] = d < p.D && n < p.N && has_gradient(p, n) ? ldexpf(p.X[(size_t)d * p.N + n], e) : 0.f;
         }
         store_pair(p.xByFeat + ((size_t)block * p.Kn + kb) * PAIR, lane, y);
     }
@@ -644,7 +666,7 @@ constexpr int CW = 512, CW_LD = CW + 4;
 // magnitudes of a case add up to 2 at most), so with this bound on the exponents no weights below 2^48 take it out of range.  It
 // leaves a group whose largest weight is below 2^-50 with less than 22 bits below 2^-78.
 constexpr int CLASS_EXP_MAX = 64;
-constexpr int PACK_LDS = (32 * CW_LD + 8) * 4;
+constexpr int PACK_LDS = (32 * CW_LD + 16) * 4;
 __device__ __forceinline__ void pack_classes(const PackArgs& p, int block, float* tile) {
     float* maxima = tile + 32 * CW_LD;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, v0 = block * 32, c = lane & 15, g = lane >> 4, D = p.D;
@@ -676,7 +698,7 @@ __device__ __forceinline__ void pack_classes(const PackArgs& p, int block, float
                 t[r][h] = x;
             }
     };
-    float m = 0.f;
+    float m = 0.f, zero = 0.f;  // zero: a NaN once an infinity or NaN has been met
     for (int d0 = 0; d0 < D; d0 += CW) {
         load(d0);
 #pragma unroll
@@ -684,10 +706,19 @@ __device__ __forceinline__ void pack_classes(const PackArgs& p, int block, float
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) m = max_or_nan(m, fabsf(t[r][h][j]));
+                for (int j = 0; j < 4; j++) {
+                    m = fmaxf(m, fabsf(t[r][h][j]));
+                    zero = fmaf(t[r][h][j], 0.f, zero);
+                }
     }
-    for (int o = 1; o < 64; o <<= 1) m = max_or_nan(m, __shfl_xor(m, o, 64));
-    if (lane == 0) maxima[wave] = m;
+    for (int o = 1; o < 64; o <<= 1) {
+        m = fmaxf(m, __shfl_xor(m, o, 64));
+        zero += __shfl_xor(zero, o, 64);
+    }
+    if (lane == 0) {
+        maxima[wave] = m;
+        maxima[8 + wave] = zero;
+    }
     int e = 0;
     for (int d0 = 0; d0 < p.Kd * 32; d0 += CW) {
         if (D > CW) load(d0);
@@ -697,9 +728,31 @@ __device__ __forceinline__ void pack_classes(const PackArgs& p, int block, float
 #pragma unroll
             for (int h = 0; h < 2; h++) *reinterpret_cast<f32x4*>(tile + (wave * 4 + r) * CW_LD + h * 256 + lane * 4) = t[r][h];
         if (d0 == 0) {
-            for (int w = 0; w < 8; w++) m = max_or_nan(m, maxima[w]);  // (every wave: the barrier above covers the maxima)
+            for (int w = 0; w < 8; w++) {  // (every wave: the barrier above covers the maxima)
+                m = fmaxf(m, maxima[w]);
+                zero += maxima[8 + w];
+            }
+            const bool odd = zero != zero;  // the same for all threads
+            if (odd) {                      // the finite ones' maximum; the first features are in the tile already
+                m = 0.f;
+                bool met = false;
+                for (int d = 0; d < D; d += CW) {
+                    load(d);
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++)
+#pragma unroll
+                            for (int j = 0; j < 4; j++) max_finite(m, met, fabsf(t[r][h][j]));
+                }
+                for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+                __syncthreads();
+                if (lane == 0) maxima[wave] = m;
+                __syncthreads();
+                for (int w = 0; w < 8; w++) m = fmaxf(m, maxima[w]);
+            }
             e = min(scale_exp(m) & ~7, CLASS_EXP_MAX);
-            if (threadIdx.x == 0) p.classExp[block] = m == 0.f ? EXP_ZERO : e;
+            if (threadIdx.x == 0) p.classExp[block] = exp_odd(m == 0.f ? EXP_ZERO : e, odd);
         }
         __syncthreads();
         for (int f = wave; f < 2 * CW / 32; f += 8) {
@@ -730,13 +783,39 @@ __global__ __launch_bounds__(512) void k_fcl_pack(PackArgs p) {
 struct WideArgs {
     const char *wByClass, *xByCase;
     const int *classExp, *caseExp;
-    const float *bias, *labels, *stats;
-    int V, N, v0, rows, Kd, kSteps, vTiles, nTiles;
+    const float *W, *X, *bias, *labels, *stats;
+    int D, V, N, v0, rows, Kd, kSteps, vTiles, nTiles;
     float *part, *labelLogits;  // forward: part + the piece's first tile
     char* dz;                   // backward: dz / coeff, (rows = cases, k = classes)
     float* dbPart;              // backward: [nTiles][V], row sums of dz / coeff
     int Kv;
 };
+
+// Logits whose weights or inputs hold an infinity or NaN: the products of pieces make a NaN of any of them, where the formula has the sum
+// of the terms that are not finite (all of one sign: that infinity).  Where an infinite input meets the zeros of a class that is taken
+// out, too.  Rare: a lane's entries lie in LDS, 256 floats apart, and are gone through one by one.
+typedef const __attribute__((address_space(4))) WideArgs* LateArgs;
+template <int MB>
+__device__ __forceinline__ void odd_logits(LateArgs p, float* z, int vFirst, int nFirst) {
+#pragma unroll 1
+    for (int e = 0; e < 16 * MB; e++, z += 256) {
+        const int v = vFirst + (e >> 4) * 16 + (e & 3), n = nFirst + ((e >> 2) & 3) * 16;
+        const float bv = v < p->rows ? (p->bias ? p->bias[p->v0 + v] : 0.f) : -INFINITY;
+        const float was = *z;
+        const bool look = n < p->N && bv != -INFINITY && was != was;
+        if (bv == -INFINITY) *z = -INFINITY;
+        if (!__any(look)) continue;
+        float s = 0.f;
+        const float *w = p->W + (size_t)(p->v0 + v) * p->D, *x = p->X + n;
+        for (int d = 0; d < p->D && __any(look && s == s); d++) {
+            if (look) {
+                const float a = w[d], b = x[(size_t)d * p->N];
+                if (!(fabsf(a) < INFINITY && fabsf(b) < INFINITY)) s += a * b;
+            }
+        }
+        if (look && s != 0.f) *z = s + bv;
+    }
+}
 
 // SHARED: two blocks per CU (MB = 4).  512 x 100000 x 1024: forward 346 us, 909 TFLOP/s of fp16 products, backward, which writes dz,
 // 393 us, 800; a large library product of fp16 operands reaches 1126.
@@ -757,16 +836,20 @@ __global__ __launch_bounds__(256, SHARED ? 2 : 1) void k_fcl_logits(WideArgs p) 
     const int vBase = tv * 32 * MB + wm * 16 * MB, nBase = tn * TILE + wn * 64;
     // z in place of the first accumulator.  A class behind the last one, or taken out by its bias, has fragments of zeros: -inf.
     int ex[4], label[4];
+    bool odd = false;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const int n = nBase + j * 16 + c;
-        ex[j] = p.caseExp[n];
+        const int eo = p.caseExp[n];
+        ex[j] = exp_of(eo);
+        odd |= is_odd(eo);
         label[j] = -1;
         if (n < p.N) label_of(p.labels[n], p.V, label[j]);
     }
 #pragma unroll
     for (int i = 0; i < MB; i++) {
-        const int we = p.classExp[(vBase + i * 16) / 32], ew = we == EXP_ZERO ? 0 : we;
+        const int eo = p.classExp[(vBase + i * 16) / 32], we = exp_of(eo), ew = we == EXP_ZERO ? 0 : we;
+        odd |= is_odd(eo);
         float bv[4];
 #pragma unroll
         for (int r = 0; r < 4; r++) {
@@ -777,6 +860,18 @@ __global__ __launch_bounds__(256, SHARED ? 2 : 1) void k_fcl_logits(WideArgs p) 
         for (int j = 0; j < 4; j++)
 #pragma unroll
             for (int r = 0; r < 4; r++) acc.c[0][i][j][r] = ldexpf(acc.value(i, j, r), -(ew + ex[j])) + bv[r];
+    }
+    if (__builtin_expect(__any(odd), 0)) {  // (the stages' LDS is free)
+        static_assert(16 * MB * 256 * 4 <= (SHARED ? SHARED_LDS : tile_lds(MB)), "the tile's logits in the stages' LDS");
+        float* mine = reinterpret_cast<float*>(lds) + threadIdx.x;
+#pragma unroll
+        for (int k = 0; k < 16 * MB; k++) mine[k * 256] = acc.c[0][k >> 4][(k >> 2) & 3][k & 3];
+        // arguments that only this branch needs are loaded in it: with their loads moved to the front 512 x 10575, 509 cases, took 28.5 us for 24.1
+        LateArgs late = (LateArgs)__builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+s"(late));
+        odd_logits<MB>(late, mine, vBase + g * 4, nBase + c);
+#pragma unroll
+        for (int k = 0; k < 16 * MB; k++) acc.c[0][k >> 4][(k >> 2) & 3][k & 3] = mine[k * 256];
     }
     // where the label's entry lies among a lane's 4 MB rows, if it does: row 16 i + r from here
     int at[4];
@@ -966,7 +1061,7 @@ struct CarryScale {
     __device__ __forceinline__ CarryScale(const int* e, int n) : exps(e), count(n), held(load(0)), cur(EXP_ZERO) {}
     __device__ __forceinline__ int load(int t) const {
         const int i = t + (int)(threadIdx.x & 63);
-        return i < count ? exps[i] : EXP_ZERO;
+        return i < count ? exp_of(exps[i]) : EXP_ZERO;
     }
     template <int MB>
     __device__ __forceinline__ void operator()(int t, Acc<MB>& acc) const {
@@ -1154,8 +1249,11 @@ void launch_logits(TileKind kind, const WideArgs& a, hipStream_t s) {
     else MCN_LAUNCH((k_fcl_logits<2, BWD, false>), grid, block, tile_bytes(HALF), s, a);
 }
 
-WideArgs wide_args(const WidePlan& q, const float* bias, const float* labels, int V, int N, char* ws) {
+WideArgs wide_args(const WidePlan& q, const float* W, const float* X, const float* bias, const float* labels, int D, int V, int N, char* ws) {
     WideArgs a = {};
+    a.W = W;
+    a.X = X;
+    a.D = D;
     a.wByClass = ws + q.wByClass;
     a.xByCase = ws + q.xByCase;
     a.classExp = (const int*)(ws + q.classExp);
@@ -1182,9 +1280,9 @@ TileKind wide_piece(const WidePlan& q, WideArgs& a, PackArgs& k, const float* W,
     k.caseBlocks = k.featBlocks = 0;
     return kind;
 }
-PackArgs pack_args(const WidePlan& q, const float* X, const float* labels, int D, int V, int N, bool feats, char* ws) {
+PackArgs pack_args(const WidePlan& q, const float* X, const float* labels, const float* stats, int D, int V, int N, bool feats, char* ws) {
     PackArgs k = {};
-    k.X = X; k.labels = labels;
+    k.X = X; k.labels = labels; k.stats = stats;
     k.caseExp = (int*)(ws + q.caseExp); k.featExp = (int*)(ws + q.featExp);
     k.xByCase = ws + q.xByCase; k.xByFeat = ws + q.xByFeat;
     k.D = D; k.V = V; k.N = N; k.Kd = q.Kd; k.Kn = q.Kn;
@@ -1196,9 +1294,9 @@ PackArgs pack_args(const WidePlan& q, const float* X, const float* labels, int D
 int wide_cost(const float* W, const float* X, const float* bias, const float* labels, float* stats, float* logp, float* correct, int D, int V,
               int N, char* ws, hipStream_t s) {
     const WidePlan q = wide_plan(D, V, N, false);
-    WideArgs a = wide_args(q, bias, labels, V, N, ws);
+    WideArgs a = wide_args(q, W, X, bias, labels, D, V, N, ws);
     a.labelLogits = (float*)(ws + q.labelLogits);
-    PackArgs pack = pack_args(q, X, labels, D, V, N, false, ws);
+    PackArgs pack = pack_args(q, X, labels, nullptr, D, V, N, false, ws);
     int tiles = 0;
     for (int v0 = 0; v0 < V; v0 += a.rows) {
         const TileKind kind = wide_piece(q, a, pack, W, D, v0, s);
@@ -1215,13 +1313,13 @@ int wide_grad(const float* W, const float* X, const float* bias, const float* la
               int V, int N, float coeff, float scaleInputTargets, float scaleWeightTargets, float scaleWeightOutput, float scaleBiasTargets,
               float scaleBiasOutput, char* ws, hipStream_t s) {
     const WidePlan q = wide_plan(D, V, N, true);
-    WideArgs a = wide_args(q, bias, labels, V, N, ws);
+    WideArgs a = wide_args(q, W, X, bias, labels, D, V, N, ws);
     a.stats = stats;
     a.dz = ws + q.dz;
     a.dbPart = dB ? (float*)(ws + q.dbPart) : nullptr;
     float* slabs = (float*)(ws + q.slabs);
     const bool narrow = !wide_cost_usable(N);  // (the forward call's logits, to the bit)
-    PackArgs pack = pack_args(q, X, labels, D, V, N, dW != nullptr, ws);
+    PackArgs pack = pack_args(q, X, labels, stats, D, V, N, dW != nullptr, ws);
     if (narrow) pack.caseBlocks = 0;
     NarrowArgs few = {W, X, bias, labels, D, V, N};
     few.stats = stats; few.dz = a.dz; few.dbPart = a.dbPart;

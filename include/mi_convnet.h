@@ -608,7 +608,8 @@ int mcn_counter_add(uint64_t* counter, uint64_t by, void* stream);
  *   caseStats (2, numCases) = max_v z, then sum_v exp(z - max);  labelLogProbs = log p[label];
  *   correctProbs = (z[label] is the max) / (number of entries at the max);
  *   costOut (device doubles, may be NULL): [0] += -sum(labelLogProbs), [1] += cases that count - sum(correctProbs).
- * A case all of whose classes are -inf has statistics (-inf, 0), log probability -inf and no gradient.  What the weights of a class
+ * Infinite weights and inputs go by the formula, whatever the number of cases: a logit of -inf takes its class out of that case.  A case
+ * all of whose classes are at -inf has statistics (-inf, 0), log probability -inf and no gradient.  What the weights of a class
  * that is taken out hold, or the inputs of a case that does not count, comes through nowhere, except for such a case's own statistics.
  * numOutputs from 1 to 2^24 (labels are fp32), numInputs and numCases to 2^20, numInputs * numCases to 2^34.  No output overlaps an operand
  * or another output (MCN_EINVAL).  Workspaces as for mcn_layer_norm; backward != 0: for both calls, 0: the cost alone. */

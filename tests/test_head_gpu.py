@@ -565,6 +565,86 @@ def test_fc_logreg_cases_that_do_not_count_have_no_gradient_whatever_the_weights
     assert np.array_equal(fcl_run(w, x, b, lab, 0.5, (0.5, 0.0, 1.0, 0.0, 1.0), (t, None, None))[3][:, off], np.float32(0.5) * t[:, off])
 
 
+def fcl_check(ref, got, cases, feats):
+    """Statistics and costs of `cases`, gradients of `feats`, against a reference."""
+    st, lp, ok, dx, dw, db, _ = got
+    within(st[:, cases], np.stack([ref['top'], ref['tot']])[:, cases], np.stack([ref['ez'] + 2 * U * np.abs(ref['top']), ref['tot'] * ref['er']])[:, cases], 'stats')
+    within(lp[cases], ref['logp'][cases], (2 * ref['er'] + 4 * U * np.abs(ref['logp']))[cases], 'logp')
+    within(dx[feats][:, cases], ref['dx'][feats][:, cases], ref['edx'][feats][:, cases], 'dx')
+    within(dw, ref['dw'], ref['edw'], 'dw')
+    within(db, ref['db'], ref['edb'], 'db')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('d,v,n', [(36, 500, 6), (36, 500, 64), (36, 500, 65), (36, 500, 140), (600, 300, 70), (40, 9000, 520)])
+def test_fc_logreg_minus_infinite_logits_of_live_classes(d, v, n):
+    """Weights of -inf against positive inputs: the class is out as one with a bias of -inf is, on either side of the number of cases
+    that takes the other products; only its own features' input gradients are 0 * inf.  Its neighbours' small weights keep their bits."""
+    w, x, b, lab = fcl_data(d, v, n, 35, padded=n // 4)
+    x[3:6] = np.abs(x[3:6]) + 0.1
+    out = np.array([50, 51, v - 1])
+    w[52:60] *= 1e-6
+    lab[np.isin(lab, out)] = 1
+    w0, b0 = w.copy(), b.copy()
+    w0[out], b0[out] = 0, -np.inf
+    w[50, 3], w[51, 4:6], w[v - 1, 3:6] = -np.inf, -np.inf, -np.inf
+    ref = fcl_ref(w0, x, b0, lab, 0.5)
+    got = fcl_run(w, x, b, lab, 0.5)
+    feats = np.array([k for k in range(d) if k not in (3, 4, 5)])
+    fcl_check(ref, got, slice(None), feats)
+    on = lab >= 0
+    assert np.isnan(got[3][3:6][:, on]).all() and not got[3][:, ~on].any()
+    assert not got[4][out].any() and not got[5][out].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n', [6, 140])
+def test_fc_logreg_infinities_that_leave_no_number(n):
+    """A logit of +inf, and infinities of both signs in one logit: no finite cost, and only for the cases that have them."""
+    d, v = 36, 500
+    w, x, b, lab = fcl_data(d, v, n, 36)
+    x[3:5] = np.abs(x[3:5]) + 0.1
+    x[5, ::2], x[5, 1::2] = 1, -1
+    for k, (at, val) in enumerate([((60, 3), np.inf), ((60, slice(3, 5)), [np.inf, -np.inf])]):
+        w2 = w.copy()
+        w2[at] = val
+        st, lp, ok, *_ = fcl_run(w2, x, b, lab)
+        assert np.isnan(lp).all() and np.isnan(st[1]).all()
+    w2 = w.copy()
+    w2[60, 5] = np.inf  # +inf for the even cases, -inf for the odd ones
+    lab[lab == 60] = 61
+    b0 = b.copy()
+    b0[60] = -np.inf
+    ref = fcl_ref(w, x, b0, lab, 1.0)
+    st, lp, ok, dx, dw, db, _ = fcl_run(w2, x, b, lab)
+    assert np.isnan(lp[::2]).all()
+    within(lp[1::2], ref['logp'][1::2], (2 * ref['er'] + 4 * U * np.abs(ref['logp']))[1::2], 'logp')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n', [6, 140])
+def test_fc_logreg_infinite_inputs(n):
+    """An input of +inf against negative weights takes every class out: the case has statistics (-inf, 0) and no gradient, and the others
+    do not see it.  One with classes taken out by their bias as well, whose weights count for nothing."""
+    d, v = 36, 500
+    w, x, b, lab = fcl_data(d, v, n, 37)
+    w[:, 5] = -np.abs(w[:, 5]) - 0.01
+    b[100:140] = -np.inf
+    w[100:140, 5] = 1
+    lab[(lab >= 100) & (lab < 140)] = 7
+    bad = np.array([1, n - 1])
+    x0, lab0 = x.copy(), lab.copy()
+    x0[5, bad], lab0[bad] = 0, -1
+    x[5, bad] = np.inf
+    ref = fcl_ref(w, x0, b, lab0, 0.5)
+    got = fcl_run(w, x, b, lab, 0.5)
+    others = np.array([k for k in range(n) if k not in bad])
+    fcl_check(ref, got, others, np.arange(d))
+    st, lp, ok, dx, dw, db, cost = got
+    assert np.all(st[0, bad] == -np.inf) and not st[1, bad].any() and np.all(lp[bad] == -np.inf) and not ok[bad].any()
+    assert not dx[:, bad].any()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize('n', [1, 6, 140])
 def test_fc_logreg_label_of_a_masked_class(n):
