@@ -1885,6 +1885,11 @@ ConvNet::ConvNet(const std::vector<Params>& layers, int minibatchSize, int devic
     }
     for (auto& l : _layers)
         for (Layer* p : l->prev()) p->addNext(l.get());
+    std::map<uint64_t, std::string> seeds;  // (the same seed is the same masks)
+    for (auto& l : _layers)
+        if (auto* d = dynamic_cast<DropoutLayer*>(l.get()))
+            if (!seeds.emplace(d->seed(), l->name()).second)
+                throw NetError("layer '" + l->name() + "': its seed is layer '" + seeds[d->seed()] + "'s, and would give the same masks");
     for (auto& l : _layers)
         if (l->type() == "classifier" && (l->prev().size() != 1 || l->next().size() != 1 || l->next()[0]->type() != "cost.logreg" ||
                                           l->next()[0]->prev().size() != 2 || l->next()[0]->prev()[1] != l.get()))

@@ -262,6 +262,7 @@ class DropoutLayer : public Layer {
    public:
     DropoutLayer(ConvNet* net, const Params& p);
     ~DropoutLayer() override;
+    uint64_t seed() const { return _seed; }
     void allocate(int maxCases) override;
     void copyToCPU() override;
     void copyToGPU() override;

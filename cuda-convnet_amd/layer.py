@@ -330,7 +330,10 @@ def _parse_dropout(name, cfg, prev, ctx):
     dic['dropout'] = cfg.get_float(name, 'dropout')
     _check(0 <= dic['dropout'] < 1, "Layer '%s': parameter 'dropout' must be in [0, 1)" % name)
     seed = cfg.get_int(name, 'seed', default=-1)
+    _check(seed < 1 << 63, "Layer '%s': parameter 'seed' must be below 2^63" % name)
     dic['seed'] = int(ctx.rng.integers(1 << 62)) if seed < 0 else seed
+    for l in prev:
+        _check(l['type'] != 'dropout' or l['seed'] != dic['seed'], "Layer '%s': seed %d is layer '%s's, and would give the same masks" % (name, dic['seed'], l['name']))
     dic['steps'] = np.zeros((1, 3), dtype=np.float32)  # minibatches drawn for so far, in base 2^20: a checkpoint goes on with new masks
     dic['usesActs'] = dic['usesInputs'] = False
     dic['forceOwnActs'] = prev[dic['inputs'][0]]['type'] == 'data'  # never in the data batch itself

@@ -45,6 +45,20 @@ def test_dropout_key_of_other_layers_stays_without_effect(tmp_path):
     assert [(l['name'], l['type']) for l in parse(str(p))] == [(l['name'], l['type']) for l in parse()]
 
 
+def test_dropout_layers_differ_in_their_seed(tmp_path):
+    """The mask follows from (seed, step, element) alone: the same seed twice would drop the same elements in both layers."""
+    src = open(CFG).read().replace('inputs=drop1', 'inputs=drop2').replace('[id]', '[drop2]\ntype=dropout\ninputs=drop1\ndropout=0.2\nseed=%d\n\n[id]')
+    p = tmp_path / 'a.cfg'
+    p.write_text(src % 77)
+    with pytest.raises(layer.LayerParsingError, match="'drop2': seed 77 is layer 'drop1's"):
+        parse(str(p))
+    p.write_text(src % 78)
+    assert [l['seed'] for l in parse(str(p)) if l['type'] == 'dropout'] == [77, 78]
+    p.write_text(src % (1 << 63))
+    with pytest.raises(layer.LayerParsingError, match='below 2'):
+        parse(str(p))
+
+
 @pytest.mark.parametrize('edit,msg', [
     (('dropout=0.4', 'dropout=1.0'), 'must be in'),
     (('dropout=0.4', 'dropout=-0.1'), 'must be in'),

@@ -321,3 +321,16 @@ def test_classifier_refusals():
     with pytest.raises(RuntimeError, match='classifier layer'):
         with Native(bad, 32):
             pass
+
+
+def test_dropout_layers_with_one_seed_are_refused(tmp_path):
+    src = open(CFG).read().replace('inputs=drop1', 'inputs=drop2').replace('[id]', '[drop2]\ntype=dropout\ninputs=drop1\ndropout=0.2\nseed=78\n\n[id]')
+    p = tmp_path / 'a.cfg'
+    p.write_text(src)
+    _, L = net(32, str(p))
+    with Native(copy.deepcopy(L), 32):
+        pass
+    [l for l in L if l['name'] == 'drop2'][0]['seed'] = 77
+    with pytest.raises(RuntimeError, match="its seed is layer 'drop1's"):
+        with Native(L, 32):
+            pass
