@@ -95,3 +95,33 @@ def test_ranks_on_one_gpu_equal_the_single_gpu_step(name, steps, world, tmp_path
         assert abs(got[0] - v[0]) <= 2e-4 * abs(v[0]) + 1e-6, (k, got, v)
         if k == 'logprob':
             assert got[1] == v[1]   # error counts are integers
+
+
+def test_ranks_draw_masks_of_their_own(tmp_path):
+    """The head preset on two ranks: replicas stay bit-identical, and every rank's cost is the one of a single run on its shard with the
+    seed seed + 0x9E3779B97F4A7C15 rank; the increments are the mean of the two runs' (one step: 1e-4 of a matrix's largest entry)."""
+    from cuda_convnet_amd.data import shard_for_rank
+    ranks = run_ranks('deepid-head', 1, tmp_path)
+    for k in ranks[0].files:
+        if '.' in k and not k.startswith('cost.'):
+            assert np.array_equal(ranks[0][k], ranks[1][k]), '%s differs between the ranks' % k
+    runs, costs = [], []
+    for r, mask in ((0, 0), (1, 1), (1, 0)):
+        dp, L = preset('deepid-head', 256, minibatch=256)
+        drop = [l for l in L if l['type'] == 'dropout'][0]
+        seed = (drop['seed'] + 0x9E3779B97F4A7C15 * mask) % (1 << 64)
+        drop['seed'] = seed - (1 << 64) if seed >= 1 << 63 else seed
+        with Native(L, minibatch=128) as lib:
+            lib.startBatch(shard_for_rank(dp.get_next_batch()[2], r, 2, 128), 0)
+            costs.append(lib.finishBatch()[0]['logprob'])
+            lib.syncWithHost()
+        runs.append(L)
+    for r in range(2):
+        got = ranks[r]['cost.logprob']
+        assert abs(got[0] - costs[r][0]) <= 1e-6 * abs(costs[r][0]) and got[1] == costs[r][1]
+    assert abs(ranks[1]['cost.logprob'][0] - costs[2][0]) > 1e-5 * abs(costs[2][0])  # (not rank 0's masks)
+    for l, m in zip(runs[0], runs[1]):
+        if 'weights' in l:
+            for i, (p, q) in enumerate(zip(l['weightsInc'], m['weightsInc'])):
+                close_but_for_decisions(ranks[0]['%s.inc%d' % (l['name'], i)], (p + q) / 2, 1e-4, l['name'])
+            close_but_for_decisions(ranks[0]['%s.binc' % l['name']], (l['biasesInc'] + m['biasesInc']) / 2, 1e-4, l['name'] + ' biases')

@@ -334,3 +334,22 @@ def test_dropout_layers_with_one_seed_are_refused(tmp_path):
     with pytest.raises(RuntimeError, match="its seed is layer 'drop1's"):
         with Native(L, 32):
             pass
+
+
+@pytest.mark.parametrize('env', [{}, {'MCN_NO_GRAD_STREAM': '1'}, {'MCN_NO_FUSION': '1'}, 'data parallel'])
+def test_classifier_beside_a_verification_cost(tmp_path, env):
+    """DeepID2's own net with its fc6 and softmax as a classifier layer: the features get the identification's and the verification's
+    gradients, the latter from another stream.  Three minibatches against the layers it stands for."""
+    from cuda_convnet_amd import CFG_DIR
+    text = open(os.path.join(CFG_DIR, 'deepid2_10575.cfg')).read()
+    a, b = text.index('[fc6]'), text.index('[logprob]')
+    text = text[:a] + '[fc6]\ntype=classifier\noutputs=10575\ninputs=fc5\ninitW=0.01\n\n' + text[b:].replace('labels,probs', 'labels,fc6')
+    p = tmp_path / 'joint.cfg'
+    p.write_text(text)
+    dp, La = build(str(p), os.path.join(CFG_DIR, 'deepid_params.cfg'), 'deepid2', (55, 55, 3), 384)
+    _, Lb = preset('deepid2', 384)
+    data = dp.get_next_batch()[2]
+    forced = env == 'data parallel'
+    a, b = (run(L, data, {} if forced else env, minibatch=128, dp=forced) for L in (La, Lb))
+    check_costs(a, b)
+    check_weights(La, [l for l in Lb if l['type'] != 'softmax'])
