@@ -1266,10 +1266,12 @@ WideArgs wide_args(const WidePlan& q, const float* W, const float* X, const floa
     a.kSteps = q.kSteps;
     return a;
 }
+// the classes of the piece that begins at v0
+int piece_rows(const WidePlan& q, int V, int v0) { return V - v0 <= q.last ? V - v0 : q.rows; }
 // one piece: its packed rows, tiles and k blocks; with the first one, x
 TileKind wide_piece(const WidePlan& q, WideArgs& a, PackArgs& k, const float* W, int D, int v0, hipStream_t s) {
     a.v0 = v0;
-    a.rows = k.rows = a.V - v0 <= q.last ? a.V - v0 : q.rows;
+    a.rows = k.rows = piece_rows(q, a.V, v0);
     a.nTiles = q.nTiles;
     a.Kv = divup(a.rows, TILE) * 4;
     const TileKind kind = tile_choice(a.Kv, q.nTiles);
@@ -1290,6 +1292,13 @@ PackArgs pack_args(const WidePlan& q, const float* X, const float* labels, const
     k.classExp = (int*)(ws + q.classExp); k.wByClass = ws + q.wByClass;
     return k;
 }
+
+// k blocks of a share of a piece's input gradient: the last piece has no more shares than there are slabs, and a short one fewer, not
+// shorter ones
+int piece_share(const WidePlan& q, int Kv) { return Kv == q.Kv ? q.kPerSplit : std::max(8, divup(Kv, q.splits)); }
+// two blocks a CU once there is more than one for each; one with its stages further ahead / two: 512 x 4213 x 128, all gradients,
+// 39.9 / 41.5 us; 512 x 10575 x 128 53 / 50 us
+bool grads_shared(int blocks) { return blocks > 256; }
 
 int wide_cost(const float* W, const float* X, const float* bias, const float* labels, float* stats, float* logp, float* correct, int D, int V,
               int N, char* ws, hipStream_t s) {
@@ -1340,17 +1349,14 @@ int wide_grad(const float* W, const float* X, const float* bias, const float* la
         } else {
             launch_logits<true>(kind, a, s);
         }
-        // (the last piece has no more shares of the input gradient than there are slabs, and a short one fewer, not shorter ones)
-        t.kPerSplit = a.Kv == q.Kv ? q.kPerSplit : std::max(8, divup(a.Kv, q.splits));
+        t.kPerSplit = piece_share(q, a.Kv);
         t.inputBlocks = dX ? divup(a.Kv, t.kPerSplit) * q.nTiles * q.dTiles : 0;
         t.dW = dW ? dW + (size_t)v0 * D : nullptr;
         t.rows = a.rows;
         t.Kv = a.Kv;
         t.first = v0 == 0;
         const int blocks = t.inputBlocks + (dW ? a.Kv / 4 * q.dTiles : 0);
-        // (two blocks a CU once there is more than one for each; one with its stages further ahead / two: 512 x 4213 x 128, all gradients,
-        // 39.9 / 41.5 us; 512 x 10575 x 128 53 / 50 us)
-        if (blocks > 256) MCN_LAUNCH(k_fcl_grads<true>, dim3(blocks), dim3(256), tile_bytes(SHARED), s, t);
+        if (grads_shared(blocks)) MCN_LAUNCH(k_fcl_grads<true>, dim3(blocks), dim3(256), tile_bytes(SHARED), s, t);
         else if (blocks > 0) MCN_LAUNCH(k_fcl_grads<false>, dim3(blocks), dim3(256), tile_bytes(WHOLE), s, t);
         if (int rc = MCN_LAUNCH_CHECK("fcLogregGrad")) return rc;
     }
@@ -1435,3 +1441,26 @@ MCN_API int mcn_fc_logreg_grad(const float* weights, const float* inputs, const 
                      scaleInputTargets, scaleWeightTargets, scaleWeightOutput, scaleBiasTargets, scaleBiasOutput, (char*)workspace,
                      (hipStream_t)stream);
 }
+
+#ifdef MCN_TEST_HOOKS
+// What the pieces of a call take, so that a test knows which forms it runs: five numbers for each of the first `most` pieces (classes, tiles
+// of the logits as in TileKind, or 3 for few cases, k blocks of a share of the input gradient, shares, 1 where all gradients' tiles go
+// two to a CU).  The number of pieces.
+MCN_API int mcn_fc_logreg_test_forms(int numInputs, int numOutputs, int numCases, int backward, int* out, int most) {
+    if (!fcl_sizes_ok(numInputs, numOutputs, numCases)) return 0;
+    const WidePlan q = wide_plan(numInputs, numOutputs, numCases, backward != 0);
+    int pieces = 0;
+    for (int v0 = 0, rows; v0 < numOutputs; v0 += rows, pieces++) {
+        rows = piece_rows(q, numOutputs, v0);
+        const int Kv = divup(rows, TILE) * 4, share = piece_share(q, Kv), shares = divup(Kv, share);
+        if (pieces >= most) continue;
+        int* o = out + 5 * pieces;
+        o[0] = rows;
+        o[1] = wide_cost_usable(numCases) ? (int)tile_choice(Kv, q.nTiles) : 3;
+        o[2] = share;
+        o[3] = shares;
+        o[4] = grads_shared(shares * q.nTiles * q.dTiles + Kv / 4 * q.dTiles);
+    }
+    return pieces;
+}
+#endif

@@ -4,6 +4,7 @@ Tolerances: u = 2^-24 is the largest relative rounding error of one fp32 operati
 u each, in any order, is off by at most k u sum|terms| and, with errors of either sign, by LAMBDA sqrt(k) u sum|terms| but for a
 negligible share of inputs (Higham and Mary, "A new approach to probabilistic rounding error analysis", 2019; LAMBDA = 8)."""
 import ctypes as C
+import os
 
 import numpy as np
 import pytest
@@ -442,6 +443,40 @@ def test_fc_logreg(d, v, n):
     within(got[3], t[0] + ref['dx'], ref['edx'] + 4 * U * (np.abs(t[0]) + np.abs(ref['dx'])), 'dx added')
     within(got[4], 0.9 * t[1] + 0.5 * ref['dw'], 0.5 * ref['edw'] + 4 * U * (np.abs(t[1]) + np.abs(ref['dw'])), 'dw added')
     within(got[5], 0.25 * t[2] - 2 * ref['db'], 2 * ref['edb'] + 4 * U * (np.abs(t[2]) + 2 * np.abs(ref['db'])), 'db added')
+
+
+def fcl_forms(d, v, n, backward):
+    """(classes, tiles of the logits, k blocks of a share of the input gradient, shares, gradients' tiles two to a CU) of every piece."""
+    lib = C.CDLL(os.path.join(os.path.dirname(capi.LIB_PATH), 'libmiconvnet_hooks.so'))  # (the test build: the same rules)
+    out = (C.c_int * 50)()
+    return [tuple(out[5 * i:5 * i + 5]) for i in range(lib.mcn_fc_logreg_test_forms(d, v, n, backward, out, 10))]
+
+
+SHARED, WHOLE, HALF, FEW = range(4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('d,v,n,logits,steps,shared', [
+    (160, 10575, 509, SHARED, 9, True),
+    (96, 10575, 509, SHARED, 9, False),   # two tiles a CU, several tiles of cases, the last of them in part
+    (300, 70000, 70, WHOLE, 9, True),     # more steps of 32 features than there are stages
+    (1000, 15000, 1025, WHOLE, 64, True),  # shares of more classes than exponents are loaded at a time, of groups of different scales
+    (600, 33000, 260, SHARED, 9, True),
+    (512, 10575, 128, HALF, 9, True),
+    (100, 333, 129, HALF, 1, False),
+    (96, 600, 64, FEW, 1, False)])
+def test_fc_logreg_every_form_on_dense_operands(d, v, n, logits, steps, shared):
+    for backward in (0, 1):
+        forms = fcl_forms(d, v, n, backward)
+        assert len(forms) == 1 and forms[0][1] == logits and forms[0][2] >= steps and (not backward or forms[0][4] == shared), forms
+    w, x, b, lab = fcl_data(d, v, n, 43, masked=0.05, padded=n // 10)
+    rng = np.random.default_rng(44)
+    w *= np.repeat(np.float32(10.0) ** rng.choice([-7, -3, 0], (v + 31) // 32), 32)[:v, None]  # (32 classes have one scale)
+    ref = fcl_ref(w, x, b, lab, 0.37)
+    st, lp, ok, dx, dw, db, cost = fcl_run(w, x, b, lab, 0.37)
+    check_forward(ref, st, lp, ok)
+    for got, k in ((dx, 'dx'), (dw, 'dw'), (db, 'db')):
+        within(got, ref[k], ref['e' + k], k)
 
 
 @pytest.mark.gpu
