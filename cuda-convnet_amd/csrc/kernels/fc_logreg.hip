@@ -23,6 +23,9 @@ struct NarrowArgs {
     float* labelLogits;  // forward: [N]
     const float* stats;  // backward
     char* dz;            // backward: dz / coeff, split into fragments of (rows = cases, k = classes) as the wide path's
+    size_t near;         // and once more, this far behind it, without the levels
+    unsigned char* levels;
+    int* anyLevel;
     float* dbPart;       // backward: [V], row sums of dz / coeff
     int Kv;
 };
@@ -53,6 +56,24 @@ constexpr int FRAG = 1024, PAIR = 2 * FRAG;  // bytes of a fragment, of its two 
 constexpr int TILE = 128;                    // columns of a product's tile
 constexpr float LO = 2048.f;                 // scale of the low piece
 constexpr int DZ_EXP = 14;                   // |dz / coeff| <= 1
+// dz / coeff of a class that is far from 64 cases, all of it below 2^-28, is stored times a further 2^28, below 2^-56 2^56 and below 2^-84
+// 2^74 (a level, one byte for every class and 64 cases): so what a class's weight gradient sums has its 22 bits down to 2^-102, and fewer down
+// to 2^-124.  (At one scale for all, 2^14, an entry of 2^-36 is off by 6e-5 of itself, one of 2^-48 by 0.2, and below 2^-50 nothing is left.)
+constexpr float FAR = 1.f / (1 << 28);
+__device__ __forceinline__ int level_of(float most) { return most == 0.f || !(most < FAR) ? 0 : most >= FAR * FAR ? 1 : most >= FAR * FAR * FAR ? 2 : 3; }
+__device__ __forceinline__ int level_exp(int level) { return min(28 * level, 74); }
+__device__ __forceinline__ float level_scale(int level) { return ldexpf(1.f, DZ_EXP + level_exp(level)); }
+// the largest of the 16 lanes of a row; a NaN is larger than anything
+__device__ __forceinline__ float row_max(float v) {
+    unsigned m = __float_as_uint(v);
+#define ROTATED(n) (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x120 + n, 0xf, 0xf, false)
+    m = max(m, ROTATED(8));
+    m = max(m, ROTATED(4));
+    m = max(m, ROTATED(2));
+    m = max(m, ROTATED(1));
+#undef ROTATED
+    return __uint_as_float(m);
+}
 constexpr int EXP_ZERO = 1 << 20;            // a group of zeros: any scale will do
 // The exponents of the cases and of the groups of 32 classes are kept with a flag: whether the group holds an infinity or NaN.
 __device__ __forceinline__ int exp_odd(int e, bool odd) { return e * 2 + (odd ? 1 : 0); }
@@ -85,7 +106,7 @@ __device__ __forceinline__ float exp_neg(float x) {
 template <bool BWD, int NB, int RG>
 __global__ __launch_bounds__(256) void k_fcl_narrow(NarrowArgs p) {
     __shared__ f32x4 red[4][RG][NB][64];
-    __shared__ float rowSum[4][16 * RG];
+    __shared__ float rowSum[4][16 * RG], rowMax[4][16 * RG];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int vBase = blockIdx.x * 16 * RG;
     const float* rowPtr[RG];
@@ -151,26 +172,55 @@ __global__ __launch_bounds__(256) void k_fcl_narrow(NarrowArgs p) {
         const float inv = counts ? 1.f / S : 0.f;
         char* out = p.dz + ((size_t)wave * p.Kv + vBase / 32) * PAIR + lane * 8;
         char* rest = out + (size_t)4 * p.Kv * PAIR;  // cases 64 .. 127 of the tile: there are none
+        auto place = [&](int q) { return ((vBase / 16 + q) & 1) * 512 + (((vBase & 16) + q * 16) >> 5) * PAIR; };
+        auto store = [&](char* to, const float (&t)[4], const float (&scale)[4]) {
+            f16x4 hi, lo;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float y = t[r] * scale[r];
+                hi[r] = (_Float16)y;
+                lo[r] = (_Float16)((y - (float)hi[r]) * LO);
+            }
+            *reinterpret_cast<f16x4*>(to) = hi;
+            *reinterpret_cast<f16x4*>(to + FRAG) = lo;
+        };
 #pragma unroll
         for (int q = 0; q < RG; q++) {
-            f16x4 hi = {}, lo = {};
+            const float one = (float)(1 << DZ_EXP);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 float t = 0.f;
                 if (wave < NB && counts) t = (label == p.v0 + vBase + q * 16 + g * 4 + r ? 1.f : 0.f) - exp_neg(z[q][r] - M) * inv;
-                const float y = t * (float)(1 << DZ_EXP);
-                hi[r] = (_Float16)y;
-                lo[r] = (_Float16)((y - (float)hi[r]) * LO);
+                z[q][r] = t;
+                const float most = row_max(fabsf(t));
                 for (int o = 1; o < 16; o <<= 1) t += __shfl_xor(t, o, 64);
-                if (c == 0) rowSum[wave][q * 16 + g * 4 + r] = t;
+                if (c == 0) {
+                    rowSum[wave][q * 16 + g * 4 + r] = t;
+                    rowMax[wave][q * 16 + g * 4 + r] = most;
+                }
             }
-            const int at = ((vBase / 16 + q) & 1) * 512 + (((vBase & 16) + q * 16) >> 5) * PAIR;
-            *reinterpret_cast<f16x4*>(out + at) = hi;
-            *reinterpret_cast<f16x4*>(out + at + FRAG) = lo;
-            *reinterpret_cast<f16x4*>(rest + at) = (f16x4){};
-            *reinterpret_cast<f16x4*>(rest + at + FRAG) = (f16x4){};
+            store(out + p.near + place(q), z[q], {one, one, one, one});
         }
         __syncthreads();
+#pragma unroll
+        for (int q = 0; q < RG; q++) {
+            float scale[4];
+            unsigned levels = 0;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int v = q * 16 + g * 4 + r;
+                const int level = level_of(fmaxf(fmaxf(rowMax[0][v], rowMax[1][v]), fmaxf(rowMax[2][v], rowMax[3][v])));
+                scale[r] = level_scale(level);
+                levels |= level << 8 * r;
+            }
+            store(out + place(q), z[q], scale);
+            *reinterpret_cast<f16x4*>(rest + place(q)) = (f16x4){};
+            *reinterpret_cast<f16x4*>(rest + place(q) + FRAG) = (f16x4){};
+            if (c == 0 && wave == 0 && levels) {  // (of cases 64 .. 127 there are none)
+                *reinterpret_cast<unsigned*>(p.levels + vBase + q * 16 + g * 4) = levels;
+                *p.anyLevel = 1;
+            }
+        }
         if (p.dbPart && tid < 16 * RG && vBase + tid < p.rows)
             p.dbPart[p.v0 + vBase + tid] = (rowSum[0][tid] + rowSum[1][tid]) + (rowSum[2][tid] + rowSum[3][tid]);
         return;
@@ -303,9 +353,10 @@ __global__ __launch_bounds__(256) void k_fcl_cost(const float* __restrict__ labe
 // fp32, and hi hi, hi lo and lo hi are summed (3 instructions), the cross terms in an accumulator of their own, so that lo keeps its
 // bits.  With the largest magnitude of a scaled group below 2^15 the relative error of a product is about 2^-22 for entries down to
 // 2^-21 of the group's largest, and an entry further down is off by at most 2^-43 of it.  The groups: a case's features for the
-// logits, a feature's cases for the weight gradient, 32 classes' weights, and +-1 for dz / coeff.  Along the summed dimension a group
-// is either whole or, for the classes of the input gradient, its scale is carried along (CarryScale), so a row of large weights
-// takes no bits from the other groups.
+// logits, a feature's cases for the weight gradient, 32 classes' weights, and for dz / coeff a class over 64 cases in the weight gradient
+// (levels, above) and all of it in the input gradient, where the label's entry, 1 - p, is off by 2^-25 anyway.  Along the summed dimension
+// a group is either whole or its scale is carried along (CarryScale, CarryLevels), so a row of large weights takes no bits from the
+// other groups, nor one case that is sure of a class from the class's other cases.
 //
 // Operands are split ONCE by a pack launch into fragments of 16 rows x 32 k entries and two pieces, 1 KB each:
 //   entry (row c, k = 16 h + 4 g + j) of a piece lies at byte 512 h + 128 g + 8 c + 2 j, zero-padded to whole tiles.
@@ -383,10 +434,13 @@ __device__ __forceinline__ f16x8 read_frag_turned(const char* p, const char* q) 
 struct NoScale {
     template <int MB>
     __device__ __forceinline__ void operator()(int, Acc<MB>&) const {}
+    __device__ __forceinline__ bool moves(int) const { return false; }
+    __device__ __forceinline__ size_t move(int) const { return 0; }
 };
 
 // A: pair (row block 0 of the tile, k block 0); aRow: bytes between its row blocks.  B: the same, or, TURNED, pair (row block 0, k block 0
-// of the tile's columns) of fragments whose rows are this product's k.  scale(step, acc) runs in front of a step's products.
+// of the tile's columns) of fragments whose rows are this product's k.  scale(step, acc) runs in front of a step's products,
+// where scale.moves(step), scale.move(step) is added to where this wave copies from, from that step on.
 //
 // Step t multiplies what step t - 1 read, reads stage t + 1 and asks for stage t + STAGES, whose buffer everyone has read by then.  One
 // wave a SIMD: whatever is not a matrix instruction has to be issued while one runs (16 cycles), so the reads and copies stand between
@@ -438,13 +492,22 @@ __device__ __forceinline__ void product_tile(const char* A, size_t aRow, const c
             f.a[i][q] = read_frag(s + offA + i * PAIR + q * FRAG);
         }
     };
-    int left = n - 1;           // stages behind the one that src points at
+    int at = 0;                   // the stage that src points at
+    auto move_source = [&] {
+        if (__builtin_expect(scale.moves(at), 0)) {
+            const size_t by = scale.move(at);
+#pragma unroll
+            for (int i = 0; i < MINE; i++) src[i] += by;
+        }
+    };
+    move_source();
     unsigned fill = 0, take = 0;  // byte offsets of the buffers that are copied to, and read
     auto next_stage = [&] {
-        const bool more = left > 0;
-        left -= more ? 1 : 0;
+        const bool more = at < n - 1;
+        at += more ? 1 : 0;
 #pragma unroll
         for (int i = 0; i < MINE; i++) src[i] += more ? adv[i] : 0;
+        if (more) move_source();
         fill = fill == (STAGES - 1) * STAGE ? 0 : fill + STAGE;
     };
     auto step = [&](int t, Frags<MB>& now, Frags<MB>& next) {
@@ -523,17 +586,25 @@ __device__ __forceinline__ void product_tile_shared(const char* A, size_t aRow, 
     const int offA = wm * 4 * PAIR + lane * 8;
     const int offB = (8 + (TURNED ? wn * 2 : wn * 4)) * PAIR + (TURNED ? (lane & 3) * 128 + ((lane >> 4) * 4 + ((lane & 15) >> 2)) * 8 : lane * 8);
     unsigned fill = 0, take = 0;
-    auto copy = [&] {
+    auto move_source = [&](int t) {
+        if (__builtin_expect(scale.moves(t), 0)) {
+            const size_t by = scale.move(t);
+#pragma unroll
+            for (int i = 0; i < MINE; i++) src[i] += by;
+        }
+    };
+    auto copy = [&](int t) {
+        move_source(t);
 #pragma unroll
         for (int o = 0; o < 2 * MINE; o++) copy_pair_half(src[o >> 1], ldsBase + fill + (o >> 1) * PAIR, laneOff, o & 1);
 #pragma unroll
         for (int i = 0; i < MINE; i++) src[i] += adv;
         fill ^= STAGE;
     };
-    copy();
+    copy(0);
     for (int t = 0; t < n; t++) {
         wait_copies_and_meet<0>();  // stage t has landed, and everyone has read the other buffer
-        if (t + 1 < n) copy();
+        if (t + 1 < n) copy(t + 1);
         Frags<4> f;
         const char* s = lds + take;
         take ^= STAGE;
@@ -584,7 +655,9 @@ struct PackArgs {
     const float *W, *bias;  // of the piece
     int* classExp;
     char* wByClass;
-    int rows;
+    unsigned char* levels;  // backward: cleared by the classes' blocks
+    int* anyLevel;
+    int rows, Kv;
 };
 
 // Bound by memory: W is read once and written once, as two pieces of 16 bits (10575 x 512: 13 us, 3.3 TB/s; 100000 x 512, one call: 83 us,
@@ -776,19 +849,31 @@ __global__ __launch_bounds__(512) void k_fcl_pack(PackArgs p) {
     const int b = blockIdx.x;
     if (b < p.caseBlocks) pack_cases(p, b, tile, exps);
     else if (b < p.caseBlocks + p.featBlocks) pack_feats(p, b - p.caseBlocks, exps);
-    else pack_classes(p, b - p.caseBlocks - p.featBlocks, tile);
+    else {
+        const int block = b - p.caseBlocks - p.featBlocks;
+        if (p.levels) {
+            for (int i = threadIdx.x; i < p.Kn / 2 * 8; i += 512) reinterpret_cast<unsigned*>(p.levels + ((size_t)(i >> 3) * p.Kv + block) * 32)[i & 7] = 0;
+            if (block == 0 && threadIdx.x == 0) *p.anyLevel = 0;
+        }
+        pack_classes(p, block, tile);
+    }
 }
 
 // ---- logits of a piece
 struct WideArgs {
     const char *wByClass, *xByCase;
     const int *classExp, *caseExp;
-    const float *W, *X, *bias, *labels, *stats;
-    int D, V, N, v0, rows, Kd, kSteps, vTiles, nTiles;
+    const float *bias, *labels, *stats;
+    int V, N, v0, rows, Kd, kSteps, vTiles, nTiles;
     float *part, *labelLogits;  // forward: part + the piece's first tile
     char* dz;                   // backward: dz / coeff, (rows = cases, k = classes)
     float* dbPart;              // backward: [nTiles][V], row sums of dz / coeff
     int Kv;
+    size_t near;                // backward: dz of 32 classes x 64 cases with a level is there once more, this far behind, without
+    unsigned char* levels;      // backward: [Np / 64][32 Kv], zeros
+    int* anyLevel;              // backward: whether there are any, zero
+    const float *W, *X;
+    int D;
 };
 
 // Logits whose weights or inputs hold an infinity or NaN: the products of pieces make a NaN of any of them, where the formula has the sum
@@ -938,6 +1023,9 @@ __global__ __launch_bounds__(256, SHARED ? 2 : 1) void k_fcl_logits(WideArgs p) 
         return;
     } else {
         float sums[MB][4] = {};
+        auto largest = [&](int i, int r) {
+            return fmaxf(fmaxf(fmaxf(fabsf(acc.c[0][i][0][r]), fabsf(acc.c[0][i][1][r])), fabsf(acc.c[0][i][2][r])), fabsf(acc.c[0][i][3][r]));
+        };
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int n = nBase + j * 16 + c;
@@ -961,20 +1049,67 @@ __global__ __launch_bounds__(256, SHARED ? 2 : 1) void k_fcl_logits(WideArgs p) 
 #pragma unroll
                     for (int r = 0; r < 4; r++) acc.c[0][i][j][r] += counts && at[j] == i * 16 + r ? 1.f : 0.f;
             }
-            char* out = p.dz + ((size_t)(nBase / 16 + j) * p.Kv + vBase / 32) * PAIR + lane * 8;
 #pragma unroll
-            for (int i = 0; i < MB; i++) {
-                f16x4 hi, lo;
+            for (int i = 0; i < MB; i++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float t = acc.c[0][i][j][r];
-                    sums[i][r] += t;
-                    const float y = t * (float)(1 << DZ_EXP);
-                    hi[r] = (_Float16)y;
-                    lo[r] = (_Float16)((y - (float)hi[r]) * LO);
+                for (int r = 0; r < 4; r++) sums[i][r] += acc.c[0][i][j][r];
+        }
+        auto store = [&](char* to, int i, int j, auto scale) {  // rows 16 i .. + 15, cases 16 j .. + 15
+            f16x4 hi, lo;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float y = acc.c[0][i][j][r] * scale(r);
+                hi[r] = (_Float16)y;
+                lo[r] = (_Float16)((y - (float)hi[r]) * LO);
+            }
+            *reinterpret_cast<f16x4*>(to + (i >> 1) * PAIR + (i & 1) * 512) = hi;
+            *reinterpret_cast<f16x4*>(to + (i >> 1) * PAIR + FRAG + (i & 1) * 512) = lo;
+        };
+        auto plain = [](int) { return (float)(1 << DZ_EXP); };
+        // The classes that are far from this wave's cases are looked for where the sum of what a lane holds of one is small.  Its entries are
+        // -p, or 1 - p, which is no number between 0 and 2^-24: the sum is below 0 then, and a zero is no sign of it.
+        unsigned least = ~0u;
+#pragma unroll
+        for (int i = 0; i < MB; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) least = min(least, __float_as_uint(sums[i][r]) - 0x80000001u);
+        if (__builtin_expect(__any(least < __float_as_uint(4 * FAR) - 1), 0)) {
+            LateArgs late = (LateArgs)__builtin_amdgcn_kernarg_segment_ptr();
+            asm volatile("" : "+s"(late));
+            unsigned char* levels = late->levels + (size_t)(nBase / 64) * late->Kv * 32 + vBase + g * 4;
+#pragma unroll
+            for (int q = 0; q < MB / 2; q++) {
+                unsigned packed[2] = {};
+                float scale[2][4];
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const int level = level_of(row_max(largest(2 * q + h, r)));
+                        packed[h] |= level << 8 * r;
+                        scale[h][r] = level_scale(level);
+                    }
+                const bool any = __any(packed[0] | packed[1]);
+                if (any) {
+                    if (c < 2) *reinterpret_cast<unsigned*>(levels + (2 * q + c) * 16) = c == 0 ? packed[0] : packed[1];
+                    if (lane == 0) *late->anyLevel = 1;
                 }
-                *reinterpret_cast<f16x4*>(out + (i >> 1) * PAIR + (i & 1) * 512) = hi;
-                *reinterpret_cast<f16x4*>(out + (i >> 1) * PAIR + FRAG + (i & 1) * 512) = lo;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    char* out = late->dz + ((size_t)(nBase / 16 + j) * late->Kv + vBase / 32) * PAIR + lane * 8;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        store(out, 2 * q + h, j, [&](int r) { return scale[h][r]; });
+                        if (any) store(out + late->near, 2 * q + h, j, plain);
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                char* out = p.dz + ((size_t)(nBase / 16 + j) * p.Kv + vBase / 32) * PAIR + lane * 8;
+#pragma unroll
+                for (int i = 0; i < MB; i++) store(out, i, j, plain);
             }
         }
         if (p.dbPart) {  // row sums: over the lanes of a row, then the two waves of 64 cases
@@ -1002,6 +1137,10 @@ struct GradArgs {
     int D, rows, Kn, Kv, Kd, Np, Dp, nTiles, dTiles, kPerSplit, first;
     int inputBlocks;  // blocks of the input gradient, then those of the weight gradient
     float scaleTargets, scaleOutput;
+    const unsigned char* levels;
+    const int* anyLevel;
+    size_t near;
+    int allNear;  // few cases: all of dz is there twice
 };
 
 template <bool SHARED, class Scale>
@@ -1010,6 +1149,62 @@ __device__ __forceinline__ void turned_tile(const char* A, size_t aRow, const ch
     if constexpr (SHARED) product_tile_shared<true>(A, aRow, B, bRow, k0, k1, lds, acc, scale);
     else product_tile<4, true>(A, aRow, B, bRow, k0, k1, lds, acc, scale);
 }
+
+// The weight gradient's accumulators are in units of 2^-(14 + level_exp) of the class they add for: where its level changes from 64 cases to
+// the next they are brought to it, exactly.  |sum| < 2^49 at any level, so 2^74 takes none out of range.
+struct CarryLevels {
+    const unsigned char* levels;  // of this wave's 64 classes
+    size_t row;
+    int halves;
+    mutable int next;              // the step that has something to do: a change, or 64 x 64 cases further on
+    mutable unsigned long long far;  // a bit for each 64 cases: whether any class has a level
+    mutable unsigned cur;          // a byte for each of a lane's four classes
+    __device__ __forceinline__ CarryLevels(const unsigned char* l, size_t r, int n, bool any) : levels(l), row(r), halves(n), next(any ? 0 : -1), far(0), cur(0) {}
+    __device__ __forceinline__ bool moves(int) const { return false; }
+    __device__ __forceinline__ size_t move(int) const { return 0; }
+    template <int MB>
+    __device__ __forceinline__ void operator()(int t, Acc<MB>& acc) const {
+        if (__builtin_expect(t != next, 1)) return;
+        const int h = t >> 1, b = h & 63;
+        if (b == 0) {
+            const int i = h + (int)(threadIdx.x & 63);
+            unsigned any = 0;
+            if (i < halves) {
+                const uint4* p = reinterpret_cast<const uint4*>(levels + i * row);
+                const uint4 q = p[0], r = p[1], s = p[2], u = p[3];
+                any = q.x | q.y | q.z | q.w | r.x | r.y | r.z | r.w | s.x | s.y | s.z | s.w | u.x | u.y | u.z | u.w;
+            }
+            far = __ballot(any != 0);
+        }
+        unsigned now = 0;
+        if (far >> b & 1) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) now |= (unsigned)levels[h * row + j * 16 + (threadIdx.x & 15)] << 8 * j;
+        }
+        bring(now, acc);
+        const unsigned long long later = b == 63 ? 0 : ((far | far << 1) >> (b + 1)) << (b + 1);  // cases with levels, and the ones behind them
+        next = 2 * (later ? h - b + __builtin_ctzll(later) : h - b + 64);
+    }
+    template <int MB>
+    __device__ __forceinline__ void bring(unsigned now, Acc<MB>& acc) const {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int up = level_exp(now >> 8 * j & 255) - level_exp(cur >> 8 * j & 255);
+            if (!__any(up != 0)) continue;
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int i = 0; i < MB; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) acc.c[k][i][j][r] = ldexpf(acc.c[k][i][j][r], up);
+        }
+        cur = now;
+    }
+    template <int MB>
+    __device__ __forceinline__ void end(Acc<MB>& acc) const {  // no level
+        if (__builtin_expect(__any(cur != 0), 0)) bring(0, acc);
+    }
+};
 
 // weight gradient: (features x classes) tiles, so that a lane's four rows are four neighbours of one row of W
 template <bool SHARED>
@@ -1020,7 +1215,9 @@ __device__ __forceinline__ void weight_tile(const GradArgs& p, int L, char* lds)
     const int c = lane & 15, g = lane >> 4;
     const size_t row = (size_t)p.Kn * PAIR;
     Acc<4> acc;
-    turned_tile<SHARED>(p.xByFeat + (size_t)td * 8 * row, row, p.dz + (size_t)tv * 4 * PAIR, (size_t)p.Kv * PAIR, 0, p.Kn, lds, acc, NoScale());
+    const CarryLevels carry(p.levels + tv * TILE + wn * 64, (size_t)p.Kv * 32, p.Kn / 2, __builtin_amdgcn_readfirstlane(*p.anyLevel) != 0);
+    turned_tile<SHARED>(p.xByFeat + (size_t)td * 8 * row, row, p.dz + (size_t)tv * 4 * PAIR, (size_t)p.Kv * PAIR, 0, p.Kn, lds, acc, carry);
+    carry.end(acc);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int d = td * TILE + wm * 64 + i * 16 + g * 4;
@@ -1054,11 +1251,37 @@ __device__ __forceinline__ void weight_tile(const GradArgs& p, int L, char* lds)
 
 // The accumulators are in units of 2^-(exponent of the group they last added): when the next 32 classes have another scale, they are
 // brought to it, exactly, by a power of two.  A group of zeros has none.  Exponents come 64 at a time into a register of the lanes.
+// Here every class's dz is wanted at the one scale: the waves that copy it take 32 classes with levels from behind.
 struct CarryScale {
     const int* exps;  // of the product's k blocks, from k0 on
     int count;
+    const unsigned char* levels;  // of the 64 cases that this wave copies, or NULL
+    size_t near;
     mutable int held, cur;
-    __device__ __forceinline__ CarryScale(const int* e, int n) : exps(e), count(n), held(load(0)), cur(EXP_ZERO) {}
+    mutable int next;                // the step from which it copies from the other place, or 64 further on
+    mutable unsigned long long far;  // a bit for each k block
+    mutable bool there;
+    __device__ __forceinline__ CarryScale(const int* e, int n, const unsigned char* l, size_t d)
+        : exps(e), count(n), levels(l), near(d), held(load(0)), cur(EXP_ZERO), next(l ? 0 : -1), far(0), there(false) {}
+    __device__ __forceinline__ bool moves(int t) const { return t == next; }
+    __device__ __forceinline__ size_t move(int t) const {
+        const int b = t & 63;
+        if (b == 0) {
+            const int i = t + (int)(threadIdx.x & 63);
+            unsigned any = 0;
+            if (i < count) {
+                const uint4* p = reinterpret_cast<const uint4*>(levels + (size_t)i * 32);
+                const uint4 q = p[0], r = p[1];
+                any = q.x | q.y | q.z | q.w | r.x | r.y | r.z | r.w;
+            }
+            far = __ballot(any != 0);
+        }
+        const bool now = far >> b & 1, was = there;
+        there = now;
+        const unsigned long long later = (now ? ~far : far) >> b;  // (its lowest bit is not set)
+        next = later ? t + __builtin_ctzll(later) : t - b + 64;
+        return (now ? near : 0) - (was ? near : 0);
+    }
     __device__ __forceinline__ int load(int t) const {
         const int i = t + (int)(threadIdx.x & 63);
         return i < count ? exp_of(exps[i]) : EXP_ZERO;
@@ -1094,8 +1317,9 @@ __device__ __forceinline__ void input_tile(const GradArgs& p, int L, char* lds) 
     const size_t row = (size_t)p.Kv * PAIR;
     const int k0 = s * p.kPerSplit, k1 = min(p.Kv, k0 + p.kPerSplit);
     Acc<4> acc;
-    const CarryScale carry(p.classExp + k0, k1 - k0);
-    turned_tile<SHARED>(p.dz + (size_t)tn * 8 * row, row, p.wByClass + (size_t)td * 4 * PAIR, (size_t)p.Kd * PAIR, k0, k1, lds, acc, carry);
+    const unsigned char* levels = wave < 2 && !p.allNear && __builtin_amdgcn_readfirstlane(*p.anyLevel) ? p.levels + ((size_t)(tn * 2 + wave) * p.Kv + k0) * 32 : nullptr;
+    const CarryScale carry(p.classExp + k0, k1 - k0, levels, p.near);
+    turned_tile<SHARED>(p.dz + (p.allNear ? p.near : 0) + (size_t)tn * 8 * row, row, p.wByClass + (size_t)td * 4 * PAIR, (size_t)p.Kd * PAIR, k0, k1, lds, acc, carry);
     const int e = carry.cur == EXP_ZERO ? 0 : -(carry.cur + DZ_EXP);
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -1171,7 +1395,7 @@ struct WidePlan {
     int Kv;                                      // k blocks of the first piece, padded
     int kPerSplit, splits;                       // input gradient: every split of a whole piece holds something, so that the first piece
                                                  // writes every slab
-    size_t classExp, caseExp, featExp, xByCase, xByFeat, wByClass, dz, dbPart, slabs, part, labelLogits, total;
+    size_t classExp, caseExp, featExp, xByCase, xByFeat, wByClass, dz, dzNear, levels, anyLevel, dbPart, slabs, part, labelLogits, total;
 };
 // When the packed operands pay for the logits (us of a whole cost call, narrow / wide).  512 x 10575: 16 cases 16 / 34, 64 cases 26 / 35;
 // 512 x 100000: 56 / 145, 121 / 147.  Both calls go by the number of cases alone: the gradients' logits are the cost's, to the bit.
@@ -1212,6 +1436,9 @@ WidePlan wide_plan(int D, int V, int N, bool bwd) {
         p.featExp = take((size_t)p.Dp * 4);
         p.xByFeat = take((size_t)p.Dp / 16 * p.Kn * PAIR);
         p.dz = take((size_t)p.Np / 16 * mostKv * PAIR);
+        p.dzNear = take((size_t)p.Np / 16 * mostKv * PAIR);
+        p.levels = take((size_t)p.Np / 64 * mostKv * 32);
+        p.anyLevel = take(4);
         p.dbPart = take((size_t)p.nTiles * V * 4);
         p.slabs = take((size_t)p.splits * p.Dp * p.Np * 4);
     } else {
@@ -1273,7 +1500,7 @@ TileKind wide_piece(const WidePlan& q, WideArgs& a, PackArgs& k, const float* W,
     a.v0 = v0;
     a.rows = k.rows = piece_rows(q, a.V, v0);
     a.nTiles = q.nTiles;
-    a.Kv = divup(a.rows, TILE) * 4;
+    a.Kv = k.Kv = divup(a.rows, TILE) * 4;
     const TileKind kind = tile_choice(a.Kv, q.nTiles);
     a.vTiles = a.Kv / tile_rows32(kind);
     k.W = W + (size_t)v0 * D;
@@ -1325,15 +1552,21 @@ int wide_grad(const float* W, const float* X, const float* bias, const float* la
     WideArgs a = wide_args(q, W, X, bias, labels, D, V, N, ws);
     a.stats = stats;
     a.dz = ws + q.dz;
+    a.near = q.dzNear - q.dz;
+    a.levels = (unsigned char*)ws + q.levels;
+    a.anyLevel = (int*)(ws + q.anyLevel);
     a.dbPart = dB ? (float*)(ws + q.dbPart) : nullptr;
     float* slabs = (float*)(ws + q.slabs);
     const bool narrow = !wide_cost_usable(N);  // (the forward call's logits, to the bit)
     PackArgs pack = pack_args(q, X, labels, stats, D, V, N, dW != nullptr, ws);
     if (narrow) pack.caseBlocks = 0;
+    pack.levels = a.levels;
+    pack.anyLevel = a.anyLevel;
     NarrowArgs few = {W, X, bias, labels, D, V, N};
-    few.stats = stats; few.dz = a.dz; few.dbPart = a.dbPart;
+    few.stats = stats; few.dz = a.dz; few.near = a.near; few.levels = a.levels; few.anyLevel = a.anyLevel; few.dbPart = a.dbPart;
     GradArgs t = {};
     t.xByFeat = ws + q.xByFeat; t.dz = ws + q.dz; t.wByClass = ws + q.wByClass;
+    t.levels = a.levels; t.anyLevel = a.anyLevel; t.near = a.near; t.allNear = narrow;
     t.featExp = (const int*)(ws + q.featExp); t.classExp = (const int*)(ws + q.classExp);
     t.slabs = slabs;
     t.D = D; t.Kn = q.Kn; t.Kd = q.Kd; t.Np = q.Np; t.Dp = q.Dp; t.nTiles = q.nTiles; t.dTiles = q.dTiles;

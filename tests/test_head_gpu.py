@@ -716,6 +716,30 @@ def test_fc_logreg_weights_of_very_different_sizes(n, large, tiny):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('d,v,n', [(36, 500, 6), (36, 500, 64), (40, 33000, 20), (40, 700, 140), (160, 10575, 509), (96, 10575, 509), (300, 70000, 70), (64, 3000, 1025), (20, 300, 4500)])
+def test_fc_logreg_classes_that_no_case_comes_near(d, v, n):
+    """Probabilities from 1 down to 2^-90: every class's weight gradient is right relative to itself, beside labels' classes and others, and
+    where a class is near some cases and far from others (feature 0 changes its sign every 64 to 192 cases)."""
+    rng = np.random.default_rng(45)
+    w = (rng.standard_normal((v, d)) / np.sqrt(d)).astype(np.float32)
+    x = rng.standard_normal((d, n)).astype(np.float32)
+    x[0] = np.where(np.arange(n) // 64 % 5 < 2, 1, -1)
+    w[:, 0] = rng.choice([-10, 0, 10], v)
+    b = (-np.log(2) * 52 * rng.random(v)).astype(np.float32)
+    near = rng.permutation(v)[:max(v // 8, 4)]
+    b[near], w[near, 0] = 0, 0
+    lab = rng.choice(near, n).astype(np.float32)
+    lab[n - n // 7:] = -1
+    ref = fcl_ref(w, x, b, lab, 0.5)
+    largest = np.abs(ref['dz']).max(1)
+    assert (largest < 2.0 ** -45).sum() > v // 20 and largest[largest > 0].min() > 2.0 ** -92
+    st, lp, ok, dx, dw, db, cost = fcl_run(w, x, b, lab, 0.5)
+    check_forward(ref, st, lp, ok)
+    for got, k in ((dx, 'dx'), (dw, 'dw'), (db, 'db')):
+        within(got, ref[k], ref['e' + k], k)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('d,v,n', [(12, 30, 9), (40, 150, 66)])
 def test_fc_logreg_gradient_against_differences(d, v, n):
     """d sum(log p) along random directions (central differences of the float64 formula, step 1e-4: 1e-6 of the magnitudes)."""
