@@ -735,10 +735,6 @@ __device__ __forceinline__ void pack_feats(const PackArgs& p, int block, int* ex
 // (all of a thread's loads in flight at once) and LDS; rows of at most 512 features are read once, longer ones a second time for their
 // max.
 constexpr int CW = 512, CW_LD = CW + 4;
-// A sum that has groups of large weights in it is multiplied up where a group of tiny ones follows: |sum| <= 2 max|w| (of dz / coeff, the
-// magnitudes of a case add up to 2 at most), so with this bound on the exponents no weights below 2^48 take it out of range.  It
-// leaves a group whose largest weight is below 2^-50 with less than 22 bits below 2^-78.
-constexpr int CLASS_EXP_MAX = 64;
 constexpr int PACK_LDS = (32 * CW_LD + 16) * 4;
 __device__ __forceinline__ void pack_classes(const PackArgs& p, int block, float* tile) {
     float* maxima = tile + 32 * CW_LD;
@@ -824,7 +820,7 @@ __device__ __forceinline__ void pack_classes(const PackArgs& p, int block, float
                 __syncthreads();
                 for (int w = 0; w < 8; w++) m = fmaxf(m, maxima[w]);
             }
-            e = min(scale_exp(m) & ~7, CLASS_EXP_MAX);
+            e = scale_exp(m) & ~7;
             if (threadIdx.x == 0) p.classExp[block] = exp_odd(m == 0.f ? EXP_ZERO : e, odd);
         }
         __syncthreads();
@@ -1250,19 +1246,40 @@ __device__ __forceinline__ void weight_tile(const GradArgs& p, int L, char* lds)
 }
 
 // The accumulators are in units of 2^-(exponent of the group they last added): when the next 32 classes have another scale, they are
-// brought to it, exactly, by a power of two.  A group of zeros has none.  Exponents come 64 at a time into a register of the lanes.
+// brought to it, exactly, by a power of two.  A group of zeros has none.  |sum| < 2^30 in the units of its largest weights (the dz / coeff
+// of a case add up to 2 at most); where a group's are more than 2^80 times smaller, or larger, the sum goes to the slab and begins anew, so
+// that it stays in range whatever the weights.  Exponents come 64 at a time into a register of the lanes.
 // Here every class's dz is wanted at the one scale: the waves that copy it take 32 classes with levels from behind.
 struct CarryScale {
+    f32x4* out;       // of the slab: this lane's four cases of row block 0 and column block 0
+    size_t column;    // entries from one feature to the next
+    mutable bool fresh;  // there is nothing in the slab yet
     const int* exps;  // of the product's k blocks, from k0 on
     int count;
     const unsigned char* levels;  // of the 64 cases that this wave copies, or NULL
     size_t near;
-    mutable int held, cur;
+    mutable int held, cur, low;      // low: the smallest since the sum began
     mutable int next;                // the step from which it copies from the other place, or 64 further on
     mutable unsigned long long far;  // a bit for each k block
     mutable bool there;
-    __device__ __forceinline__ CarryScale(const int* e, int n, const unsigned char* l, size_t d)
-        : exps(e), count(n), levels(l), near(d), held(load(0)), cur(EXP_ZERO), next(l ? 0 : -1), far(0), there(false) {}
+    __device__ __forceinline__ CarryScale(float* o, size_t c, bool f, const int* e, int n, const unsigned char* l, size_t d)
+        : out(reinterpret_cast<f32x4*>(o)), column(c / 4), fresh(f), exps(e), count(n), levels(l), near(d), held(load(0)), cur(EXP_ZERO), low(0),
+          next(l ? 0 : -1), far(0), there(false) {}
+    template <int MB>
+    __device__ __forceinline__ void put(const Acc<MB>& acc) const {
+        const int e = cur == EXP_ZERO ? 0 : -(cur + DZ_EXP);
+#pragma unroll
+        for (int i = 0; i < MB; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                f32x4* to = out + j * 16 * column + i * 4;
+                f32x4 y;
+#pragma unroll
+                for (int r = 0; r < 4; r++) y[r] = ldexpf(acc.value(i, j, r), e);
+                *to = fresh ? y : *to + y;
+            }
+        fresh = false;
+    }
     __device__ __forceinline__ bool moves(int t) const { return t == next; }
     __device__ __forceinline__ size_t move(int t) const {
         const int b = t & 63;
@@ -1291,7 +1308,11 @@ struct CarryScale {
         if (t > 0 && (t & 63) == 0) held = load(t);
         const int e = __builtin_amdgcn_readlane(held, t & 63);
         if (e == EXP_ZERO || e == cur) return;
-        if (cur != EXP_ZERO) {
+        if (cur == EXP_ZERO) {
+            low = e;
+        } else {
+            const bool anew = e - low > 80 || e - cur < -80;
+            if (__builtin_expect(anew, 0)) put(acc);
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
@@ -1299,7 +1320,8 @@ struct CarryScale {
 #pragma unroll
                     for (int j = 0; j < 4; j++)
 #pragma unroll
-                        for (int r = 0; r < 4; r++) acc.c[h][i][j][r] = ldexpf(acc.c[h][i][j][r], e - cur);
+                        for (int r = 0; r < 4; r++) acc.c[h][i][j][r] = anew ? 0.f : ldexpf(acc.c[h][i][j][r], e - cur);
+            low = anew ? e : min(low, e);
         }
         cur = e;
     }
@@ -1318,20 +1340,10 @@ __device__ __forceinline__ void input_tile(const GradArgs& p, int L, char* lds) 
     const int k0 = s * p.kPerSplit, k1 = min(p.Kv, k0 + p.kPerSplit);
     Acc<4> acc;
     const unsigned char* levels = wave < 2 && !p.allNear && __builtin_amdgcn_readfirstlane(*p.anyLevel) ? p.levels + ((size_t)(tn * 2 + wave) * p.Kv + k0) * 32 : nullptr;
-    const CarryScale carry(p.classExp + k0, k1 - k0, levels, p.near);
+    float* out = p.slabs + ((size_t)s * p.Dp + td * TILE + wn * 64 + c) * p.Np + tn * TILE + wm * 64 + g * 4;
+    const CarryScale carry(out, p.Np, p.first, p.classExp + k0, k1 - k0, levels, p.near);
     turned_tile<SHARED>(p.dz + (p.allNear ? p.near : 0) + (size_t)tn * 8 * row, row, p.wByClass + (size_t)td * 4 * PAIR, (size_t)p.Kd * PAIR, k0, k1, lds, acc, carry);
-    const int e = carry.cur == EXP_ZERO ? 0 : -(carry.cur + DZ_EXP);
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int d = td * TILE + wn * 64 + j * 16 + c, n = tn * TILE + wm * 64 + i * 16 + g * 4;
-            f32x4* out = reinterpret_cast<f32x4*>(p.slabs + ((size_t)s * p.Dp + d) * p.Np + n);
-            f32x4 y;
-#pragma unroll
-            for (int r = 0; r < 4; r++) y[r] = ldexpf(acc.value(i, j, r), e);
-            *out = p.first ? y : *out + y;
-        }
+    carry.put(acc);
 }
 
 // ---- both gradients of a piece in one launch: they wait for the same logits and not for each other.  512 x 100000 x 1024: 579 us, 1087

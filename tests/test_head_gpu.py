@@ -716,6 +716,32 @@ def test_fc_logreg_weights_of_very_different_sizes(n, large, tiny):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('n', [6, 140])
+@pytest.mark.parametrize('sizes', [(1e30, 1e-20), (1e-20, 1e30), (1e-37, 1e8, 1e-30, 1e30, 1, 1e-12, 1e-37, 1e30), (2.0 ** 49, 1e-25)])
+def test_fc_logreg_weights_of_any_sizes_stay_in_range(sizes, n):
+    """Groups of classes whose weights differ by up to 2^220, in both orders: the sum over the classes is neither infinite nor lost."""
+    d, v = 40, 64 * len(sizes)
+    w, x, b, lab = fcl_data(d, v, n, 38, lean=0)
+    rng = np.random.default_rng(39)
+    w *= np.repeat(np.float32(sizes), 64)[:, None]
+    x /= np.float32(max(sizes))
+    ref = fcl_ref(w, x, b, lab, 0.5)
+    st, lp, ok, dx, dw, db, _ = fcl_run(w, x, b, lab, 0.5)
+    check_forward(ref, st, lp, ok)
+    for got, k in ((dx, 'dx'), (db, 'db')):
+        within(got, ref[k], ref['e' + k], k)
+    within(dw, ref['dw'], ref['edw'] + 2.0 ** -126, 'dw')  # (products down to 1e-38: what is below the smallest normal number may be zero)
+    # and where the large classes are out, by a bias of -inf or by one that leaves no probability: the small ones' sum and nothing else
+    large = np.repeat(np.float32(sizes), 64) >= 1
+    lab2 = rng.choice(np.flatnonzero(~large), n).astype(np.float32)
+    for out in (-np.inf, -1000):
+        b2 = np.where(large, np.float32(out), b)
+        ref = fcl_ref(np.where(np.isneginf(b2)[:, None], 0, w), x, b2, lab2, 0.5)
+        dx = fcl_run(w, x, b2, lab2, 0.5)[3]
+        within(dx, ref['dx'], ref['edx'] + 2.0 ** -126, 'dx of small weights')
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('d,v,n', [(36, 500, 6), (36, 500, 64), (40, 33000, 20), (40, 700, 140), (160, 10575, 509), (96, 10575, 509), (300, 70000, 70), (64, 3000, 1025), (20, 300, 4500)])
 def test_fc_logreg_classes_that_no_case_comes_near(d, v, n):
     """Probabilities from 1 down to 2^-90: every class's weight gradient is right relative to itself, beside labels' classes and others, and
