@@ -610,7 +610,11 @@ int mcn_counter_add(uint64_t* counter, uint64_t by, void* stream);
  *   costOut (device doubles, may be NULL): [0] += -sum(labelLogProbs), [1] += cases that count - sum(correctProbs).
  * Infinite weights and inputs go by the formula, whatever the number of cases: a logit of -inf takes its class out of that case.  A case
  * all of whose classes are at -inf has statistics (-inf, 0), log probability -inf and no gradient.  What the weights of a class
- * that is taken out hold, or the inputs of a case that does not count, comes through nowhere, except for such a case's own statistics.
+ * that is taken out hold, or the inputs of a case that does not count, comes through nowhere, except for such a case's own statistics,
+ * and for the input gradient of a case that has such a class for its label (and others left): the formula's weights[label] is in it.
+ * Operands of at most 64 cases' logits are taken in fp32; else, and for both gradients' products, as two 16-bit pieces under a scale in
+ * common: the weights of 32 neighbouring classes, the inputs of a case (for weightGrads: of a feature), 22 bits, an entry far below the
+ * largest of its group off by at most 2^-43 of that one.  All sums are fp32.
  * numOutputs from 1 to 2^24 (labels are fp32), numInputs and numCases to 2^20, numInputs * numCases to 2^34.  No output overlaps an operand
  * or another output (MCN_EINVAL).  Workspaces as for mcn_layer_norm; backward != 0: for both calls, 0: the cost alone. */
 size_t mcn_fc_logreg_workspace_bytes(int numInputs, int numOutputs, int numCases, int backward);
@@ -622,7 +626,9 @@ int mcn_fc_logreg_cost(const float* weights, const float* inputs, const float* b
  * (not all of them) and none may overlap an operand or another output:
  *   inputGrads (numInputs, numCases) = scaleInputTargets*inputGrads + weights^T dz,
  *   weightGrads (as weights) = scaleWeightTargets*weightGrads + scaleWeightOutput * dz inputs^T,
- *   biasGrads (numOutputs) = scaleBiasTargets*biasGrads + scaleBiasOutput * (row sums of dz). */
+ *   biasGrads (numOutputs) = scaleBiasTargets*biasGrads + scaleBiasOutput * (row sums of dz).
+ * dz / coeff is held to 22 bits: in weightGrads, where all of a class in 64 neighbouring cases is small, down to 2^-102 (fewer to 2^-124); in
+ * inputGrads, and beside larger ones, down to 2^-28 (fewer to 2^-50). */
 int mcn_fc_logreg_grad(const float* weights, const float* inputs, const float* biases, const float* labels, const float* caseStats,
                        float* inputGrads, float* weightGrads, float* biasGrads, int numInputs, int numOutputs, int numCases,
                        float coeff, float scaleInputTargets, float scaleWeightTargets, float scaleWeightOutput,
