@@ -13,7 +13,10 @@ namespace {
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // (16-byte accesses at any multiple of four bytes)
 
 constexpr int NARROW = 64;  // k_fcl_narrow: most cases
-constexpr int PIECE_MB = 192;  // fragments of a piece; 512 x 100000 x 1024, both calls: 128 MB 1.52 ms, 160 MB 1.50 ms, 192 MB 1.41 ms, 256 MB 1.48 ms
+// Fragments of a piece, the most MB.  Both calls at 96 / 128 / 160 / 192 / 256 MB, ms: 512 x 100000 x 1024 1.51 / 1.52 / 1.52 / 1.44 / 1.49,
+// 1024 x 50000 x 1024 1.51 / 1.46 / 1.42 / 1.39 / 1.41, 160 x 300000 x 512 1.49 / 1.51 / 1.46 / 1.44 / 1.46, 512 x 60000 x 2048 1.84 / 1.65 /
+// 1.60 / 1.60 / 1.65, 512 x 200000 x 512 1.90 / 1.71 / 1.74 / 1.69 / 1.66; 2048 x 60000 x 256 alone would have 256: 1.65 / 1.50 / 1.60 / 1.50 / 1.37.
+constexpr int PIECE_MB = 192;
 
 struct NarrowArgs {
     const float *W, *X, *bias, *labels;
@@ -1426,7 +1429,8 @@ WidePlan wide_plan(int D, int V, int N, bool bwd) {
     p.Dp = p.dTiles * TILE;
     p.Kn = p.Np / 32;
     // a piece's fragments should stay in the 256 MB last-level cache between the launches that write and read them; whole rounds of
-    // shared tiles where the classes fill some; a rest of at most a quarter goes with the last piece
+    // shared tiles where the classes fill some; a rest of at most a quarter goes with the last piece (with it / a piece of its own, ms:
+    // 512 x 100000 x 1024 1.44 / 1.46, 160 x 100000 x 1024 0.81 / 0.82, cost of 2048 x 100000 x 256 0.80 / 0.83, 512 x 100000 x 512 0.88 / 0.87)
     const size_t perRow = (size_t)p.Kd * 128 + (bwd ? (size_t)p.Np * 4 : 0);
     const int most = (int)std::max<size_t>(TILE, std::min<size_t>(((size_t)PIECE_MB << 20) / perRow / TILE * TILE, (size_t)1 << 17));
     const int round = std::max(1, 512 / p.nTiles) * TILE;
