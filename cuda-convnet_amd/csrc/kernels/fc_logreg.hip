@@ -102,8 +102,8 @@ __device__ __forceinline__ float exp_neg(float x) {
 // Few cases (at most 16 NB): bound by reading W once, so fp32 matrix instructions do, straight from the operands' own layouts.  A block
 // takes 16 RG classes, its four waves a quarter of the features each (16 at a time: a lane reads 16 bytes of its class's row, and the
 // four matrix instructions that follow take one feature of every lane's four); their sums are joined in LDS.  RG = 1 while the classes
-// do not fill the chip, 4 beyond, where it keeps the number of tiles to join down.  160 x 4213, one case: 4.4 us and 5.4 us to join, bound
-// by two launches; 512 x 100000, 16 cases: 56 us with the join, 3.7 TB/s.
+// do not fill the chip, 4 beyond, where it keeps the number of tiles to join down.  160 x 4213, one case: 4.4 us and 5.2 us to join, bound
+// by two launches; 512 x 100000, 16 cases: 42 us (4.9 TB/s) and 14 us to join.
 // Backward, the logits are computed again in the same way, and so to the same bits: where a case is all but certain, 1 - p of its label
 // is a difference that other roundings of z would drown.
 template <bool BWD, int NB, int RG>
@@ -255,8 +255,8 @@ __global__ __launch_bounds__(256) void k_fcl_narrow(NarrowArgs p) {
 }
 
 // Joins the tiles of every case: 16 cases x 64 tile lanes per block; first the max, then the sums, so that no exponential waits for
-// another.  A lane asks for all of its first eight tiles at once and keeps them (up to 512 tiles: one trip to memory, 5.4-6.4 us; 100000
-// classes x 1024 cases, 800 tiles: 12.8 us).
+// another.  A lane asks for all of its first eight tiles at once and keeps them (up to 512 tiles: one trip to memory, 5.2-6.3 us; 100000
+// classes x 1024 cases, 800 tiles: 12.6 us).
 __global__ __launch_bounds__(1024) void k_fcl_join(const float* __restrict__ part, const float* __restrict__ labelLogits,
                                                    const float* __restrict__ labels, float* __restrict__ caseStats, float* __restrict__ logProbs,
                                                    float* __restrict__ correct, int V, int N, int tiles) {
@@ -663,8 +663,8 @@ struct PackArgs {
     int rows, Kv;
 };
 
-// Bound by memory: W is read once and written once, as two pieces of 16 bits (10575 x 512: 13 us, 3.3 TB/s; 100000 x 512, one call: 83 us,
-// 5.0 TB/s).  Each block finds its rows' largest magnitudes first; what it reads then comes from its caches.
+// Bound by memory: W is read once and written once, as two pieces of 16 bits (10575 x 512: 12.4 us, 3.5 TB/s; 100000 x 512, one call: 89 us,
+// 4.6 TB/s).  Each block finds its rows' largest magnitudes first; what it reads then comes from its caches.
 __device__ __forceinline__ void pack_cases(const PackArgs& p, int block, float* sh, int* exps) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4, n = block * 16 + c;
     float m = 0.f;
@@ -901,8 +901,8 @@ __device__ __forceinline__ void odd_logits(LateArgs p, float* z, int vFirst, int
     }
 }
 
-// SHARED: two blocks per CU (MB = 4).  512 x 100000 x 1024: forward 346 us, 909 TFLOP/s of fp16 products, backward, which writes dz,
-// 393 us, 800; a large library product of fp16 operands reaches 1126.
+// SHARED: two blocks per CU (MB = 4).  512 x 100000 x 1024: forward 328 us, 959 TFLOP/s of fp16 products, backward, which writes dz,
+// 387 us, 813; a large library product of fp16 operands reaches 1126.
 template <int MB, bool BWD, bool SHARED>
 __global__ __launch_bounds__(256, SHARED ? 2 : 1) void k_fcl_logits(WideArgs p) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -1349,8 +1349,8 @@ __device__ __forceinline__ void input_tile(const GradArgs& p, int L, char* lds) 
     carry.put(acc);
 }
 
-// ---- both gradients of a piece in one launch: they wait for the same logits and not for each other.  512 x 100000 x 1024: 579 us, 1087
-// TFLOP/s of fp16 products; 512 x 10575 x 128: 17.5 us.
+// ---- both gradients of a piece in one launch: they wait for the same logits and not for each other.  512 x 100000 x 1024: 568 us, 1108
+// TFLOP/s of fp16 products; 512 x 10575 x 128: 16.3 us.
 template <bool SHARED>
 __global__ __launch_bounds__(256, SHARED ? 2 : 1) void k_fcl_grads(GradArgs p) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -1414,7 +1414,7 @@ struct WidePlan {
 };
 // When the packed operands pay for the logits (us of a whole cost call, narrow / wide).  512 x 10575: 16 cases 16 / 34, 64 cases 26 / 35;
 // 512 x 100000: 56 / 145, 121 / 147.  Both calls go by the number of cases alone: the gradients' logits are the cost's, to the bit.
-// The other products of the gradients always take them (512 x 10575: one case 50 us, 16 cases 43 us, 64 cases 49 us).
+// The other products of the gradients always take them (512 x 10575: one case 50 us, 16 cases 43 us, 64 cases 51 us).
 bool wide_cost_usable(int N) { return N > NARROW; }
 
 size_t al256(size_t b) { return (b + 255) / 256 * 256; }
@@ -1466,7 +1466,8 @@ WidePlan wide_plan(int D, int V, int N, bool bwd) {
 }
 
 // RG of k_fcl_narrow.  Forward, 1 / 4 (us of a cost call, 512 features, 16 cases): 10575 classes 16 / 18, 20000 24 / 22, 100000 86 / 53.
-// Backward nothing is joined, and only the reads of x are fewer (gradients, 64 cases): 20000 classes 79 / 83, 100000 383 / 365.
+// Backward nothing is joined, and only the reads of x are fewer (gradients, 64 cases): 10575 classes 50 / 56, 20000 81 / 85, 40000 158 / 160,
+// 100000 411 / 397.
 int narrow_groups(int rows, bool bwd) { return rows > (bwd ? 32 : 16) * 1024 ? 4 : 1; }
 int narrow_tiles(int rows) { return divup(rows, 16 * narrow_groups(rows, false)); }
 // blocks: narrow_tiles(rows) forward, all of the piece's packed classes backward

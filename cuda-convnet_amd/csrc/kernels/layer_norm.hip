@@ -104,7 +104,7 @@ __device__ __forceinline__ void sum_rows(float (&v)[NV], int cl, int logLanes, f
 }
 
 // ---- forward, a block holds all rows of its columns in registers (R a thread): one read, the variance from exact deviations.
-// 512 x 1: 3.0 us, 512 x 128: 5.4 us, 1024 x 16384: 22.6 us (134 MB in all, the input from the last-level cache).
+// 512 x 1: 2.8 us, 512 x 128: 5.3 us, 1024 x 16384: 22.9 us (134 MB in all, the input from the last-level cache).
 template <int VW, int R>
 __global__ __launch_bounds__(T_WHOLE) void k_ln_whole(const float* x, const float* __restrict__ gain, const float* __restrict__ bias, float* y,
                                                       float* __restrict__ caseStats, float eps, int F, int N, int logLanes, int tiles) {
@@ -198,7 +198,7 @@ __device__ __forceinline__ void row_sums_block(const float* g, const float* x, c
 }
 
 // ---- backward, the same way: both matrices in registers.  A block goes through its tiles one after the other with its rows fixed, so
-// the row sums for gains and biases stay in registers too and leave once per block: rowPart[block][2][F].  512 x 128: 4.4 us.
+// the row sums for gains and biases stay in registers too and leave once per block: rowPart[block][2][F].  512 x 128: 4.7 us.
 template <int VW, int R>
 __global__ __launch_bounds__(T_WHOLE) void k_ln_undo_whole(const float* g, const float* x, const float* __restrict__ gain,
                                                      const float* __restrict__ caseStats, float* target, float* __restrict__ rowPart,
@@ -280,8 +280,9 @@ __global__ __launch_bounds__(T_WHOLE) void k_ln_undo_whole(const float* g, const
 }
 
 // ---- more rows than a block's registers hold: ranges of rows, joined by a second launch that reads the matrices again.
-// 4096 x 16384 (268 MB a matrix): sums 67 us (4.0 TB/s), apply 101 us (5.3 TB/s); backward 132 us (4.1 TB/s) and 145 us (5.5 TB/s).  A copy
-// reaches 5.2 TB/s.  4213 x 509: 4.7 + 8.2 and 7.2 + 8.4 us, bound by the launches.
+// 4096 x 16384 (268 MB a matrix): sums 67 us (4.0 TB/s), apply 89 us (6.0 TB/s, part of it from the last-level cache); backward 137 us (3.9
+// TB/s) and 146 us (5.5 TB/s).  A copy reaches 5.2 TB/s.  4213 x 509: 4.7 + 8.2 and 7.4 + 8.5 us; the apply launches' 512 blocks each read the
+// partial sums of all 64 ranges, 16.8 MB a launch, as much as the matrix there.
 struct Split {
     int F, N, logLanes, colTiles, splits, rowsPerSplit;
 };

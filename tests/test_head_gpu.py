@@ -766,6 +766,42 @@ def test_fc_logreg_classes_that_no_case_comes_near(d, v, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('d,v,n', [(36, 500, 64), (40, 700, 140), (160, 10575, 509)])
+def test_fc_logreg_nothing_of_an_earlier_call_stays(d, v, n):
+    """One workspace, eager and in a replayed graph: classes far from every case, then near ones, then far again -- the bits of a workspace of
+    one's own."""
+    w, x, b, lab = fcl_data(d, v, n, 47)
+    far = np.where(np.arange(v) % 2, np.float32(-30), np.float32(0))
+    lab = np.floor(lab / 2) * 2  # (classes at 0)
+    ws, size = need('mcn_fc_logreg_workspace_bytes', d, v, n, 1)
+    kw, kx, kl, kb = dev(w), dev(x), dev(lab), dev(b)
+    outs = [Out(s) for s in ((2, n), (n,), (n,), (d, n), (v, d), (v,))]
+    stream = C.c_void_p()
+    call('mcn_stream_create', C.byref(stream))
+
+    def step():
+        call('mcn_fc_logreg_cost', kw, kx, kb, kl, *outs[:3], d, v, n, None, ws, size, stream)
+        call('mcn_fc_logreg_grad', kw, kx, kb, kl, outs[0], *outs[3:], d, v, n, 0.5, 0.0, 0.0, 1.0, 0.0, 1.0, ws, size, stream)
+
+    want = {False: fcl_run(w, x, b, lab, 0.5), True: fcl_run(w, x, b + far, lab, 0.5)}
+    step()
+    exe = C.c_void_p()
+    call('mcn_stream_sync', stream)
+    call('mcn_graph_begin_capture', stream)
+    step()
+    call('mcn_graph_end_capture', stream, C.byref(exe), None)
+    for k, distant in enumerate((True, False, True, True, False, False, True)):
+        kb.upload(b + far if distant else b)
+        call('mcn_device_sync')
+        call('mcn_graph_launch', exe, stream) if k % 3 else step()
+        call('mcn_stream_sync', stream)
+        for o, a in zip(outs, want[distant]):
+            assert np.array_equal(o.get(), a), k
+    call('mcn_graph_destroy', exe)
+    call('mcn_stream_destroy', stream)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('d,v,n', [(12, 30, 9), (40, 150, 66)])
 def test_fc_logreg_gradient_against_differences(d, v, n):
     """d sum(log p) along random directions (central differences of the float64 formula, step 1e-4: 1e-6 of the magnitudes)."""
