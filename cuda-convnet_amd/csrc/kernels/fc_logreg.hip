@@ -877,27 +877,51 @@ struct WideArgs {
 
 // Logits whose weights or inputs hold an infinity or NaN: the products of pieces make a NaN of any of them, where the formula has the sum
 // of the terms that are not finite (all of one sign: that infinity).  Where an infinite input meets the zeros of a class that is taken
-// out, too.  Rare: a lane's entries lie in LDS, 256 floats apart, and are gone through one by one.
+// out, too.  Rare: a lane's entries lie in LDS, 256 floats apart; a lane looks for such operands at one of 64 features, and the features that
+// have some are gone through one by one.
 typedef const __attribute__((address_space(4))) WideArgs* LateArgs;
 template <int MB>
-__device__ __forceinline__ void odd_logits(LateArgs p, float* z, int vFirst, int nFirst) {
+__device__ __forceinline__ void odd_logits(LateArgs p, float* z, int vBase, int nBase, int lane) {
+    constexpr unsigned NOTHING_YET = 0x7FC0BEEFu;  // (a NaN, which it stays if no term turns up)
+    const int vFirst = vBase + (lane >> 4) * 4, nFirst = nBase + (lane & 15), D = p->D, N = p->N, rows = p->rows;
+    const float *W = p->W + (size_t)p->v0 * D, *X = p->X, *bias = p->bias ? p->bias + p->v0 : nullptr;
+    auto class_of = [&](int e) { return vFirst + (e >> 4) * 16 + (e & 3); };
+    auto case_of = [&](int e) { return nFirst + ((e >> 2) & 3) * 16; };
+    auto bias_of = [&](int v) { return v < rows ? (bias ? bias[v] : 0.f) : -INFINITY; };
 #pragma unroll 1
-    for (int e = 0; e < 16 * MB; e++, z += 256) {
-        const int v = vFirst + (e >> 4) * 16 + (e & 3), n = nFirst + ((e >> 2) & 3) * 16;
-        const float bv = v < p->rows ? (p->bias ? p->bias[p->v0 + v] : 0.f) : -INFINITY;
-        const float was = *z;
-        const bool look = n < p->N && bv != -INFINITY && was != was;
-        if (bv == -INFINITY) *z = -INFINITY;
-        if (!__any(look)) continue;
-        float s = 0.f;
-        const float *w = p->W + (size_t)(p->v0 + v) * p->D, *x = p->X + n;
-        for (int d = 0; d < p->D && __any(look && s == s); d++) {
-            if (look) {
-                const float a = w[d], b = x[(size_t)d * p->N];
-                if (!(fabsf(a) < INFINITY && fabsf(b) < INFINITY)) s += a * b;
-            }
+    for (int e = 0; e < 16 * MB; e++) {
+        const float was = z[e * 256];
+        if (bias_of(class_of(e)) == -INFINITY) z[e * 256] = -INFINITY;
+        else if (case_of(e) < N && was != was) z[e * 256] = __uint_as_float(NOTHING_YET);
+    }
+#pragma unroll 1
+    for (int d0 = 0; d0 < D; d0 += 64) {
+        float none = 0.f;  // a NaN once there is one
+        if (d0 + lane < D) {
+#pragma unroll 8
+            for (int v = vBase; v < min(rows, vBase + 16 * MB); v++) none = fmaf(W[(size_t)v * D + d0 + lane], 0.f, none);
+#pragma unroll 8
+            for (int n = nBase; n < min(N, nBase + 64); n++) none = fmaf(X[(size_t)(d0 + lane) * N + n], 0.f, none);
         }
-        if (look && s != 0.f) *z = s + bv;
+        unsigned long long odd = __ballot(none != 0.f);
+        for (; odd; odd &= odd - 1) {
+            const int d = d0 + __builtin_ctzll(odd);
+            bool open = false;  // whether a further term can change anything: not where there is a NaN
+#pragma unroll 1
+            for (int e = 0; e < 16 * MB; e++) {
+                const int v = class_of(e), n = case_of(e);
+                const float b = bias_of(v);
+                if (n >= N || b == -INFINITY) continue;
+                const float w = W[(size_t)v * D + d], x = X[(size_t)d * N + n];
+                float sum = z[e * 256];
+                if (!(fabsf(w) < INFINITY && fabsf(x) < INFINITY)) {
+                    sum = __float_as_uint(sum) == NOTHING_YET ? w * x + b : sum + w * x;
+                    z[e * 256] = sum;
+                }
+                open |= __float_as_uint(sum) == NOTHING_YET || fabsf(sum) == INFINITY;
+            }
+            if (!__any(open)) return;
+        }
     }
 }
 
@@ -953,7 +977,7 @@ __global__ __launch_bounds__(256, SHARED ? 2 : 1) void k_fcl_logits(WideArgs p) 
         // arguments that only this branch needs are loaded in it: with their loads moved to the front 512 x 10575, 509 cases, took 28.5 us for 24.1
         LateArgs late = (LateArgs)__builtin_amdgcn_kernarg_segment_ptr();
         asm volatile("" : "+s"(late));
-        odd_logits<MB>(late, mine, vBase + g * 4, nBase + c);
+        odd_logits<MB>(late, mine, vBase, nBase, lane);
 #pragma unroll
         for (int k = 0; k < 16 * MB; k++) acc.c[0][k >> 4][(k >> 2) & 3][k & 3] = mine[k * 256];
     }

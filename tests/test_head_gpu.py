@@ -657,6 +657,26 @@ def test_fc_logreg_infinities_that_leave_no_number(n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('n', [6, 70, 300])
+def test_fc_logreg_infinite_weights_far_apart(n):
+    """Infinities of one sign, and of both, at features far from each other; a NaN behind an infinity."""
+    d, v = 700, 300
+    w, x, b, lab = fcl_data(d, v, n, 46)
+    for k in (3, 500, 699):
+        x[k] = np.abs(x[k]) + 0.1
+    lab[np.isin(lab, (50, 60, 70))] = 1
+    out, b0, w0 = [50], b.copy(), w.copy()
+    b0[out], w0[out] = -np.inf, 0
+    w[50, [3, 500, 699]] = -np.inf
+    fcl_check(fcl_ref(w0, x, b0, lab, 0.5), fcl_run(w, x, b, lab, 0.5), slice(None), np.array([k for k in range(d) if k not in (3, 500, 699)]))
+    for row, at, vals in ((60, [3, 699], [-np.inf, np.inf]), (60, [500, 699], [np.inf, -np.inf]), (70, [3, 500], [-np.inf, np.nan]), (70, [3, 500], [np.nan, -np.inf])):
+        w2 = w.copy()
+        w2[row, at] = vals
+        st, lp, *_ = fcl_run(w2, x, b, lab)
+        assert np.isnan(lp).all() and np.isnan(st[1]).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('n', [6, 140])
 def test_fc_logreg_infinite_inputs(n):
     """An input of +inf against negative weights takes every class out: the case has statistics (-inf, 0) and no gradient, and the others
