@@ -354,8 +354,9 @@ __global__ __launch_bounds__(256) void k_fcl_cost(const float* __restrict__ labe
 // Many cases: the three products on fp16 matrix instructions with fp32 accuracy.  fp32 matrix instructions reach 157 TFLOP/s, fp16 ones
 // 2500: an fp32 operand, scaled by a power of two, is split into y = hi + 2^-11 lo with 11 bits each; the products of pieces are exact in
 // fp32, and hi hi, hi lo and lo hi are summed (3 instructions), the cross terms in an accumulator of their own, so that lo keeps its
-// bits.  With the largest magnitude of a scaled group below 2^15 the relative error of a product is about 2^-22 for entries down to
-// 2^-21 of the group's largest, and an entry further down is off by at most 2^-43 of it.  The groups: a case's features for the
+// bits.  With the largest magnitude of a scaled group below 2^15 the relative error of a product is at most 2^-21 (2^-23 of either operand and
+// lo lo, which is left out, 2^-22; 2^-24 in the mean square) for entries down to 2^-21 of the group's largest, and an entry further down is off
+// by at most 2^-43 of it.  The groups: a case's features for the
 // logits, a feature's cases for the weight gradient, 32 classes' weights, and for dz / coeff a class over 64 cases in the weight gradient
 // (levels, above) and all of it in the input gradient, where the label's entry, 1 - p, is off by 2^-25 anyway.  Along the summed dimension
 // a group is either whole or its scale is carried along (CarryScale, CarryLevels), so a row of large weights takes no bits from the
